@@ -572,6 +572,77 @@ int rivoli_v4_token_step_bf16(const V4Geom* g, int n_seqs, const int32_t* pos, c
 /* Synchronises the stream; 1008 if a bounded wait of the tensor-core block scorer gave up since the last call. */
 int rivoli_v4_select_status(void* stream);
 
+/* ---- drafted tokens: several new tokens of a sequence in one step ------------------------------------------------------
+ * No counterpart in the reference, whose decode step takes one token (crates/engine/src/glm/decode.rs:128-165). A host that drafts
+ * T tokens of a sequence ahead of its model does, per step: the projections of all T rows (rivoli_rope_rows_bf16 for their positions),
+ * per layer rivoli_kv_append_paged of the rows at positions tree_pos + j and rivoli_mla_tree_attend_paged_bf16, then
+ * rivoli_draft_verify on the probabilities, and rivoli_kv_commit_paged of what was accepted. Node 0 of a sequence's tree is the token
+ * that was decided last (its row is not in the cache yet); every other node hangs below a node of a smaller index. Nodes of all
+ * sequences are packed: those of sequence b are node_start[b] .. node_start[b + 1) (i32 [B + 1], on the device), at most 64.
+ *
+ * Rotary positions of bf16 rows. Of every vector `seg` values at src are rotated by the angles pos[row] * inv_freq[i] (f64,
+ * i < seg / 2; remainders by a turn in f64), multiplied by `scale`, rounded once and stored at dst. Layouts: ADJACENT pairs
+ * (2i, 2i+1) in place; HALF pairs (i, i + seg/2) in place; SPLIT pairs (2i, 2i+1) to (i, i + seg/2), the order of
+ * rivoli_rope_interleave (crates/backend/kernels/activation.hip:362-371). Strides in elements, any sign. dst may be src with the same
+ * strides (in place); otherwise the two must not overlap. k may be NULL. Segments of a multiple of 16 values whose bases and strides
+ * are multiples of 16 bytes are read and written 16 bytes at a time.
+ * 1001 nulls or sizes; 1002 seg > 512 or n_vec > 65536; 1003 layout; 1004 odd seg; 1005 odd addresses. */
+enum { RV_ROPE_ADJACENT = 0, RV_ROPE_HALF = 1, RV_ROPE_SPLIT = 2 };
+typedef struct RopeVecs {                  /* vectors of a row: where their segments are read and written */
+    const uint16_t* src; uint16_t* dst;
+    int64_t src_row, src_vec, dst_row, dst_vec;
+    int32_t n_vec;
+} RopeVecs;
+int rivoli_rope_rows_bf16(const RopeVecs* q, const RopeVecs* k, int n_rows, const int32_t* pos, const double* inv_freq, int seg,
+                          int layout, float scale, void* stream);
+
+/* Attention of all nodes of all trees: q bf16 [n_nodes][n_heads][kv_lora + rope_dim], out bf16 [n_nodes][n_heads][kv_lora], out_lse
+ * f32 [n_nodes][n_heads] (may be NULL). A node of sequence b sees n_rows[b] rows of the prefix - rows u32 [B][row_stride], one list for
+ * the whole tree (its root's selection, say), or with rows NULL the first n_rows[b] tokens, n_rows NULL meaning tree_pos[b] of them;
+ * a list that begins with the dense marker 0xFFFFFFFF stands for the first n_rows[b] tokens - and node i of its own tree, whose row is
+ * token tree_pos[b] + i, where bit i of node_mask (u64 [n_nodes]) is up: for a tree its ancestors and itself. A node that sees nothing
+ * gets zeros and -inf. Rows on unmapped pages are seen by nobody. Outputs of nodes from node_start[B] on, and of a sequence's nodes
+ * behind its 64th, are left as they were. scratch = rivoli_mla_tree_attend_scratch_bytes(), zeroed once (it begins with a sticky error
+ * word); calls that may run at the same time need one each. kv_lora 512 with rope_dim 64 runs on the tensor cores for any number of
+ * heads (given scratch), other geometries on CUDA cores. Which rows share a block goes by the whole call, so that the last bits of a
+ * node's output may differ between batches; the same call gives the same bits.
+ * 1001 nulls or sizes; 1002 n_nodes * n_heads or the pool too large; 1003-1004 geometry; 1005 alignment. */
+size_t rivoli_mla_tree_attend_scratch_bytes(const DsaGeom* g, int B, int n_nodes);
+int rivoli_mla_tree_attend_paged_bf16(const DsaGeom* g, const uint16_t* q, const uint8_t* latent_pool, const float* latent_scale,
+                                      const int32_t* block_table, const uint32_t* rows, int row_stride, const int32_t* n_rows,
+                                      const int32_t* tree_pos, const int32_t* node_start, const uint64_t* node_mask, int B,
+                                      int n_nodes, uint16_t* out, float* out_lse, void* scratch, void* stream);
+/* Synchronises `stream`; 1008 if a bounded wait of the tensor-core form gave up since the last call on this scratch (output
+ * undefined), else 0. */
+int rivoli_mla_tree_attend_status(const DsaGeom* g, void* scratch, void* stream);
+
+/* Drafted tokens held against the target's probabilities. target: rows of `vocab` probabilities, one per node (row of node i: what
+ * follows node i), f32 (prob_bits 32) or bf16 (16), row stride in elements; draft the same from the draft model, or NULL for tokens
+ * that were chosen and not drawn. u f32 [n_nodes], u_next f32 [B]: random numbers in [0, 1). From node 0 on, with r = the target's row
+ * of the current node: its children in the order of their indices; child x is accepted if u[x] * q(token[x]) < r(token[x]), q = the draft's row of the
+ * current node (draft NULL: u[x] < r(token[x])), and becomes the current node; if not, r <- max(r - q, 0) / sum (draft NULL: r without
+ * token[x], / sum). The next token is the first v with r(0) + .. + r(v) > u_next[b] * sum r, the last with r(v) > 0 if none. If nothing
+ * is left of r the remaining children are refused and the next token is drawn from the target's own row; -1 if that holds nothing.
+ * Probabilities that are negative, infinite or NaN count as 0, and so does a token outside the vocabulary; a parent that is not an
+ * earlier node is nobody's. Sums and comparisons in f64. path i32 [B][max_path]: the accepted nodes, ascending, from node 0 on, n_path[b]
+ * of them (entries behind are left alone; once max_path are accepted no further child is tried); next i32 [B]. A sequence without nodes:
+ * n_path 0, next -1. 1001 nulls or sizes; 1002 vocab > 2^20, max_path > 64; 1004 prob_bits; 1005 strides below vocab, alignment. */
+int rivoli_draft_verify(const int32_t* node_start, const int32_t* parent, const int32_t* token, const void* target,
+                        long long target_stride, const void* draft, long long draft_stride, int prob_bits, int vocab, const float* u,
+                        const float* u_next, int B, int32_t* path, int max_path, int32_t* n_path, int32_t* next, void* stream);
+
+/* What was accepted becomes the sequence: the pool rows of positions tree_pos[b] + path[b][k], k < n_path[b] (at most path_stride), move
+ * to positions tree_pos[b] + k, codes and scales of latents and indexer keys, in n_layers layers (a device array; index_pool NULL: a
+ * layer without an indexer) that share block_table. seq_len (i32 [B], may be NULL, not tree_pos itself) receives tree_pos + n_path.
+ * The paths are what rivoli_draft_verify writes: strictly ascending, path[b][k] >= k. A sequence whose path is not, or whose rows lie
+ * on unmapped pages, is left as it is, seq_len included, and raises bit 0 of *status (device i32, may be NULL). Rows behind the path
+ * are left as they were. Sequences must not share the pages that their drafts lie on.
+ * 1001 nulls or sizes; 1002 path_stride > 64; 1003-1004 geometry; 1005 alignment, seq_len == tree_pos. */
+typedef struct CommitLayer { uint8_t* latent_pool; float* latent_scale; uint8_t* index_pool; float* index_scale; } CommitLayer;
+int rivoli_kv_commit_paged(const DsaGeom* g, const CommitLayer* layers, int n_layers, const int32_t* block_table,
+                           const int32_t* tree_pos, const int32_t* path, int path_stride, const int32_t* n_path, int B,
+                           int32_t* seq_len, int32_t* status, void* stream);
+
 /* ---- measurement hook ------------------------------------------------------------------------------------------
  * events[0..5): cudaEvent_t handles that the following rivoli_dsa_decode_step_paged / rivoli_dsa_append_select_paged
  * calls record on their stream: 0 before the prologue kernel (append + query preparation), 1 before the scorer,

@@ -95,6 +95,9 @@ _SIGNATURES = {
     "v4_token_step_bf16": "pi" + "p" * 14, "act_quant_f8_prefix": "ppiiiip", "kv_compress_deposit": "ppppppiip",
     "kv_compress_prefill": "pppppip", "kv_compress_decode": "ppppip",
     "v4_compress_step_bf16": "pi" + "p" * 8 + "ipiipppp",
+    "rope_rows_bf16": "ppippiifp", "mla_tree_attend_scratch_bytes": "pii",
+    "mla_tree_attend_paged_bf16": "ppppppippppiipppp", "mla_tree_attend_status": "ppp",
+    "draft_verify": "ppppqpqiippipippp", "kv_commit_paged": "ppipppipippp",
     "dsa_step_set_timing_events": "p", "attend_mma_test_hook": "iii", "index_select_test_cluster": "i", "kernels_arch": "",
 }
 _CTYPE = {"p": C.c_void_p, "i": C.c_int, "f": C.c_float, "d": C.c_double, "z": C.c_size_t, "q": C.c_longlong}
@@ -707,6 +710,97 @@ def launch_v4_compress_step_bf16(p: CompGeom, n_seqs: int, pos, kv_proj, score_p
         C.byref(p), n_seqs, _ptr(pos), _ptr(kv_proj), _ptr(score_proj), _ptr(ape), _ptr(kv_state),
         _ptr(score_state), _ptr(norm), _ptr(freqs), int(rotate), _ptr(cache), cache_rows,
         cache_row0, _ptr(prequant), _ptr(packed), _ptr(packed_exp), _stream(stream)), "v4_compress_step_bf16")
+
+
+# --- drafted tokens -----------------------------------------------------------------------------------
+ROPE_LAYOUTS = {"adjacent": 0, "half": 1, "split": 2}
+
+
+def rope_vecs(src, dst=None) -> tuple:
+    """The fields of ``RopeVecs`` (include/rivoli_kernels.h) for tensors ``[rows, vectors, seg]`` or ``[rows, seg]`` whose last axis is
+    contiguous: views of the rotated part of wider rows. ``dst`` None rotates in place."""
+    dst = src if dst is None else dst
+    if src.shape != dst.shape or src.dim() not in (2, 3):
+        raise ValueError(f"rope_vecs: shapes {tuple(src.shape)} and {tuple(dst.shape)}")
+    if src.element_size() != 2 or dst.element_size() != 2 or src.stride(-1) != 1 or dst.stride(-1) != 1:
+        raise ValueError("rope_vecs: bf16 tensors with a contiguous last axis")
+    if src.dim() == 2:
+        return src, dst, src.stride(0), 0, dst.stride(0), 0, 1
+    return src, dst, src.stride(0), src.stride(1), dst.stride(0), dst.stride(1), src.shape[1]
+
+
+def rope_frequencies(seg: int, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0, original: int = 4096,
+                     beta_fast: float = 32.0, beta_slow: float = 1.0):
+    """Angle per position of the ``seg / 2`` pairs (f64 array) and the factor of cosines and sines, for
+    ``launch_rope_rows_bf16``. ``scaling``: how positions past the ``original`` context are reached by ``factor``: "linear" divides all
+    frequencies; "ntk" raises theta so that the lowest frequency is divided and the highest kept; "yarn" divides the pairs that turn less
+    than ``beta_slow`` times over the original context, keeps those that turn more than ``beta_fast`` times, blends between, and
+    scales by 0.1 ln(factor) + 1."""
+    import numpy as np
+    if seg <= 0 or seg % 2 or theta <= 1 or factor < 1:
+        raise ValueError(f"rope_frequencies: seg {seg}, theta {theta}, factor {factor}")
+    if scaling == "ntk":
+        if seg < 4:
+            raise ValueError("rope_frequencies: ntk needs two pairs")
+        theta = theta * factor ** (seg / (seg - 2))
+    f, scale = np.float64(theta) ** (-np.arange(0, seg, 2, dtype=np.float64) / seg), 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        def pair_of(turns):     # the pair that turns so often over the original context
+            return seg * np.log(original / (turns * 2 * np.pi)) / (2 * np.log(theta))
+        low, high = max(np.floor(pair_of(beta_fast)), 0), min(np.ceil(pair_of(beta_slow)), seg - 1)
+        ramp = np.clip((np.arange(seg // 2) - low) / max(high - low, 1e-3), 0, 1)
+        f = f / factor * ramp + f * (1 - ramp)
+        scale = float(0.1 * np.log(factor) + 1.0)
+    elif scaling not in ("none", "ntk"):
+        raise ValueError(f"rope_frequencies: scaling {scaling!r}")
+    return f, scale
+
+
+def launch_rope_rows_bf16(q: tuple, k: "tuple | None", n_rows: int, pos, inv_freq, seg: int, layout: int, scale: float = 1.0,
+                          stream=None) -> None:
+    """Rotary positions of the vectors ``q`` and ``k`` (``rope_vecs``) of ``n_rows`` rows at positions ``pos``."""
+    ensure_status((_native or _launch()).rope_rows_bf16(q, k, n_rows, pos, inv_freq, seg, layout, scale, stream), "rope_rows_bf16")
+
+
+def mla_tree_attend_scratch_bytes(g: DsaGeom, B: int, n_nodes: int) -> int:
+    """Never 0, so that a tensor of this size has an address."""
+    return max(int(lib().rivoli_mla_tree_attend_scratch_bytes(C.byref(g), B, n_nodes)), 16)
+
+
+def launch_mla_tree_attend_paged_bf16(g: DsaGeom, q, latent_pool, latent_scale, block_table, rows, row_stride: int, n_rows, tree_pos,
+                                      node_start, node_mask, B: int, n_nodes: int, out, out_lse, scratch, stream=None) -> None:
+    """Attention of trees of drafted tokens over each sequence's prefix and its tree (``rivoli_mla_tree_attend_paged_bf16``)."""
+    ensure_status((_native or _launch()).mla_tree_attend_paged_bf16(g, q, latent_pool, latent_scale, block_table, rows, row_stride,
+        n_rows, tree_pos, node_start, node_mask, B, n_nodes, out, out_lse, scratch, stream), "mla_tree_attend_paged_bf16")
+
+
+def mla_tree_attend_status(g: DsaGeom, scratch, stream=None) -> None:
+    """Raises BackendError(1008) if a bounded wait of the tensor-core form gave up on this scratch (synchronises)."""
+    ensure_status(lib().rivoli_mla_tree_attend_status(C.byref(g), _ptr(scratch), _stream(stream)), "mla_tree_attend_status")
+
+
+def launch_draft_verify(node_start, parent, token, target, target_stride: int, draft, draft_stride: int, prob_bits: int, vocab: int,
+                        u, u_next, B: int, path, max_path: int, n_path, next_token, stream=None) -> None:
+    """Drafted tokens against the target's probabilities, and the token that follows (``rivoli_draft_verify``)."""
+    ensure_status((_native or _launch()).draft_verify(node_start, parent, token, target, target_stride, draft, draft_stride, prob_bits,
+        vocab, u, u_next, B, path, max_path, n_path, next_token, stream), "draft_verify")
+
+
+def commit_layers(layers):
+    """The device array of ``CommitLayer`` for tensors (latent pool, latent scales, index pool, index scales) of each layer; the last
+    two None for a layer without an indexer. It holds addresses: the tensors have to outlive it."""
+    import torch
+    words = [[_ptr(t) or 0 for t in layer] for layer in layers]
+    return torch.tensor(words, dtype=torch.int64, device=layers[0][0].device)
+
+
+def launch_kv_commit_paged(g: DsaGeom, layers, n_layers: int, block_table, tree_pos, path, path_stride: int, n_path, B: int,
+                           seq_len=None, status=None, stream=None) -> None:
+    """Cache rows of the accepted nodes to where the sequence goes on, in all layers (``rivoli_kv_commit_paged``)."""
+    ensure_status((_native or _launch()).kv_commit_paged(g, layers, n_layers, block_table, tree_pos, path, path_stride, n_path, B,
+        seq_len, status, stream), "kv_commit_paged")
 
 
 def kernels_arch() -> str:

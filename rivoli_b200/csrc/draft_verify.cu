@@ -1,0 +1,327 @@
+// Drafted tokens against the target's probabilities, with given random numbers, and the token that follows them.
+//
+// Node 0 of a sequence's tree is the token decided last. From there: the children of the current node are tried in the order of
+// their indices; with r the target's probabilities behind the current node (negative, infinite and NaN ones count as 0) and q the
+// draft's, child x is accepted if u[x] * q(token) < r(token), and the walk goes on from it. If it is not, what is left is
+//     r <- max(r - q, 0) / Z,   Z = sum max(r - q, 0)
+// (tokens that were chosen and not drawn, draft = NULL: q is 1 at the token and 0 elsewhere), so that the token that comes out is
+// distributed as the target says. Where no child is left the next token is the first v with r(0) + .. + r(v) > u_next * sum r, or the
+// last with r(v) > 0 if none; where nothing is left of r (Z = 0) the remaining children are refused and the target's own row is drawn
+// from; -1 if that is empty too.
+//
+// Every r in that chain is max(a p - b q, 0) with two numbers a and b: a rejection needs one pass over the rows (for Z), which also
+// leaves the sums by chunk that the draw needs, and nothing is written but the answer. Sums, products and comparisons are in 64 bits:
+// a draw next to a border has to come out the same whatever the order of summation.
+//
+// A cluster of blocks per sequence, each a contiguous part of the vocabulary; every block walks the tree itself (the few
+// probabilities that decide are gathered at once for all nodes), and only sums are exchanged, through distributed shared memory. Bound by memory: one
+// row of the target and one of the draft per sequence, a chunk of 2 KiB of each per warp and step.
+#include "codec.cuh"
+#include "common.cuh"
+
+namespace {
+
+constexpr int DV_THREADS = 512, DV_WARPS = DV_THREADS / 32;
+constexpr int DV_NODES = 64, DV_MAX_VOCAB = 1 << 20, DV_MAX_CLUSTER = 8;
+
+struct VerifyArgs {
+    const int32_t* node_start; const int32_t* parent; const int32_t* token;
+    const void* target; const void* draft;
+    long long target_stride, draft_stride;
+    int vocab, chunks;                   // chunks: of a block
+    const float* u; const float* u_next;
+    int32_t* path; int max_path; int32_t* n_path; int32_t* next;
+};
+
+__device__ __forceinline__ float clean(float x) { return x > 0.0f && x < INFINITY ? x : 0.0f; }
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void put_remote(double* mine, uint32_t rank, double v) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(v) : "memory");
+}
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+template <class T> struct Row;           // 16 bytes of probabilities
+template <> struct Row<float> {
+    static constexpr int PER = 4;
+    __device__ static float one(const float* p, long long i) { return clean(p[i]); }
+    __device__ static void unpack(const uint4 w, float* x) {
+        x[0] = clean(__uint_as_float(w.x)); x[1] = clean(__uint_as_float(w.y)); x[2] = clean(__uint_as_float(w.z)); x[3] = clean(__uint_as_float(w.w));
+    }
+};
+template <> struct Row<uint16_t> {
+    static constexpr int PER = 8;
+    __device__ static float one(const uint16_t* p, long long i) { return clean(rv_bf16_to_f32(p[i])); }
+    __device__ static void unpack(const uint4 w, float* x) {
+        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { x[2 * i] = clean(__uint_as_float(v[i] << 16)); x[2 * i + 1] = clean(__uint_as_float(v[i] & 0xffff0000u)); }
+    }
+};
+constexpr int DV_STEPS = 4;              // 16-byte loads of a lane per chunk and row
+template <class T> __host__ __device__ constexpr int chunk_of() { return 32 * DV_STEPS * Row<T>::PER; }
+
+template <class T, bool DRAFT, bool VEC>
+__global__ void __launch_bounds__(DV_THREADS)
+draft_verify_kernel(VerifyArgs A) {
+    constexpr int PER = Row<T>::PER, CHUNK = chunk_of<T>();
+    extern __shared__ double sums[];                           // [chunks] of this block's part, from the last pass
+    __shared__ int s_parent[DV_NODES], s_token[DV_NODES];
+    __shared__ float s_u[DV_NODES], s_p[DV_NODES], s_q[DV_NODES];
+    __shared__ unsigned long long s_kids[DV_NODES];
+    __shared__ int s_out[DV_NODES];                            // tokens left out of r (given drafts)
+    __shared__ double s_part[2][DV_MAX_CLUSTER];               // the blocks' sums of a pass, by the pass's parity
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.y;
+    const uint32_t rank = cluster_rank(), n_rank = cluster_size();
+    rv_grid_dep_wait();
+    rv_grid_dep_trigger();
+    const int start = A.node_start[b], T_all = A.node_start[b + 1] - start, T_n = min(T_all, DV_NODES);
+    const T* target = reinterpret_cast<const T*>(A.target);
+    const T* draft = reinterpret_cast<const T*>(A.draft);
+    if (tid < DV_NODES) s_kids[tid] = 0ull;
+    __syncthreads();
+    if (tid < T_n) {
+        const int par = A.parent[start + tid], tok = A.token[start + tid];
+        const bool child = tid > 0 && par >= 0 && par < tid, known = tok >= 0 && tok < A.vocab;
+        s_token[tid] = known ? tok : -1;
+        s_u[tid] = A.u[start + tid];
+        s_p[tid] = child && known ? Row<T>::one(target + (long long)(start + par) * A.target_stride, tok) : 0.0f;
+        s_q[tid] = DRAFT ? (child && known ? Row<T>::one(draft + (long long)(start + par) * A.draft_stride, tok) : 0.0f) : 1.0f;
+        if (child) atomicOr(&s_kids[par], 1ull << tid);
+    }
+    __syncthreads();
+    int32_t* path = A.path + (size_t)b * A.max_path;
+    if (T_n <= 0) {                                            // (the same for all blocks of the cluster)
+        if (rank == 0 && tid == 0) { A.n_path[b] = 0; A.next[b] = -1; }
+        return;
+    }
+
+    const int lo = (int)rank * A.chunks * CHUNK, hi = min(A.vocab, lo + A.chunks * CHUNK);   // (at most 2^20 + 8 chunks)
+    const int n_chunks = hi > lo ? (hi - lo + CHUNK - 1) / CHUNK : 0;
+    int parity = 0;
+    // r at an index of the current node's rows
+    auto value = [&](double a, double bq, float p, float q) -> double { return DRAFT ? fmax(a * (double)p - bq * (double)q, 0.0) : (double)p; };
+    auto left_out = [&](int v, int n_out) -> bool {
+        bool hit = false;
+        for (int i = 0; i < n_out; ++i) hit |= s_out[i] == v;
+        return hit;
+    };
+    // one pass over the rows of node `cur`: chunk sums of r, and its sum over the vocabulary (the same in every thread)
+    auto pass = [&](int cur, double a, double bq, int n_out) -> double {
+        const T* p = target + (long long)(start + cur) * A.target_stride;
+        const T* q = DRAFT ? draft + (long long)(start + cur) * A.draft_stride : nullptr;
+        const bool with_q = DRAFT && bq != 0.0;
+        for (int c = warp; c < n_chunks; c += DV_WARPS) {
+            const int at = lo + c * CHUNK;
+            double s = 0.0;
+            if (VEC && at + CHUNK <= hi) {
+                uint4 wp[DV_STEPS], wq[DV_STEPS];
+#pragma unroll
+                for (int i = 0; i < DV_STEPS; ++i) wp[i] = __ldg(reinterpret_cast<const uint4*>(p + at) + i * 32 + lane);
+                if (with_q)
+#pragma unroll
+                    for (int i = 0; i < DV_STEPS; ++i) wq[i] = __ldg(reinterpret_cast<const uint4*>(q + at) + i * 32 + lane);
+                else
+#pragma unroll
+                    for (int i = 0; i < DV_STEPS; ++i) wq[i] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                for (int i = 0; i < DV_STEPS; ++i) {
+                    float xp[PER], xq[PER];
+                    Row<T>::unpack(wp[i], xp);
+                    if (DRAFT) Row<T>::unpack(wq[i], xq);
+                    if (!DRAFT && n_out > 0)
+                        for (int k = 0; k < n_out; ++k) {
+                            const int d = s_out[k] - (at + (i * 32 + lane) * PER);
+#pragma unroll
+                            for (int e = 0; e < PER; ++e) xp[e] = d == e ? 0.0f : xp[e];
+                        }
+#pragma unroll
+                    for (int e = 0; e < PER; ++e) s += value(a, bq, xp[e], DRAFT ? xq[e] : 0.0f);
+                }
+            } else {
+                for (int v = at + lane; v < min(at + CHUNK, hi); v += 32)
+                    if (DRAFT || !left_out(v, n_out)) s += value(a, bq, Row<T>::one(p, v), with_q ? Row<T>::one(q, v) : 0.0f);
+            }
+            s = warp_sum(s);
+            if (lane == 0) sums[c] = s;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            double s = 0.0;
+            for (int c = lane; c < n_chunks; c += 32) s += sums[c];
+            s = warp_sum(s);
+            if (lane < (int)n_rank) put_remote(&s_part[parity][rank], lane, s);
+        }
+        cluster_sync();
+        double z = 0.0;
+        for (uint32_t i = 0; i < n_rank; ++i) z += s_part[parity][i];
+        parity ^= 1;                     // (the next pass writes the other set: a block may still be reading this one)
+        return z;
+    };
+
+    int cur = 0, n = 1, n_out = 0;
+    double a = 1.0, bq = 0.0, total = 0.0;
+    double da = 1.0, db = 0.0;           // the two numbers of the last pass: the chunk sums' scale, and the draw's
+    bool have = false, dead = false;     // have: the chunk sums are those of r; dead: nothing is left of r
+    unsigned long long kids = s_kids[0];
+    if (rank == 0 && tid == 0) path[0] = 0;
+    while (kids && n < A.max_path) {
+        const int j = __ffsll((long long)kids) - 1;
+        kids &= kids - 1;
+        const double p = s_p[j], q = s_q[j];
+        double r;
+        if (DRAFT) r = fmax(a * p - bq * q, 0.0);
+        else r = left_out(s_token[j], n_out) ? 0.0 : a * p;
+        if (!dead && (double)s_u[j] * q < r) {
+            if (rank == 0 && tid == 0) path[n] = j;
+            cur = j; ++n; kids = s_kids[j];
+            a = 1.0; bq = 0.0; n_out = 0; have = dead = false;
+            continue;
+        }
+        if (dead) continue;
+        if (DRAFT) bq += 1.0;
+        else {
+            __syncthreads();             // (everyone has looked at the list)
+            if (tid == 0) s_out[n_out] = s_token[j];
+            ++n_out;
+            __syncthreads();
+        }
+        da = a; db = bq;
+        total = pass(cur, da, db, n_out);
+        have = true;
+        if (!(total > 0.0)) { dead = true; have = false; continue; }
+        // r / Z (the draw needs no division)
+        if (DRAFT) { a /= total; bq /= total; }
+        else a = 1.0 / total;
+    }
+    if (!have) { da = 1.0; db = 0.0; n_out = 0; total = pass(cur, da, db, 0); }
+    if (rank == 0 && tid == 0) A.n_path[b] = n;
+
+    // The block whose part holds the draw finds the chunk and the place in it, with one warp.
+    const double want = (double)A.u_next[b] * total;
+    const double* part = s_part[parity ^ 1];
+    int owner = -1, last = -1;
+    double before = 0.0, run = 0.0;
+    for (uint32_t i = 0; i < n_rank; ++i) {
+        const double s = part[i];
+        if (s > 0.0) last = (int)i;
+        if (owner < 0 && run + s > want && s > 0.0) { owner = (int)i; before = run; }
+        run += s;
+    }
+    const bool none = owner < 0;         // the last value that is not zero
+    if (none) { owner = last; before = 0.0; }
+    if (last < 0) { if (rank == 0 && tid == 0) A.next[b] = -1; }
+    else if (owner == (int)rank && warp == 0) {
+        // chunk: lanes take runs of chunks in order
+        const int each = (n_chunks + 31) >> 5;
+        auto find = [&](double mine, double from, bool& hit, double& base) -> int {   // the first lane whose running sum passes `want`
+            double inc = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const double t = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += t; }
+            const double over = __shfl_up_sync(0xffffffffu, inc, 1);
+            const double exc = from + (lane ? over : 0.0);
+            const uint32_t m = __ballot_sync(0xffffffffu, mine > 0.0 && from + inc > want && !none), pos = __ballot_sync(0xffffffffu, mine > 0.0);
+            hit = m != 0;
+            const int who = m ? __ffs(m) - 1 : 31 - __clz(pos | 1u);
+            base = __shfl_sync(0xffffffffu, exc, who);
+            return who;
+        };
+        double mine = 0.0;
+        for (int i = 0; i < each; ++i) { const int c = lane * each + i; if (c < n_chunks) mine += sums[c]; }
+        bool hit;
+        double base;
+        const int who = find(mine, before, hit, base);
+        int chunk = -1;
+        double run2 = base;
+        for (int i = 0; i < each; ++i) {                       // (uniform: all lanes look at the same chunks)
+            const int c = who * each + i;
+            if (c >= n_chunks) break;
+            const double s = sums[c];
+            if (s > 0.0) {
+                chunk = c; base = run2;
+                if (hit && run2 + s > want) break;
+            }
+            run2 += s;
+        }
+        // place: lanes take runs of the chunk's values in order
+        const T* p = target + (long long)(start + cur) * A.target_stride;
+        const T* q = DRAFT ? draft + (long long)(start + cur) * A.draft_stride : nullptr;
+        const int at = lo + chunk * CHUNK, end = min(at + CHUNK, hi), run_len = CHUNK / 32;
+        auto at_value = [&](int v) -> double {
+            if (!DRAFT && left_out(v, n_out)) return 0.0;
+            return value(da, db, Row<T>::one(p, v), DRAFT && db != 0.0 ? Row<T>::one(q, v) : 0.0f);
+        };
+        mine = 0.0;
+        for (int i = 0; i < run_len; ++i) { const int v = at + lane * run_len + i; if (v < end) mine += at_value(v); }
+        const int who2 = find(mine, base, hit, run2);
+        if (lane == who2) {
+            int found = -1;
+            for (int i = 0; i < run_len; ++i) {
+                const int v = at + lane * run_len + i;
+                if (v >= end) break;
+                const double x = at_value(v);
+                if (x > 0.0) {
+                    found = v;
+                    if (hit && run2 + x > want) break;
+                }
+                run2 += x;
+            }
+            A.next[b] = found;
+        }
+    }
+    cluster_sync();                      // no block leaves while another may still write into it
+}
+
+template <class T, bool DRAFT, bool VEC>
+int launch(const VerifyArgs& a, int n, int B, cudaStream_t st) {
+    rv_drain_error();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)n, (unsigned)B); cfg.blockDim = dim3(DV_THREADS);
+    cfg.dynamicSmemBytes = (size_t)a.chunks * sizeof(double); cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)n; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 2;
+    (void)cudaLaunchKernelEx(&cfg, draft_verify_kernel<T, DRAFT, VEC>, a);
+    return rv_launch_status();
+}
+template <class T>
+int dispatch(VerifyArgs& a, int B, cudaStream_t st) {
+    // blocks a sequence: until there are two to an SM, a part being at least two chunks a warp
+    const int sms = rv_sm_count(), all = (a.vocab + chunk_of<T>() - 1) / chunk_of<T>();
+    int n = 1;
+    while (n < DV_MAX_CLUSTER && (long long)B * n < 2 * sms && all / (2 * n) >= 2 * DV_WARPS) n *= 2;
+    a.chunks = (all + n - 1) / n;
+    const bool vec = (((uintptr_t)a.target | (uintptr_t)a.draft) & 15) == 0 && a.target_stride * (long long)sizeof(T) % 16 == 0 &&
+                     (!a.draft || a.draft_stride * (long long)sizeof(T) % 16 == 0);
+    if (a.draft) return vec ? launch<T, true, true>(a, n, B, st) : launch<T, true, false>(a, n, B, st);
+    return vec ? launch<T, false, true>(a, n, B, st) : launch<T, false, false>(a, n, B, st);
+}
+
+}  // namespace
+
+RIVOLI_API int rivoli_draft_verify(const int32_t* node_start, const int32_t* parent, const int32_t* token, const void* target,
+                                   long long target_stride, const void* draft, long long draft_stride, int prob_bits, int vocab,
+                                   const float* u, const float* u_next, int B, int32_t* path, int max_path, int32_t* n_path,
+                                   int32_t* next, void* stream) {
+    if (!node_start || !parent || !token || !target || !u || !u_next || !path || !n_path || !next || B <= 0 || vocab <= 0 || max_path <= 0)
+        return 1001;
+    if (vocab > DV_MAX_VOCAB || max_path > DV_NODES || B > 65535) return 1002;
+    if (prob_bits != 32 && prob_bits != 16) return 1004;
+    if (target_stride < vocab || (draft && draft_stride < vocab)) return 1005;
+    if (((uintptr_t)target | (uintptr_t)draft) & (prob_bits / 8 - 1)) return 1005;
+    VerifyArgs a{node_start, parent, token, target, draft, target_stride, draft_stride, vocab, 0, u, u_next, path, max_path, n_path, next};
+    return prob_bits == 32 ? dispatch<float>(a, B, (cudaStream_t)stream) : dispatch<uint16_t>(a, B, (cudaStream_t)stream);
+}

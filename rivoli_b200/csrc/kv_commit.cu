@@ -1,0 +1,116 @@
+// The accepted rows of a drafted tree, moved in the paged pools to where the sequence goes on, in all layers with one launch.
+//
+// Sequence b drafted its nodes into the rows of positions tree_pos[b] + j; path[b][0 .. n_path[b]) (ascending node indices) stays.
+// Row tree_pos[b] + path[b][k] becomes row tree_pos[b] + k: codes and scales of the latent row and of the indexer key, bit for bit.
+// A row only ever moves down (path[k] >= k), so that no move of a later k reads what an earlier one has written; of the rows that a
+// block moves together all are read before any is written. Rows that stay where they are (a chain that was accepted from its root)
+// are not touched.
+// Bound by memory: 712 bytes read and written per moved row and layer of the model geometry, a 16-byte chunk per lane.
+#include "common.cuh"
+
+namespace {
+
+constexpr int KC_WARPS = 8, KC_MAX_PATH = 64;
+constexpr int KC_CHUNKS = 3;            // 16-byte chunks of a row a lane holds: (512 + 128 + 512) / 16 <= 3 * 32
+
+struct CommitArgs {
+    DsaGeom g;
+    const CommitLayer* layers; int n_layers, layers_per_block;
+    const int32_t* block_table; const int32_t* tree_pos; const int32_t* path; const int32_t* n_path;
+    int path_stride;
+    int32_t* seq_len; int32_t* status;
+};
+
+__global__ void __launch_bounds__(KC_WARPS * 32)
+kv_commit_kernel(CommitArgs A) {
+    __shared__ long long s_src[KC_MAX_PATH], s_dst[KC_MAX_PATH];   // pool rows; -1: nothing to move
+    __shared__ int s_bad;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.y;
+    rv_grid_dep_wait();
+    rv_grid_dep_trigger();
+    const int pos = A.tree_pos[b], n = min(max(A.n_path[b], 0), A.path_stride);
+    if (tid == 0) s_bad = 0;
+    __syncthreads();
+    if (tid < n) {
+        const int node = A.path[(size_t)b * A.path_stride + tid];
+        const int before = tid ? A.path[(size_t)b * A.path_stride + tid - 1] : -1;
+        long long src = -1, dst = -1;
+        if (node != tid || before != tid - 1) {
+            auto pool_row = [&](int t) -> long long {
+                const int lp = t / A.g.page_tokens;
+                const int pg = lp < A.g.max_pages_per_seq ? A.block_table[(size_t)b * A.g.max_pages_per_seq + lp] : -1;
+                return pg >= 0 && pg < A.g.n_pool_pages ? (long long)pg * A.g.page_tokens + t % A.g.page_tokens : -1;
+            };
+            const bool sound = node > before && node >= tid && node < KC_MAX_PATH && pos >= 0 && pos < 0x7fffffff - KC_MAX_PATH;
+            src = sound ? pool_row(pos + node) : -1;
+            dst = sound ? pool_row(pos + tid) : -1;
+            if (src < 0 || dst < 0) s_bad = 1;
+        }
+        s_src[tid] = src; s_dst[tid] = dst;
+    }
+    __syncthreads();
+    if (s_bad) {                        // an unsound path or an unmapped page: the sequence is left as it is
+        if (A.status && tid == 0 && blockIdx.x == 0) atomicOr(A.status, 1);
+        return;
+    }
+    if (A.seq_len && tid == 0 && blockIdx.x == 0) A.seq_len[b] = pos + n;
+    int first = 0;
+    while (first < n && s_src[first] < 0) ++first;
+    const int wl = (A.g.kv_lora + A.g.rope_dim) >> 4, wi = A.g.index_dim >> 4;   // chunks
+    const int l0 = blockIdx.x * A.layers_per_block, l1 = min(A.n_layers, l0 + A.layers_per_block);
+    for (int k0 = first; k0 < n; k0 += KC_WARPS) {
+        const int k = k0 + warp;
+        const bool moves = k < n && s_src[k] >= 0;
+        const size_t src = moves ? s_src[k] : 0, dst = moves ? s_dst[k] : 0;
+        for (int l = l0; l < l1; ++l) {
+            const CommitLayer L = A.layers[l];
+            const int chunks = wl + (L.index_pool ? wi : 0);
+            uint4 v[KC_CHUNKS];
+            float sc = 0.0f;
+            if (moves) {
+#pragma unroll
+                for (int u = 0; u < KC_CHUNKS; ++u) {
+                    const int c = lane + 32 * u;
+                    if (c < chunks)
+                        v[u] = c < wl ? reinterpret_cast<const uint4*>(L.latent_pool)[src * wl + c]
+                                      : reinterpret_cast<const uint4*>(L.index_pool)[src * wi + (c - wl)];
+                }
+                if (lane == 0) sc = L.latent_scale[src];
+                if (lane == 1 && L.index_pool) sc = L.index_scale[src];
+            }
+            __syncthreads();            // all rows of the block's eight are in registers
+            if (moves) {
+#pragma unroll
+                for (int u = 0; u < KC_CHUNKS; ++u) {
+                    const int c = lane + 32 * u;
+                    if (c < chunks) {
+                        if (c < wl) reinterpret_cast<uint4*>(L.latent_pool)[dst * wl + c] = v[u];
+                        else reinterpret_cast<uint4*>(L.index_pool)[dst * wi + (c - wl)] = v[u];
+                    }
+                }
+                if (lane == 0) L.latent_scale[dst] = sc;
+                if (lane == 1 && L.index_pool) L.index_scale[dst] = sc;
+            }
+        }
+    }
+}
+
+}  // namespace
+
+RIVOLI_API int rivoli_kv_commit_paged(const DsaGeom* g, const CommitLayer* layers, int n_layers, const int32_t* block_table,
+                                      const int32_t* tree_pos, const int32_t* path, int path_stride, const int32_t* n_path, int B,
+                                      int32_t* seq_len, int32_t* status, void* stream) {
+    if (int e = rv_check_geom(g)) return e;
+    if (!layers || n_layers <= 0 || !block_table || !tree_pos || !path || path_stride <= 0 || !n_path || B <= 0) return 1001;
+    if (path_stride > KC_MAX_PATH || B > 65535) return 1002;
+    if (((uintptr_t)layers & 7) || seq_len == tree_pos) return 1005;   // (blocks read tree_pos while one writes seq_len)
+    CommitArgs a{*g, layers, n_layers, 1, block_table, tree_pos, path, n_path, path_stride, seq_len, status};
+    // blocks that each move one layer's rows, several layers each once there are more than eight blocks to an SM
+    const long long blocks = (long long)n_layers * B, most = 8LL * rv_sm_count();
+    a.layers_per_block = blocks <= most ? 1 : (int)((blocks + most - 1) / most);
+    if (a.layers_per_block > n_layers) a.layers_per_block = n_layers;
+    rv_drain_error();
+    rv_launch_dependent(kv_commit_kernel, dim3((n_layers + a.layers_per_block - 1) / a.layers_per_block, B), dim3(KC_WARPS * 32), 0,
+                        (cudaStream_t)stream, a);
+    return rv_launch_status();
+}

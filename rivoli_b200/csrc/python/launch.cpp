@@ -5,7 +5,7 @@
 // on taking the addresses of its tensors, against 2.3 us for each kernel launch. Here a call takes the objects as they are:
 //   pointer   None (NULL), an integer address, an object with data_ptr() (a tensor), or one with cuda_stream (a stream)
 //   geometry  a ctypes structure, through the buffer protocol; None = NULL
-//   CompFinish, CompStep   the same, or a tuple of their fields
+//   CompFinish, CompStep, RopeVecs   the same, or a tuple of their fields
 //   integer, float         as ctypes: wrapped to the parameter's width, rounded to its precision
 // The interpreter lock is released around the call, as ctypes does. Host time with the launches: a decode step (25 arguments,
 // four launches) 14.7 -> 12.0 us, the three projection operators 18.0 -> 12.0, a V4 prompt's six calls 26.2 -> 18.4 (which is
@@ -74,6 +74,16 @@ struct Arg<int> {
     int get() { return static_cast<int>(static_cast<unsigned>(v)); }
 };
 
+template <>
+struct Arg<long long> {
+    unsigned long long v = 0;
+    bool set(PyObject* o) { return to_word(o, &v); }
+    long long get() { return static_cast<long long>(v); }
+};
+template <> struct Arg<int64_t> : Arg<long long> {
+    int64_t get() { return static_cast<int64_t>(v); }
+};
+
 template <class T>
 struct Real {
     double v = 0;
@@ -128,6 +138,7 @@ struct Fields : Struct<T> {                                      // or of a tupl
     }
     const T* get() { return tuple ? &v : Struct<T>::get(); }
 };
+template <> struct Arg<const RopeVecs*> : Fields<RopeVecs, const uint16_t*, uint16_t*, int64_t, int64_t, int64_t, int64_t, int> {};
 template <> struct Arg<const CompFinish*> : Fields<CompFinish, const float*, const float*, float*> {};
 template <>
 struct Arg<const CompStep*> : Fields<CompStep, const float*, const float*, const float*, float*, float*, const float*, const float*,
@@ -160,6 +171,7 @@ PyMethodDef methods[] = {
     ENTRY(dsa_decode_step_paged), ENTRY(mla_absorb_batched_bf16), ENTRY(mla_value_batched_bf16),
     ENTRY(index_frontend_bf16), ENTRY(act_quant_f4_rotated), ENTRY(act_quant_f8_prefix), ENTRY(kv_compress_deposit),
     ENTRY(kv_compress_prefill), ENTRY(v4_select_blocks_bf16), ENTRY(v4_sparse_attend_bf16), ENTRY(v4_token_step_bf16),
+    ENTRY(rope_rows_bf16), ENTRY(mla_tree_attend_paged_bf16), ENTRY(draft_verify), ENTRY(kv_commit_paged),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_launch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
