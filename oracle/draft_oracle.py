@@ -32,12 +32,14 @@ def tree_rows(table, page, n_pages, n, rows, tree_pos, t):
 def tree_attend(q, codes, scale, pool_rows, n, masks, softmax_scale, kvl, unit=0.0):
     """q f64 [T, H, W]; codes u8 and scale of the pool; returns out f64 [T, H, kvl], lse [T, H], and for a query whose entries are off
     by independent relative errors of deviation ``unit``: the deviations of out and lse by it, and of out by weights off the same way;
-    and sum p |L|, which bounds what weights off by a relative error do."""
+    and sum p |L|, which bounds what weights off by a relative error do. With weights times row scales as multiples of a step, an entry
+    is off by sum |code| times the step at most, by the root of sum code^2 on the whole: both for a step of the largest such weight."""
     T, H, W = q.shape
     live = pool_rows >= 0
     k = E4M3[codes[pool_rows.clip(0)]] * scale[pool_rows.clip(0)].astype(np.float64)[:, None]
     out, lse = np.zeros((T, H, kvl)), np.full((T, H), -np.inf)
-    weight, by_score, by_weight, lse_by = np.zeros((T, H, kvl)), np.zeros((T, H, kvl)), np.zeros((T, H, kvl)), np.zeros((T, H))
+    weight, by_score, by_weight, step, by_step = (np.zeros((T, H, kvl)) for _ in range(5))
+    lse_by, s_row = np.zeros((T, H)), scale[pool_rows.clip(0)].astype(np.float64)
     for j in range(T):
         sees = live & np.array([i < n or bool(int(masks[j]) >> (i - n) & 1) for i in range(len(pool_rows))], dtype=bool)
         if not sees.any():
@@ -53,7 +55,9 @@ def tree_attend(q, codes, scale, pool_rows, n, masks, softmax_scale, kvl, unit=0
         by_score[j] = np.sqrt(np.maximum(var @ v ** 2 - 2 * out[j] * (var @ v) + out[j] ** 2 * var.sum(1, keepdims=True), 0))
         by_weight[j] = unit * np.sqrt(p ** 2 @ v ** 2)
         lse_by[j] = np.sqrt(var.sum(1))
-    return out, lse, by_score, lse_by, by_weight, weight
+        top_p, c = (p * s_row[sees]).max(1, keepdims=True), v / np.where(s_row[sees] > 0, s_row[sees], 1.0)[:, None]
+        step[j], by_step[j] = top_p * np.abs(c).sum(0), top_p * np.sqrt((c ** 2).sum(0))
+    return out, lse, by_score, lse_by, by_weight, weight, step, by_step
 
 
 def clean(x):

@@ -90,6 +90,7 @@ tree_simt_kernel(TreeArgs A, int kvl, int rope) {
             for (int k = 0; k < TS_KVL / 32; ++k) acc[u][k] *= fac;
             for (int t = 0; t < TS_TILE; ++t) {
                 const float w = __shfl_sync(0xffffffffu, p, t);
+                if (w == 0.0f) continue;                       // (a hidden row may hold NaN)
 #pragma unroll
                 for (int k = 0; k < TS_KVL / 32; ++k)
                     if (lane + 32 * k < kvl) acc[u][k] = fmaf(w, tile[t * W + lane + 32 * k], acc[u][k]);
@@ -108,10 +109,6 @@ tree_simt_kernel(TreeArgs A, int kvl, int rope) {
 }
 
 }  // namespace
-
-int rv_tree_mma(const TreeArgs&, void*, cudaStream_t) { return 1004; }
-bool rv_tree_mma_supported(const DsaGeom*) { return false; }
-size_t rv_tree_mma_scratch_bytes() { return 0; }
 
 RIVOLI_API size_t rivoli_mla_tree_attend_scratch_bytes(const DsaGeom* g, int B, int n_nodes) {
     if (!g || B <= 0 || n_nodes <= 0 || rv_check_geom(g)) return 0;

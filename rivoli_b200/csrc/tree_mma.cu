@@ -1,0 +1,703 @@
+// Attention of drafted trees over the paged latent cache on the 5th-generation tensor cores, all operands fp8.
+//
+//     out[r] = sum_j softmax_j((q_r . [L_j | R_j]) * scale) * L_j,    r = (node, head) of one sequence, j = its prefix, then its tree
+//
+// The arithmetic is that of the decode step's attention (attend_mma.cu): cache rows are consumed as the e4m3 codes they are, q and the
+// softmax weights are two e4m3 terms each (2^-8 relative), a row's scale rides in its weight (P' = weight * scale * 2^5), references
+// lag behind the running maximum by at most 2^3, sums are f32. What differs is the shape of the work. The nodes of a tree share their
+// prefix, so that the rows of a sequence are nodes x heads, 64 to a block, and one tile of the cache serves them all: 240 products and
+// more per byte from a single node on and sixteen times that at sixteen nodes. The kernel is bound by the tensor cores and what feeds
+// them, the cache's tiles come from L2, and what has to be even is the number of (row block, tile) pairs per SM:
+//   * one persistent CTA per SM; the pairs of all sequences, in order, are cut into equal runs, one per CTA. A run that begins or ends
+//     inside a row block leaves that block's (maximum, sum, O) in scratch and a second, small kernel joins the parts; all others are
+//     written directly. No sequence is too long and no batch too ragged for this.
+//   * barriers and their phases run on over the row blocks of a CTA: the gather fetches the next block's tiles while this one's output
+//     is written.
+// Rows of the tree are tested against each node's mask in the tiles that hold them, the last one or two of a sequence. A hidden row's
+// weight is 0, but 0 x NaN is NaN: NaN codes of tree rows are fetched as 0 and make the row's scale NaN instead, which only reaches the
+// nodes that see it.
+//
+// Shared memory: a ring of five tiles of 64 rows (36 KiB), the rope columns of q, P' twice, 16 KiB of staging. Tensor memory: S twice
+// (64 columns each), q (128: its latent columns are the A operand of the QK products), O^T (4 x 64). Warps: 0-7 softmax and epilogue, 8 QK
+// issue, 9 PV issue, 10-13 gather. All waits are bounded (tc_common.cuh).
+#include "codec.cuh"
+#include "common.cuh"
+#include "quant.cuh"
+#include "tc_common.cuh"
+#include "tree_common.cuh"
+
+namespace {
+
+constexpr int TM_TILE = 64, TM_ROWS = 64;            // cache rows of a tile, (node, head) rows of a block
+constexpr int TM_KVL = 512, TM_ROPE = 64, TM_W = TM_KVL + TM_ROPE;
+constexpr int TM_STAGES = 5, TM_GW = 4, TM_SW = 8;
+constexpr int TM_QKW = TM_SW, TM_PVW = TM_SW + 1, TM_GW0 = TM_SW + 2;
+constexpr int TM_THREADS = (TM_GW0 + TM_GW) * 32, TM_SOFTMAX = TM_SW * 32;
+constexpr float TM_POFF = 5.0f, TM_LAG = 3.0f;       // P' = 2^(s - ref + 5) <= 2^8, see attend_mma.cu
+constexpr int TM_MIN_UNITS = 4;                      // tiles a CTA takes at least, while there are few
+
+// tensor memory columns
+constexpr int TMC_S = 0, TMC_Q = 2 * TM_TILE, TMC_O = TMC_Q + TM_KVL / 4;
+static_assert(TMC_O + 4 * TM_ROWS == 512, "tensor memory budget");
+
+// shared memory (bytes)
+constexpr int KCHUNK = 8192, KSTAGE = 4 * KCHUNK + 4096;    // four latent chunks [64 rows][128 B], 128-byte swizzle; rope [64][64 B], 64-byte swizzle
+constexpr int SM_K = 0;
+constexpr int SM_QR = SM_K + TM_STAGES * KSTAGE;            // rope columns of q: [128 virtual rows][64 B], 64-byte swizzle
+constexpr int SM_P = SM_QR + 8192;                          // twice {hi, lo} [64 rows][64 tokens], 64-byte swizzle
+constexpr int PTERM = 4096, PBUF = 2 * PTERM;
+constexpr int SM_OUT = SM_P + 2 * PBUF;                     // staging: two groups of 8 rows x 512 bf16
+constexpr int SM_TOK = SM_OUT + 2 * 8192;                   // f32 [3][stages][64]: scale | log2(scale) + offset | 1 / scale
+constexpr int TOKPLANE = TM_STAGES * TM_TILE * 4;
+constexpr int SM_AHI = SM_TOK + 3 * TOKPLANE;               // f32 [64] query scale * softmax scale * log2(e)
+constexpr int SM_WMAX = SM_AHI + 256;                       // f32 [2][64]
+constexpr int SM_FAC = SM_WMAX + 512;                       // f32 [64]
+constexpr int SM_MREF = SM_FAC + 256;                       // f32 [64]
+constexpr int SM_BARS = SM_MREF + 256;
+constexpr int SM_MISC = SM_BARS + 256;
+constexpr int SM_TOTAL = SM_MISC + 64;
+static_assert(SM_TOTAL <= 232448, "shared memory budget");
+static_assert(SM_QR % 1024 == 0 && SM_P % 1024 == 0 && KSTAGE % 1024 == 0, "operand tiles are 1024-byte aligned");
+
+struct Bars {
+    uint64_t k_full[TM_STAGES], k_empty[TM_STAGES], s_full[2], s_empty[2], p_full[2], pv_done[2], dec[2], q_full;
+};
+static_assert(sizeof(Bars) <= 256, "barrier block");
+
+// scratch: error word (256 bytes) | per CTA the block it is the first of, for the joining kernel | (reference, sum) of parts | O of parts
+constexpr int SLOTS = 2 * RV_SMS;                           // a CTA leaves at most the end of one block and the beginning of another
+struct Head { int32_t row0, valid, parts, pad; };
+constexpr size_t SC_HEAD = 256, SC_ML = SC_HEAD + RV_SMS * sizeof(Head), SC_O = (SC_ML + (size_t)SLOTS * TM_ROWS * 8 + 255) / 256 * 256;
+constexpr size_t SC_TOTAL = SC_O + (size_t)SLOTS * TM_ROWS * TM_KVL * 4;
+
+__device__ __forceinline__ uint32_t sw64_chunk(uint32_t row, uint32_t chunk) { return row * 64u + ((chunk ^ ((row >> 1) & 3u)) << 4); }
+__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes, uint32_t layout) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)((lbo_bytes >> 4) & 0x3FFFu) << 16;
+    d |= (uint64_t)((sbo_bytes >> 4) & 0x3FFFu) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)layout << 61;   // 2 = 128-byte swizzle, 4 = 64-byte swizzle
+    return d;
+}
+
+// A walk over a run of (row block, tile) pairs. Units are numbered tile by tile, block by block, sequence by sequence.
+struct Walk {
+    int b, rb, t0, t1;             // sequence, row block, tiles [t0, t1) of the current segment
+    long long left;                // units of the run from t0 on
+    int nt, nrb;                   // tiles and row blocks of the sequence
+    TreeSeq s;
+};
+__device__ __forceinline__ void units_of(const TreeArgs& A, const TreeSeq& s, int& nt, int& nrb) {
+    nrb = (s.T * A.H + TM_ROWS - 1) / TM_ROWS;
+    nt = s.T ? (s.n + s.T + TM_TILE - 1) / TM_TILE : 0;
+}
+__device__ __forceinline__ bool walk_segment(const TreeArgs& A, Walk& w) {
+    if (w.left <= 0) return false;
+    while (w.nrb == 0) {           // (only behind the first segment: the run begins in a sequence that has units)
+        if (++w.b >= A.B) return false;
+        w.s = tree_seq(A, w.b);
+        units_of(A, w.s, w.nt, w.nrb);
+    }
+    w.t1 = (int)min((long long)w.nt, w.t0 + w.left);
+    return true;
+}
+__device__ __forceinline__ void walk_on(const TreeArgs& A, Walk& w) {
+    w.left -= w.t1 - w.t0;
+    w.t0 = 0;
+    if (++w.rb == w.nrb) { w.rb = 0; w.nrb = 0; }
+}
+// First unit of CTA g's run.
+__device__ __forceinline__ long long run_begin(long long total, int g, int n) { return total * g / n; }
+
+__global__ void __launch_bounds__(TM_THREADS, 1)
+tree_mma_kernel(TreeArgs A, int* err, uint8_t* scratch, int max_polls) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    Bars& bars = *reinterpret_cast<Bars*>(smem + SM_BARS);
+    float* s_tok = reinterpret_cast<float*>(smem + SM_TOK);
+    float* s_ahi = reinterpret_cast<float*>(smem + SM_AHI);
+    float* s_wmax = reinterpret_cast<float*>(smem + SM_WMAX);
+    float* s_fac = reinterpret_cast<float*>(smem + SM_FAC);
+    float* s_mref = reinterpret_cast<float*>(smem + SM_MREF);
+    uint32_t* tmem_base_s = reinterpret_cast<uint32_t*>(smem + SM_MISC);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + SM_MISC + 4);
+    int* s_run = reinterpret_cast<int*>(smem + SM_MISC + 8);               // b, rb, t0 of the run's beginning
+    long long* s_units = reinterpret_cast<long long*>(smem + SM_MISC + 24);   // its units, all units
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+#pragma unroll
+        for (int s = 0; s < TM_STAGES; ++s) { tc::mbar_init(&bars.k_full[s], 33); tc::mbar_init(&bars.k_empty[s], 1); }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            tc::mbar_init(&bars.s_full[s], 2); tc::mbar_init(&bars.s_empty[s], TM_SW / 2);
+            tc::mbar_init(&bars.p_full[s], TM_SOFTMAX / 2); tc::mbar_init(&bars.pv_done[s], 1); tc::mbar_init(&bars.dec[s], TM_SW / 2);
+        }
+        tc::mbar_init(&bars.q_full, TM_SOFTMAX);
+        tc::mbar_init_fence();
+        *abort_flag = 0;
+    }
+    if (warp == TM_QKW) tc::tmem_alloc<512>(tmem_base_s);
+    tc::fence_proxy_async();
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = *tmem_base_s;
+    const uint32_t TM_S0 = tmem + TMC_S, TM_Q = tmem + TMC_Q, TM_O = tmem + TMC_O;
+    rv_grid_dep_wait();
+    rv_grid_dep_trigger();
+
+    // ------------------------------ the CTA's run ------------------------------------------------
+    if (warp == 0) {
+        auto scan = [&](int b, long long& inc) {   // units of sequence b, and of all of its 32 up to it
+            int nt = 0, nrb = 0;
+            if (b < A.B) { const TreeSeq s = tree_seq(A, b); units_of(A, s, nt, nrb); }
+            const long long mine = (long long)nt * nrb;
+            inc = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const long long v = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += v; }
+            return mine;
+        };
+        long long total = 0, inc;
+        for (int b0 = 0; b0 < A.B; b0 += 32) { scan(b0 + lane, inc); total += __shfl_sync(0xffffffffu, inc, 31); }
+        const int n = (int)max(1LL, min((long long)gridDim.x, total / TM_MIN_UNITS)), g = blockIdx.x;
+        const long long u0 = g < n ? run_begin(total, g, n) : total, u1 = g < n ? run_begin(total, g + 1, n) : total;
+        if (lane == 0) { s_units[0] = u1 - u0; s_units[1] = total; s_run[0] = A.B; s_run[1] = s_run[2] = 0; s_run[3] = n; }
+        __syncwarp();
+        long long before = 0;
+        for (int b0 = 0; b0 < A.B && u1 > u0; b0 += 32) {
+            const long long mine = scan(b0 + lane, inc);
+            if (u0 >= before + inc - mine && u0 < before + inc) {
+                int nt, nrb;
+                units_of(A, tree_seq(A, b0 + lane), nt, nrb);
+                const long long in = u0 - (before + inc - mine);
+                s_run[0] = b0 + lane; s_run[1] = (int)(in / nt); s_run[2] = (int)(in % nt);
+            }
+            before += __shfl_sync(0xffffffffu, inc, 31);
+        }
+    }
+    __syncthreads();
+    Walk w;
+    w.b = s_run[0]; w.rb = s_run[1]; w.t0 = s_run[2]; w.left = w.b < A.B ? s_units[0] : 0;
+    w.nt = w.nrb = 0;
+    if (w.left > 0) { w.s = tree_seq(A, w.b); units_of(A, w.s, w.nt, w.nrb); }
+
+    if (warp >= TM_GW0) {
+        // ------------------------------ gather ---------------------------------------------------
+        // A tile per warp in turn; a lane resolves two rows (entry -> page -> pool row -> scale), one of the warp's tiles ahead, and
+        // the copies go row by row with 32 lanes on 32 consecutive 16-byte chunks. No warp waits for its copies: they signal the
+        // stage themselves. Rows past the end and on unmapped pages are written as zeros.
+        const int g = warp - TM_GW0;
+        constexpr uint32_t NONE = 0xffffffffu;
+        bool ok = true;
+        int c0 = 0;                                // tiles of the CTA before this segment
+        for (; ok && walk_segment(A, w); c0 += w.t1 - w.t0, walk_on(A, w)) {
+            const int total = w.s.n + w.s.T;
+            auto locate = [&](int t, uint32_t* row, float* scl) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int j = t * TM_TILE + u * 32 + lane;
+                    row[u] = t < w.t1 && j < total ? tree_pool_row(A, w.b, tree_token(A, w.s, w.b, j)) : NONE;
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) scl[u] = row[u] != NONE ? A.pscale[row[u]] : 0.0f;
+            };
+            uint32_t row[2];
+            float scl[2];
+            int t = w.t0 + ((g - c0) & (TM_GW - 1));
+            locate(t, row, scl);
+            for (; t < w.t1; t += TM_GW) {
+                const int i = c0 + t - w.t0, s = i % TM_STAGES, use = i / TM_STAGES;
+                if (use > 0) ok = tc::mbar_wait_warp(&bars.k_empty[s], (use & 1) ^ 1, abort_flag, 41, max_polls);
+                if (!ok) break;
+                uint8_t* kbuf = smem + SM_K + s * KSTAGE;
+                uint8_t* rope = kbuf + 4 * KCHUNK;
+                uint32_t bad[2] = {0u, 0u};        // rows of the tree that hold a NaN code
+                if ((t + 1) * TM_TILE > w.s.n) {
+                    // 36 chunks a row: 32 latent, then four of the rope columns by the first four lanes
+#pragma unroll 1
+                    for (int it = 0; it < TM_TILE; ++it) {
+                        const uint32_t r = __shfl_sync(0xffffffffu, it < 32 ? row[0] : row[1], it & 31);
+                        const uint4* src = reinterpret_cast<const uint4*>(A.pool + (r != NONE ? (size_t)r * TM_W : 0));
+                        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+                        uint4 v = r != NONE ? src[lane] : zero, x = r != NONE && lane < 4 ? src[32 + lane] : zero;
+                        bool nan = false;
+                        if (t * TM_TILE + it >= w.s.n) {
+                            uint32_t* p[2] = {&v.x, &x.x};
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    // bytes whose low seven bits are all up
+                                    const uint32_t m = (((p[h][k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+                                    nan |= m != 0u;
+                                    p[h][k] &= ~(m * 0xffu);
+                                }
+                        }
+                        if (__ballot_sync(0xffffffffu, nan) && (it & 31) == lane) bad[it >> 5] = 1u;
+                        *reinterpret_cast<uint4*>(kbuf + (lane >> 3) * KCHUNK + tc::sw128_chunk(it, lane & 7)) = v;
+                        if (lane < 4) *reinterpret_cast<uint4*>(rope + sw64_chunk(it, lane)) = x;
+                    }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+#pragma unroll 8
+                        for (int it = 0; it < 32; ++it) {
+                            const uint32_t r = __shfl_sync(0xffffffffu, row[u], it);
+                            tc::cp_async16_zfill(tc::smem_u32(kbuf + (lane >> 3) * KCHUNK + tc::sw128_chunk(u * 32 + it, lane & 7)),
+                                                 A.pool + (r != NONE ? (size_t)r * TM_W + lane * 16 : 0), r != NONE ? 16u : 0u);
+                        }
+                    }
+#pragma unroll
+                    for (int it = 0; it < 8; ++it) {
+                        const int rl = it * 8 + (lane >> 2);
+                        const uint32_t r = __shfl_sync(0xffffffffu, row[it >> 2], rl & 31);
+                        tc::cp_async16_zfill(tc::smem_u32(rope + sw64_chunk(rl, lane & 3)),
+                                             A.pool + (r != NONE ? (size_t)r * TM_W + TM_KVL + (lane & 3) * 16 : 0), r != NONE ? 16u : 0u);
+                    }
+                }
+                tc::cp_async_mbar_arrive_noinc(&bars.k_full[s]);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const bool live = row[u] != NONE && !(scl[u] <= 0.0f);
+                    const float sc = bad[u] ? __int_as_float(0x7fffffff) : scl[u];
+                    float* tp = s_tok + s * TM_TILE + u * 32 + lane;
+                    tp[0] = live ? sc : 0.0f;
+                    tp[TOKPLANE / 4] = live ? __log2f(sc) + TM_POFF : -INFINITY;
+                    // (0 for a NaN: times a weight that is NaN itself where the row is seen, times 0 where it is hidden)
+                    tp[2 * (TOKPLANE / 4)] = live && sc == sc ? __frcp_rn(sc) : 0.0f;
+                }
+                tc::fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&bars.k_full[s]);
+                locate(t + TM_GW, row, scl);
+            }
+        }
+    } else if (warp == TM_QKW) {
+        // ------------------------------ QK issuer: S(i) = Q . K(i)^T -----------------------------
+        const uint32_t id_qk = tc::idesc_e4m3(128, TM_TILE, 0, 0);
+        const uint64_t d_qr = smem_desc(tc::smem_u32(smem + SM_QR), 16, 512, 4);
+        bool ok = true;
+        int i = 0, seg = 0;
+        for (; ok && walk_segment(A, w); walk_on(A, w), ++seg) {
+            ok = tc::mbar_wait_warp(&bars.q_full, seg & 1, abort_flag, 51, max_polls);
+            for (int t = w.t0; t < w.t1 && ok; ++t, ++i) {
+                const int s = i % TM_STAGES, use = i / TM_STAGES, sb = i & 1;
+                ok = tc::mbar_wait_warp(&bars.k_full[s], use & 1, abort_flag, 52, max_polls) &&
+                     tc::mbar_wait_warp(&bars.s_empty[sb], ((i >> 1) & 1) ^ 1, abort_flag, 53, max_polls);
+                if (!ok) break;
+                tc::fence_proxy_async();   // the copies wrote through the generic proxy, the products read through the async one
+                tc::tc_fence_after();
+                const uint64_t d_k = smem_desc(tc::smem_u32(smem + SM_K + s * KSTAGE), 16, 1024, 2);
+                const uint64_t d_rope = smem_desc(tc::smem_u32(smem + SM_K + s * KSTAGE + 4 * KCHUNK), 16, 512, 4);
+                const uint32_t d = TM_S0 + sb * TM_TILE;
+                if (tc::elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) tc::mma_f8(d, d_qr + (uint64_t)(k * 2), d_rope + (uint64_t)(k * 2), id_qk, k != 0);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            tc::mma_f8_ta(d, TM_Q + (uint32_t)(c * 32 + k * 8), d_k + (uint64_t)((c * KCHUNK + k * 32) >> 4), id_qk, 1);
+                    tc::mma_commit(&bars.s_full[sb]);
+                    tc::mbar_arrive(&bars.s_full[sb]);   // hands the token words on: this thread has seen k_full
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == TM_PVW) {
+        // ------------------------------ PV issuer: O^T += V(i)^T . P'(i) --------------------------
+        const uint32_t id_pv = tc::idesc_e4m3(128, TM_ROWS, 1, 0);
+        bool ok = true;
+        int i = 0;
+        for (; ok && walk_segment(A, w); walk_on(A, w)) {
+            for (int t = w.t0; t < w.t1 && ok; ++t, ++i) {
+                const int s = i % TM_STAGES, pb = i & 1;
+                ok = tc::mbar_wait_warp(&bars.p_full[pb], (i >> 1) & 1, abort_flag, 54, max_polls);
+                if (!ok) break;
+                tc::fence_proxy_async();
+                tc::tc_fence_after();
+                const uint64_t d_v = smem_desc(tc::smem_u32(smem + SM_K + s * KSTAGE), KCHUNK, 1024, 2);
+                const uint64_t d_phi = smem_desc(tc::smem_u32(smem + SM_P + pb * PBUF), 16, 512, 4);
+                const uint64_t d_plo = smem_desc(tc::smem_u32(smem + SM_P + pb * PBUF + PTERM), 16, 512, 4);
+                if (tc::elect_one()) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            tc::mma_f8(TM_O + c * 64, d_v + (uint64_t)((c * KCHUNK + k * 4096) >> 4), d_phi + (uint64_t)(k * 2), id_pv, t > w.t0 || k != 0);
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            tc::mma_f8(TM_O + c * 64, d_v + (uint64_t)((c * KCHUNK + k * 4096) >> 4), d_plo + (uint64_t)(k * 2), id_pv, 1);
+                    }
+                    tc::mma_commit(&bars.k_empty[s]);
+                    tc::mma_commit(&bars.pv_done[pb]);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        // ------------------------------ queries, softmax, epilogue -------------------------------
+        // S: a thread is a tensor-memory lane, one term of one row: lanes 0-15 of warp s % 4 hold the hi terms of rows 16 s .. + 15,
+        // lanes 16-31 their lo terms. One shuffle per score adds the two and leaves each lane half of the tokens of its row. The
+        // groups of four warps take the tiles in turn.
+        const int sq = warp & 3, th = warp >> 2, tb = lane >> 4;
+        const int hd = 16 * sq + (lane & 15);
+        const int orow = sq * 32 + lane;                   // O^T: this thread's dim of each 128-dim block
+        const uint32_t lane_base = ((uint32_t)(sq * 32)) << 16;
+        constexpr int GROUP = TM_SOFTMAX / 2;
+        auto give_up = [&]() { (void)tc::barrier_any(6 + th, GROUP, true); (void)tc::barrier_any(8 + th, GROUP, true); };
+        int i0 = 0;                                        // tiles of the CTA before this segment
+        bool failed = false;
+        for (; !failed && walk_segment(A, w); i0 += w.t1 - w.t0, walk_on(A, w)) {
+            const int rows_all = w.s.T * A.H, r0 = w.rb * TM_ROWS, valid = min(TM_ROWS, rows_all - r0);
+            const size_t flat = (size_t)w.s.node0 * A.H + r0;      // first row of the block in q, out and out_lse
+            const uint64_t mask = hd < valid ? A.node_mask[w.s.node0 + (r0 + hd) / A.H] : 0ull;
+            // ---- q -> two e4m3 terms per row: hi = e4m3(q / s), s = absmax / 448, lo = e4m3(q / s - hi) ----
+            // (warp half th takes that half of the columns; a lane the 128 latent and 16 rope values on its side tb; one shuffle a
+            // word gives each lane one term of both sides, a run of the row of its own tensor-memory lane)
+            {
+                const uint16_t* src = A.q + (flat + (hd < valid ? hd : 0)) * TM_W;
+                const uint4* l4 = reinterpret_cast<const uint4*>(src + th * (TM_KVL / 2) + tb * (TM_KVL / 4));
+                const uint4* r4 = reinterpret_cast<const uint4*>(src + TM_KVL + th * (TM_ROPE / 2) + tb * (TM_ROPE / 4));
+                uint4 v[18];
+#pragma unroll
+                for (int c = 0; c < 18; ++c) v[c] = hd < valid ? (c < 16 ? l4[c] : r4[c - 16]) : make_uint4(0u, 0u, 0u, 0u);
+                uint32_t m = 0u;
+#pragma unroll
+                for (int c = 0; c < 18; ++c) m = rv_max_bf16x2(m, rv_absmax8(v[c]));
+                m = rv_max_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                if (tb == 0) s_wmax[th * 64 + hd] = __uint_as_float(m << 16);
+                tc::named_barrier(3, TM_SOFTMAX);          // (also: both groups are through with the block before)
+                const float amax = fmaxf(s_wmax[hd], s_wmax[64 + hd]);
+                const float sc = amax > 0.0f ? amax / 448.0f : 1.0f, inv = 1.0f / sc;
+                if (th == 0 && tb == 0) { s_ahi[hd] = sc * A.softmax_scale * 1.4426950408889634f; s_mref[hd] = -INFINITY; }
+                auto codes8 = [&](const uint4 x, uint2& hi, uint2& lo) {
+                    const uint32_t ww[4] = {x.x, x.y, x.z, x.w};
+                    uint16_t ch[4], cl[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float x0 = __uint_as_float(ww[k] << 16) * inv, x1 = __uint_as_float(ww[k] & 0xffff0000u) * inv;
+                        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(ch[k]) : "f"(x1), "f"(x0));
+                        const float2 xh = rv_e4m3x2_to_f32x2(ch[k]);
+                        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(cl[k]) : "f"(x1 - xh.y), "f"(x0 - xh.x));
+                    }
+                    hi = make_uint2((uint32_t)ch[0] | ((uint32_t)ch[1] << 16), (uint32_t)ch[2] | ((uint32_t)ch[3] << 16));
+                    lo = make_uint2((uint32_t)cl[0] | ((uint32_t)cl[1] << 16), (uint32_t)cl[2] | ((uint32_t)cl[3] << 16));
+                };
+                auto exchange = [&](const uint2 hi, const uint2 lo, uint32_t* first, uint32_t* second) {
+                    const uint2 keep = tb ? lo : hi, give = tb ? hi : lo;
+                    const uint2 got = make_uint2(__shfl_xor_sync(0xffffffffu, give.x, 16), __shfl_xor_sync(0xffffffffu, give.y, 16));
+                    first[0] = tb ? got.x : keep.x; first[1] = tb ? got.y : keep.y;
+                    second[0] = tb ? keep.x : got.x; second[1] = tb ? keep.y : got.y;
+                };
+                const uint32_t dst = TM_Q + lane_base + th * 64;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    uint32_t a0[8], a1[8];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint2 hi, lo;
+                        codes8(v[g * 4 + c], hi, lo);
+                        exchange(hi, lo, a0 + 2 * c, a1 + 2 * c);
+                    }
+                    tc::tmem_st8(dst + g * 8, a0);
+                    tc::tmem_st8(dst + 32 + g * 8, a1);
+                }
+                uint32_t a0[4], a1[4];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint2 hi, lo;
+                    codes8(v[16 + c], hi, lo);
+                    exchange(hi, lo, a0 + 2 * c, a1 + 2 * c);
+                }
+                *reinterpret_cast<uint4*>(smem + SM_QR + sw64_chunk(orow, 2 * th)) = make_uint4(a0[0], a0[1], a0[2], a0[3]);
+                *reinterpret_cast<uint4*>(smem + SM_QR + sw64_chunk(orow, 2 * th + 1)) = make_uint4(a1[0], a1[1], a1[2], a1[3]);
+                tc::tmem_st_wait();
+                tc::fence_proxy_async();
+                tc::tc_fence_before();
+                tc::mbar_arrive(&bars.q_full);
+                tc::named_barrier(3, TM_SOFTMAX);          // the row scales and references are read by other warps than wrote them
+            }
+
+            // ---- the tiles ----
+            const float a_h = s_ahi[hd];
+            float l_acc = 0.0f, m_ref = -INFINITY;
+            const int i1 = i0 + (w.t1 - w.t0);
+            bool ok = true;
+            for (int i = i0 + ((th ^ i0) & 1); i < i1; i += 2) {
+                const int s = i % TM_STAGES, j0 = (w.t0 + i - i0) * TM_TILE;
+                ok = tc::mbar_wait_warp(&bars.s_full[th], (i >> 1) & 1, abort_flag, 62, max_polls);
+                if (!ok) { give_up(); break; }
+                tc::tc_fence_after();
+                const float4* ti = reinterpret_cast<const float4*>(s_tok + s * TM_TILE + 16 * tb);
+                float s2[32];
+                float mx = -INFINITY;
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    uint32_t r[32];
+                    tc::tmem_ld32(TM_S0 + th * TM_TILE + lane_base + 32 * hf, r);
+                    tc::tmem_ld_wait();
+                    if (hf == 1) {
+                        tc::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&bars.s_empty[th]);
+                    }
+#pragma unroll
+                    for (int j4 = 0; j4 < 4; ++j4) {
+                        const float4 ts = ti[8 * hf + j4], tc2 = ti[TOKPLANE / 16 + 8 * hf + j4];
+                        const float sc4[4] = {ts.x, ts.y, ts.z, ts.w}, c24[4] = {tc2.x, tc2.y, tc2.z, tc2.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int j = 4 * j4 + e;
+                            const float mine = __uint_as_float(tb ? r[16 + j] : r[j]);
+                            const float give = __uint_as_float(tb ? r[j] : r[16 + j]);
+                            const float raw = mine + __shfl_xor_sync(0xffffffffu, give, 16);
+                            // rows past the end are zeros with an additive -inf: their weights are exactly 0
+                            s2[16 * hf + j] = fmaf(raw, a_h * sc4[e], c24[e]);
+                            mx = fmaxf(mx, s2[16 * hf + j]);
+                        }
+                    }
+                }
+                if (j0 + TM_TILE > w.s.n) {                // rows of the tree: what the mask hides weighs 0
+                    const uint64_t see = tree_visible(mask, w.s.T, w.s.n, j0) >> (16 * tb);
+                    mx = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        if (!((see >> (j < 16 ? j : 16 + j)) & 1)) s2[j] = -INFINITY;
+                        mx = fmaxf(mx, s2[j]);
+                    }
+                }
+                // the references as the tile before left them (the other group's)
+                if (i > i0) {
+                    ok = tc::mbar_wait_warp(&bars.dec[th ^ 1], ((i - 1) >> 1) & 1, abort_flag, 65, max_polls);
+                    if (!ok) { give_up(); break; }
+                    const float m_now = s_mref[hd];
+                    if (m_now != m_ref) { l_acc *= exp2f(m_ref - m_now); m_ref = m_now; }
+                }
+                // As long as no score exceeds its row's reference by more than the lag the references stand: one barrier with an OR.
+                if (tc::barrier_any(6 + th, GROUP, mx - m_ref > TM_LAG + TM_POFF)) {
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    float fac = 1.0f;
+                    {
+                        const float tm = mx - TM_POFF;
+                        if (m_ref == -INFINITY) { if (tm > -INFINITY) m_ref = tm; }
+                        else if (tm > m_ref) { fac = exp2f(m_ref - tm); m_ref = tm; }
+                        if (lane < 16) { s_fac[hd] = fac; s_mref[hd] = m_ref; }
+                    }
+                    if (tc::barrier_any(8 + th, GROUP, false)) { ok = false; break; }
+                    if (i > i0) ok = tc::mbar_wait_warp(&bars.pv_done[th ^ 1], ((i - 1) >> 1) & 1, abort_flag, 63, max_polls);
+                    if (!ok) { if (i + 2 < i1) give_up(); break; }
+                    tc::tc_fence_after();
+                    if (i > i0) {                          // O^T to the new references
+                        uint32_t r[32];
+#pragma unroll 1
+                        for (int c = 0; c < 8; ++c) {
+                            tc::tmem_ld32(TM_O + lane_base + c * 32, r);
+                            tc::tmem_ld_wait();
+#pragma unroll
+                            for (int h = 0; h < 32; ++h) r[h] = __float_as_uint(__uint_as_float(r[h]) * s_fac[(c & 1) * 32 + h]);
+                            tc::tmem_st32(TM_O + lane_base + c * 32, r);
+                        }
+                        tc::tmem_st_wait();
+                    }
+                    l_acc *= fac;
+                    tc::tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&bars.dec[th]);
+                // P' as two e4m3 terms (through f16); l takes the plain weight. A row that has seen nothing has no reference: its
+                // scores are all -inf and weigh 0.
+                const float m_use = m_ref == -INFINITY ? 0.0f : m_ref;
+                uint32_t hi_w[8], lo_w[8];
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                    const float4 ti4 = ti[2 * (TOKPLANE / 16) + 8 * (j >> 4) + ((j & 15) >> 2)];
+                    const float inv4[4] = {ti4.x, ti4.y, ti4.z, ti4.w};
+                    uint32_t chs[2], cls[2];
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        float p0, p1;
+                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(s2[j + e] - m_use));
+                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(s2[j + e + 1] - m_use));
+                        l_acc = fmaf(p0, inv4[e], l_acc);
+                        l_acc = fmaf(p1, inv4[e + 1], l_acc);
+                        const __half2 ph = __floats2half2_rn(p0, p1);
+                        const uint32_t phb = *reinterpret_cast<const uint32_t*>(&ph);
+                        uint16_t ch, cl;
+                        uint32_t hfb;
+                        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(ch) : "r"(phb));
+                        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hfb) : "h"(ch));
+                        const __half2 res = __hsub2(ph, *reinterpret_cast<const __half2*>(&hfb));
+                        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(cl) : "r"(*reinterpret_cast<const uint32_t*>(&res)));
+                        chs[e >> 1] = ch; cls[e >> 1] = cl;
+                    }
+                    hi_w[j >> 2] = chs[0] | (chs[1] << 16);
+                    lo_w[j >> 2] = cls[0] | (cls[1] << 16);
+                }
+                // the buffer was read by the products of this group's tile before
+                if (i >= i0 + 2) ok = tc::mbar_wait_warp(&bars.pv_done[th], ((i - 2) >> 1) & 1, abort_flag, 64, max_polls);
+                if (!ok) { if (i + 2 < i1) give_up(); break; }
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    uint8_t* prow = smem + SM_P + th * PBUF + sw64_chunk(hd, 2 * hf + tb);
+                    *reinterpret_cast<uint4*>(prow) = make_uint4(hi_w[4 * hf], hi_w[4 * hf + 1], hi_w[4 * hf + 2], hi_w[4 * hf + 3]);
+                    *reinterpret_cast<uint4*>(prow + PTERM) = make_uint4(lo_w[4 * hf], lo_w[4 * hf + 1], lo_w[4 * hf + 2], lo_w[4 * hf + 3]);
+                }
+                tc::fence_proxy_async();
+                tc::mbar_arrive(&bars.p_full[th]);
+            }
+
+            // ---- epilogue of the segment ----
+            // l per row: its four threads (two lanes 16 apart in a warp of each group) meet at the last reference
+            if (ok) ok = tc::mbar_wait_warp(&bars.pv_done[(i1 - 1) & 1], ((i1 - 1) >> 1) & 1, abort_flag, 66, max_polls);
+            failed = tc::barrier_any(1, TM_SOFTMAX, !ok);  // (all leave the loop over segments together)
+            {
+                const float m_now = s_mref[hd];
+                if (m_now != m_ref) { l_acc *= exp2f(m_ref - m_now); m_ref = m_now; }
+                const float mine = l_acc + __shfl_xor_sync(0xffffffffu, l_acc, 16);
+                if (lane < 16) s_wmax[th * 64 + hd] = mine;
+            }
+            tc::named_barrier(1, TM_SOFTMAX);
+            tc::tc_fence_after();
+            const float l = s_wmax[hd] + s_wmax[64 + hd];
+            const bool whole = w.t0 == 0 && w.t1 == w.nt;
+            if (whole) {
+                if (th == 0 && lane < 16) {
+                    // (l and O carry 2^5; NaN stays NaN)
+                    if (hd < valid && A.out_lse)
+                        A.out_lse[flat + hd] = l == 0.0f ? -INFINITY : (m_ref - TM_POFF) * 0.6931471805599453f + logf(l);
+                    s_fac[hd] = l == 0.0f ? 0.0f : 1.0f / l;
+                }
+                tc::named_barrier(1, TM_SOFTMAX);
+                // eight rows at a time through the group's staging, and out as one bulk copy
+                uint16_t* stage = reinterpret_cast<uint16_t*>(smem + SM_OUT + th * 8192);
+#pragma unroll 1
+                for (int g = 0; g < 4; ++g) {
+                    const int hg = th * 32 + g * 8;
+                    uint32_t r[4][8];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tc::tmem_ld8(TM_O + lane_base + c * 64 + hg, r[c]);
+                    tc::tmem_ld_wait();
+                    if (sq == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    tc::named_barrier(4 + th, GROUP);      // the staging is free
+                    const float4 f0 = *reinterpret_cast<const float4*>(s_fac + hg), f1 = *reinterpret_cast<const float4*>(s_fac + hg + 4);
+                    const float inv_l[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+                    uint16_t* sp = stage + orow;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int k = 0; k < 8; k += 2) {
+                            uint32_t w2;
+                            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w2) : "f"(__uint_as_float(r[c][k + 1]) * inv_l[k + 1]), "f"(__uint_as_float(r[c][k]) * inv_l[k]));
+                            sp[k * TM_KVL + c * 128] = (uint16_t)w2;
+                            sp[(k + 1) * TM_KVL + c * 128] = (uint16_t)(w2 >> 16);
+                        }
+                    tc::fence_proxy_async();
+                    tc::named_barrier(4 + th, GROUP);
+                    const int n = min(8, valid - hg);
+                    if (sq == 0 && lane == 0 && n > 0) {
+                        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
+                                     ::"l"(A.out + (flat + hg) * TM_KVL), "r"(tc::smem_u32(stage)), "r"(n * TM_KVL * 2) : "memory");
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                }
+            } else {
+                // a part: O as it is, its references and sums, for the joining kernel
+                const int slot = 2 * blockIdx.x + (w.t0 == 0 ? 1 : 0);
+                if (th == 0 && lane < 16)
+                    reinterpret_cast<float2*>(scratch + SC_ML)[slot * TM_ROWS + hd] = make_float2(m_ref, l);
+                float* po = reinterpret_cast<float*>(scratch + SC_O) + (size_t)slot * TM_ROWS * TM_KVL;
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t r[32];
+                    tc::tmem_ld32(TM_O + lane_base + c * 64 + th * 32, r);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int h = 0; h < 32; ++h)
+                        po[(size_t)(th * 32 + h) * TM_KVL + c * 128 + orow] = __uint_as_float(r[h]);
+                }
+                if (w.t0 == 0 && tid == 0) {
+                    // this CTA has the block's beginning: which runs hold the rest
+                    const long long total = s_units[1], end = run_begin(total, blockIdx.x + 1, s_run[3]) + (w.nt - w.t1) - 1;   // the block's last unit
+                    int last = (int)(end * s_run[3] / total);
+                    while (run_begin(total, last + 1, s_run[3]) <= end) ++last;
+                    Head h{(int32_t)flat, valid, last - (int)blockIdx.x + 1, 0};
+                    reinterpret_cast<Head*>(scratch + SC_HEAD)[blockIdx.x] = h;
+                    w.left = -1;                           // (told; the walk ends here in any case)
+                }
+            }
+            tc::tc_fence_before();
+        }
+        if (sq == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        // no block begins in this run and ends in another: nothing for the joining kernel
+        if (tid == 0 && w.left >= 0) {
+            Head h{0, 0, 0, 0};
+            reinterpret_cast<Head*>(scratch + SC_HEAD)[blockIdx.x] = h;
+        }
+    }
+
+    tc::tc_fence_before();
+    __syncthreads();
+    if (warp == TM_QKW) {
+        tc::settle(*abort_flag);
+        tc::tmem_dealloc<512>(tmem);
+    }
+    if (tid == 0 && *abort_flag) atomicCAS(err, 0, *abort_flag);
+}
+
+// Joins the parts of the row block whose beginning CTA blockIdx.x of the kernel before left, eight of its rows per block: a warp per row.
+__global__ void __launch_bounds__(256)
+tree_join_kernel(const uint8_t* scratch, uint16_t* out, float* out_lse) {
+    rv_grid_dep_wait();
+    rv_grid_dep_trigger();
+    const int g = blockIdx.x, row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const Head h = reinterpret_cast<const Head*>(scratch + SC_HEAD)[g];
+    if (row >= h.valid) return;
+    auto slot = [&](int p) { return p == 0 ? 2 * g + 1 : 2 * (g + p); };
+    const float2* ml = reinterpret_cast<const float2*>(scratch + SC_ML);
+    float m = -INFINITY, l = 0.0f;
+    for (int p = 0; p < h.parts; ++p) m = fmaxf(m, ml[slot(p) * TM_ROWS + row].x);
+    float4 acc[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p = 0; p < h.parts; ++p) {
+        const float2 part = ml[slot(p) * TM_ROWS + row];
+        if (part.x == -INFINITY && part.y == 0.0f) continue;       // the part saw nothing
+        const float f = exp2f(part.x - m);
+        l += part.y * f;
+        const float4* o = reinterpret_cast<const float4*>(scratch + SC_O) + ((size_t)slot(p) * TM_ROWS + row) * (TM_KVL / 4);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const float4 x = o[c * 32 + lane];
+            acc[c].x = fmaf(x.x, f, acc[c].x); acc[c].y = fmaf(x.y, f, acc[c].y);
+            acc[c].z = fmaf(x.z, f, acc[c].z); acc[c].w = fmaf(x.w, f, acc[c].w);
+        }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint2* to = reinterpret_cast<uint2*>(out + ((size_t)h.row0 + row) * TM_KVL);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        uint2 v;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v.x) : "f"(acc[c].y * inv), "f"(acc[c].x * inv));
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v.y) : "f"(acc[c].w * inv), "f"(acc[c].z * inv));
+        to[c * 32 + lane] = v;
+    }
+    if (out_lse && lane == 0) out_lse[h.row0 + row] = l == 0.0f ? -INFINITY : (m - TM_POFF) * 0.6931471805599453f + logf(l);
+}
+
+}  // namespace
+
+bool rv_tree_mma_supported(const DsaGeom* g) { return g->kv_lora == TM_KVL && g->rope_dim == TM_ROPE; }
+size_t rv_tree_mma_scratch_bytes() { return SC_TOTAL; }
+
+int rv_tree_mma(const TreeArgs& a, void* scratch, cudaStream_t st) {
+    rv_allow_smem<tree_mma_kernel>(SM_TOTAL);
+    const int sms = rv_sm_count(), grid = sms < RV_SMS ? sms : RV_SMS;   // (the scratch holds the parts of RV_SMS runs)
+    rv_drain_error();
+    uint8_t* s = reinterpret_cast<uint8_t*>(scratch);
+    rv_launch_dependent(tree_mma_kernel, dim3(grid), dim3(TM_THREADS), (size_t)SM_TOTAL, st, a, reinterpret_cast<int*>(s), s, tc::kMaxPolls);
+    if (int e = rv_launch_status()) return e;
+    rv_launch_dependent(tree_join_kernel, dim3(grid, TM_ROWS / 8), dim3(256), 0, st, (const uint8_t*)s, a.out, a.out_lse);
+    return rv_launch_status();
+}

@@ -169,12 +169,13 @@ def run_tree(be, cache, H, prefix, trees, masks, rows=None, n_rows=None, tree_po
         n = max(0, min(n, cap if dense else len(rows[b])))
         at = orc.tree_rows(cache.table[b], cache.page, cache.n_pages, n, None if dense else rows[b], tree_pos[b], T)
         unit = 2.0 ** -8 / math.sqrt(3)
-        want, want_lse, by_score, lse_by, by_weight, weight = orc.tree_attend(q[a:a + T].double().numpy(), cache.codes, cache.scale, at, n,
-                                                                              masks[a:a + T], float(np.float32(g.softmax_scale)), kvl, unit)
+        want, want_lse, by_score, lse_by, by_weight, weight, step, by_step = orc.tree_attend(
+            q[a:a + T].double().numpy(), cache.codes, cache.scale, at, n, masks[a:a + T], float(np.float32(g.softmax_scale)), kvl, unit)
         # The query as two 8-bit terms is off by up to 2^-8 relative in every entry (uniform: deviation 2^-8 / sqrt 3), which moves the
         # scores, six deviations at most; the weights as two terms by up to 2^-8 each; the result by half a bf16 step, 2^-8.
-        # 2^-18 and 2^-16: the terms' last place below an entry 2^-10 of the largest, 32-bit exponents and sums.
-        tol = 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 2.0 ** -16) * weight + 6 * by_score + 1e-30
+        # 2^-16: 32-bit exponents and sums. A weight times its row's scale is at most 2^8 and the largest at least 2^5 in units whose
+        # 8-bit terms go down in steps of 2^-9: all are off by up to 2^-10 besides, 2^-15 of the largest.
+        tol = 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 2.0 ** -16) * weight + 6 * by_score + 2.0 ** -15 * step + 1e-30
         assert (np.abs(got[a:a + T] - want) <= tol).all(), (b, (np.abs(got[a:a + T] - want) / tol).max())
         none = np.isinf(want_lse)
         assert (got_lse[a:a + T][none] == -np.inf).all() and (got[a:a + T][none] == 0).all()
@@ -182,8 +183,8 @@ def run_tree(be, cache, H, prefix, trees, masks, rows=None, n_rows=None, tree_po
         assert (np.abs(got_lse[a:a + T][~none] - want_lse[~none]) <= lse_tol[~none]).all()
         tols.append((tol, lse_tol))
         err2 += ((got[a:a + T] - want) ** 2).sum()
-        norm2 += ((unit * want) ** 2 + by_score ** 2 + by_weight ** 2).sum()
-    # the squares of the three add up; a sum over few heads and rows may come out at three times its mean's root
+        norm2 += ((unit * want) ** 2 + by_score ** 2 + by_weight ** 2 + (2.0 ** -15 * by_step) ** 2).sum()
+    # the squares add up; a sum over few heads and rows may come out at three times its mean's root
     assert math.sqrt(err2) <= 3 * math.sqrt(norm2) + 1e-30
     return out, lse, args, tols
 
@@ -237,6 +238,25 @@ def test_unmapped_pages_are_seen_by_nobody(be):
     cache.table[2, :] = -1                       # nothing at all
     masks = [m for t in (6, 10, 5) for m in masks_of(host, t, "tree")]
     run_tree(be, cache, 64, [490, 383, 80], [6, 10, 5], masks)
+
+
+@pytest.mark.parametrize("kvl", [512, 256])
+def test_a_node_that_is_nan_reaches_its_descendants_alone(be, kvl):
+    """NaN codes, and a NaN scale, in rows of the tree: nodes that do not see them give what they gave."""
+    cache = Cache(21, [100, 70], 64, kvl)
+    masks = [0b1, 0b11, 0b101, 0b1101, 0b10011] + [0b1, 0b11, 0b101]
+    out, lse, args, _ = run_tree(be, cache, 64, [95, 62], [5, 3], masks, kvl=kvl)
+    at = orc.tree_rows(cache.table[0], 64, cache.n_pages, 0, None, 95, 5)
+    bt = orc.tree_rows(cache.table[1], 64, cache.n_pages, 0, None, 62, 3)
+    codes, scale = args[2].clone(), args[3].clone()
+    codes[at[1], 7], codes[at[1], 300], codes[at[3], kvl + 5] = 0x7f, 0xff, 0x7f       # seen by nodes 1 and 4, and by node 3
+    scale[bt[1]], scale[bt[2]] = math.nan, math.inf                                    # by nodes 1 and 2 of the second
+    again, lse2 = torch.zeros_like(out), torch.zeros_like(lse)
+    be.launch_mla_tree_attend_paged_bf16(args[0], args[1], codes, scale, *args[4:13], again, lse2, *args[15:])
+    for node in (0, 2, 5):
+        assert torch.equal(again[node], out[node]) and torch.equal(lse2[node], lse[node])
+    for node in (1, 3, 4, 6, 7):
+        assert lse2[node].isnan().all() or (lse2[node] == math.inf).all() or again[node].isnan().any(), node
 
 
 def test_rows_that_no_node_may_see_do_not_matter(be):
