@@ -46,4 +46,18 @@ inline int make_tmap_rows_sw128(CUtensorMap* out, const void* base, uint64_t row
     return r == CUDA_SUCCESS ? 0 : 1008;
 }
 
+// rows x row_bytes bytes, loaded as boxes of box_rows rows of `columns` bytes (64 or 128: one swizzle row of that width).
+inline int make_tmap_columns(CUtensorMap* out, const void* base, uint64_t rows, uint32_t row_bytes, uint32_t columns, uint32_t box_rows) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return 1008;
+    const cuuint64_t dims[2] = {row_bytes, rows};
+    const cuuint64_t strides[1] = {row_bytes};
+    const cuuint32_t box[2] = {columns, box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, columns == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : 1008;
+}
+
 }  // namespace rivoli

@@ -124,7 +124,7 @@ RIVOLI_API int rivoli_mla_tree_attend_paged_bf16(const DsaGeom* g, const uint16_
     if (B <= 0 || n_nodes <= 0 || !q || !latent_pool || !latent_scale || !block_table || !tree_pos || !node_start || !node_mask || !out)
         return 1001;
     if (rows && (row_stride <= 0 || !n_rows)) return 1001;
-    if ((long long)n_nodes * g->n_heads > 0x7fffffffLL / 2 || (long long)g->n_pool_pages * g->page_tokens > 0xfffffffeLL) return 1002;
+    if ((long long)n_nodes * g->n_heads > 0x7fffffffLL / 2 || (long long)g->n_pool_pages * g->page_tokens > 0x7fffffffLL) return 1002;
     if ((((uintptr_t)latent_pool | (uintptr_t)q | (uintptr_t)out | (uintptr_t)scratch) & 15) || ((uintptr_t)node_mask & 7)) return 1005;
     const TreeArgs a{q, latent_pool, latent_scale, block_table, rows, row_stride, n_rows, tree_pos, node_start, node_mask, B, n_nodes,
                      g->n_heads, g->page_tokens, g->max_pages_per_seq, g->n_pool_pages, g->softmax_scale, out, out_lse};

@@ -24,6 +24,7 @@
 #include "common.cuh"
 #include "quant.cuh"
 #include "tc_common.cuh"
+#include "tmap.hpp"
 #include "tree_common.cuh"
 
 namespace {
@@ -59,6 +60,7 @@ constexpr int SM_TOTAL = SM_MISC + 64;
 static_assert(SM_TOTAL <= 232448, "shared memory budget");
 static_assert(SM_QR % 1024 == 0 && SM_P % 1024 == 0 && KSTAGE % 1024 == 0, "operand tiles are 1024-byte aligned");
 
+constexpr int KFULL = TM_GW * 33;                          // arrivals that fill a stage: the copies of 128 lanes, and each gather warp
 struct Bars {
     uint64_t k_full[TM_STAGES], k_empty[TM_STAGES], s_full[2], s_empty[2], p_full[2], pv_done[2], dec[2], q_full;
 };
@@ -79,6 +81,10 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo_bytes
     d |= (uint64_t)1 << 46;
     d |= (uint64_t)layout << 61;   // 2 = 128-byte swizzle, 4 = 64-byte swizzle
     return d;
+}
+
+__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(tc::smem_u32(bar)), "r"(n) : "memory");
 }
 
 // A walk over a run of (row block, tile) pairs. Units are numbered tile by tile, block by block, sequence by sequence.
@@ -111,7 +117,8 @@ __device__ __forceinline__ void walk_on(const TreeArgs& A, Walk& w) {
 __device__ __forceinline__ long long run_begin(long long total, int g, int n) { return total * g / n; }
 
 __global__ void __launch_bounds__(TM_THREADS, 1)
-tree_mma_kernel(TreeArgs A, int* err, uint8_t* scratch, int max_polls) {
+tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const __grid_constant__ CUtensorMap ropes, int box_rows, int* err, uint8_t* scratch,
+                int max_polls) {
     extern __shared__ __align__(1024) uint8_t smem[];
     Bars& bars = *reinterpret_cast<Bars*>(smem + SM_BARS);
     float* s_tok = reinterpret_cast<float*>(smem + SM_TOK);
@@ -127,7 +134,7 @@ tree_mma_kernel(TreeArgs A, int* err, uint8_t* scratch, int max_polls) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
 #pragma unroll
-        for (int s = 0; s < TM_STAGES; ++s) { tc::mbar_init(&bars.k_full[s], 33); tc::mbar_init(&bars.k_empty[s], 1); }
+        for (int s = 0; s < TM_STAGES; ++s) { tc::mbar_init(&bars.k_full[s], KFULL); tc::mbar_init(&bars.k_empty[s], 1); }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             tc::mbar_init(&bars.s_full[s], 2); tc::mbar_init(&bars.s_empty[s], TM_SW / 2);
@@ -158,15 +165,15 @@ tree_mma_kernel(TreeArgs A, int* err, uint8_t* scratch, int max_polls) {
             for (int o = 1; o < 32; o <<= 1) { const long long v = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += v; }
             return mine;
         };
-        long long total = 0, inc;
-        for (int b0 = 0; b0 < A.B; b0 += 32) { scan(b0 + lane, inc); total += __shfl_sync(0xffffffffu, inc, 31); }
+        long long total = 0, inc = 0, mine = 0;
+        for (int b0 = 0; b0 < A.B; b0 += 32) { mine = scan(b0 + lane, inc); total += __shfl_sync(0xffffffffu, inc, 31); }
         const int n = (int)max(1LL, min((long long)gridDim.x, total / TM_MIN_UNITS)), g = blockIdx.x;
         const long long u0 = g < n ? run_begin(total, g, n) : total, u1 = g < n ? run_begin(total, g + 1, n) : total;
         if (lane == 0) { s_units[0] = u1 - u0; s_units[1] = total; s_run[0] = A.B; s_run[1] = s_run[2] = 0; s_run[3] = n; }
         __syncwarp();
         long long before = 0;
         for (int b0 = 0; b0 < A.B && u1 > u0; b0 += 32) {
-            const long long mine = scan(b0 + lane, inc);
+            if (A.B > 32) mine = scan(b0 + lane, inc);     // (a batch of 32 is scanned already)
             if (u0 >= before + inc - mine && u0 < before + inc) {
                 int nt, nrb;
                 units_of(A, tree_seq(A, b0 + lane), nt, nrb);
@@ -184,93 +191,177 @@ tree_mma_kernel(TreeArgs A, int* err, uint8_t* scratch, int max_polls) {
 
     if (warp >= TM_GW0) {
         // ------------------------------ gather ---------------------------------------------------
-        // A tile per warp in turn; a lane resolves two rows (entry -> page -> pool row -> scale), one of the warp's tiles ahead, and
-        // the copies go row by row with 32 lanes on 32 consecutive 16-byte chunks. No warp waits for its copies: they signal the
+        // Tiles that lie wholly in a dense prefix are a few tensor copies (a page's rows each), a tile per warp in turn. Tiles of a row
+        // list, and those that hold rows of the tree or end inside, are gathered by all four warps together, sixteen rows each: the
+        // copies go row by row with 32 lanes on 32 consecutive 16-byte chunks (one warp per tile took 5,200 cycles to issue them, and a
+        // stage was held for that long more: 2,500 cycles a tile with five stages). No warp waits for its copies: they signal the
         // stage themselves. Rows past the end and on unmapped pages are written as zeros.
-        const int g = warp - TM_GW0;
+        const int g = warp - TM_GW0, shift = rv_log2(A.page_tokens);
         constexpr uint32_t NONE = 0xffffffffu;
         bool ok = true;
         int c0 = 0;                                // tiles of the CTA before this segment
+        // scale, log2 and reciprocal of a token of stage s
+        auto token_words = [&](int s, int slot, uint32_t r, float scl, bool nan) {
+            const bool live = r != NONE && !(scl <= 0.0f);
+            const float sc = nan ? __int_as_float(0x7fffffff) : scl;
+            float* tp = s_tok + s * TM_TILE + slot;
+            tp[0] = live ? sc : 0.0f;
+            tp[TOKPLANE / 4] = live ? __log2f(sc) + TM_POFF : -INFINITY;
+            // (0 for a NaN: times a weight that is NaN itself where the row is seen, times 0 where it is hidden)
+            tp[2 * (TOKPLANE / 4)] = live && sc == sc ? __frcp_rn(sc) : 0.0f;
+        };
         for (; ok && walk_segment(A, w); c0 += w.t1 - w.t0, walk_on(A, w)) {
             const int total = w.s.n + w.s.T;
-            auto locate = [&](int t, uint32_t* row, float* scl) {
+            {   // the block's queries on their way to L2: they are read when the softmax warps come to this segment
+                const int r0 = w.rb * TM_ROWS, bytes = min(TM_ROWS, w.s.T * A.H - r0) * TM_W * 2;
+                const char* at = reinterpret_cast<const char*>(A.q + ((size_t)w.s.node0 * A.H + r0) * TM_W);
+                for (int o = (g * 32 + lane) * 128; o < bytes; o += TM_GW * 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + o));
+            }
+            const int tj = box_rows && !w.s.listed ? max(w.t0, min(w.t1, w.s.n / TM_TILE)) : w.t0;   // tiles from here on are gathered
+            {
+                const int32_t* table = A.block_table + (size_t)w.b * A.max_pages;
+                auto page_of = [&](int t, int k) -> int {     // page of the k-th box of tile t; -1: none
+                    const int lp = (t * TM_TILE + k * box_rows) >> shift;
+                    const int pg = t < tj && lp < A.max_pages ? table[lp] : -1;
+                    return pg >= 0 && pg < A.n_pool_pages ? pg : -1;
+                };
+                auto row_of = [&](int t, int pg, int u) -> uint32_t {   // pool row of the lane's u-th token
+                    const int slot = u * 32 + lane, mine = __shfl_sync(0xffffffffu, pg, slot / box_rows);
+                    return mine >= 0 ? (uint32_t)mine * (uint32_t)A.page_tokens + (uint32_t)((t * TM_TILE + slot) & (A.page_tokens - 1)) : NONE;
+                };
+                const int boxes = tj > w.t0 ? TM_TILE / box_rows : 0;
+                int t = w.t0 + ((g - c0) & (TM_GW - 1));
+                int pg = -1, pg_next = -1;
+                float scl[2] = {0.0f, 0.0f};
+                if (boxes) {
+                    if (lane < boxes) { pg = page_of(t, lane); pg_next = page_of(t + TM_GW, lane); }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int j = t * TM_TILE + u * 32 + lane;
-                    row[u] = t < w.t1 && j < total ? tree_pool_row(A, w.b, tree_token(A, w.s, w.b, j)) : NONE;
+                    for (int u = 0; u < 2; ++u) { const uint32_t r = row_of(t, pg, u); if (r != NONE) scl[u] = A.pscale[r]; }
                 }
+                for (; t < tj; t += TM_GW) {
+                    const int i = c0 + t - w.t0, s = i % TM_STAGES, use = i / TM_STAGES;
+                    if (use > 0) ok = tc::mbar_wait_warp(&bars.k_empty[s], (use & 1) ^ 1, abort_flag, 41, max_polls);
+                    if (!ok) break;
+                    const uint32_t kbuf = tc::smem_u32(smem + SM_K + s * KSTAGE);
+                    const uint32_t mapped = __ballot_sync(0xffffffffu, lane < boxes && pg >= 0);
+                    if (lane == 0) tc::mbar_arrive_expect_tx(&bars.k_full[s], __popc(mapped) * box_rows * TM_W);
+                    __syncwarp();
+                    if (lane < boxes && pg >= 0) {
+                        const int y = pg * A.page_tokens + ((t * TM_TILE + lane * box_rows) & (A.page_tokens - 1));
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            tc::tma_load_2d(kbuf + c * KCHUNK + lane * box_rows * 128, &latents, c * 128, y, &bars.k_full[s]);
+                        tc::tma_load_2d(kbuf + 4 * KCHUNK + lane * box_rows * 64, &ropes, TM_KVL, y, &bars.k_full[s]);
+                    }
+                    if (mapped != (boxes == 32 ? ~0u : (1u << boxes) - 1)) {       // pages that are not there: zeros
+                        for (int x = lane; x < TM_TILE * 36; x += 32) {
+                            const int r = x / 36, c = x - r * 36;
+                            if ((mapped >> (r / box_rows)) & 1) continue;
+                            *reinterpret_cast<uint4*>(smem + SM_K + s * KSTAGE + (c < 32 ? (c >> 3) * KCHUNK + tc::sw128_chunk(r, c & 7) : 4 * KCHUNK + sw64_chunk(r, c - 32))) =
+                                make_uint4(0u, 0u, 0u, 0u);
+                        }
+                        tc::fence_proxy_async();
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) token_words(s, u * 32 + lane, row_of(t, pg, u), scl[u], false);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_n(&bars.k_full[s], KFULL - 1);
+                    pg = pg_next;
+                    pg_next = lane < boxes ? page_of(t + 2 * TM_GW, lane) : -1;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) { const uint32_t r = row_of(t + TM_GW, pg, u); scl[u] = r != NONE ? A.pscale[r] : 0.0f; }
+                }
+            }
+            // Four tiles at a time: a lane resolves one row of each of two of them. The words of the chain entry -> page -> scale are
+            // asked for a batch ahead, a level behind each of the batch's first tiles, and used a tile later at the earliest.
+            auto entry = [&](int tb, int u) -> uint32_t {
+                const int t = tb + 2 * u + (lane >> 4), j = t * TM_TILE + 16 * g + (lane & 15);
+                return t < w.t1 && j < total ? tree_token(A, w.s, w.b, j) : NONE;
+            };
+            auto page = [&](uint32_t tok) -> int {
+                return tok != NONE && (tok >> shift) < (uint32_t)A.max_pages ? A.block_table[(size_t)w.b * A.max_pages + (tok >> shift)] : -1;
+            };
+            auto pool_row = [&](uint32_t tok, int pg) -> uint32_t {
+                return pg >= 0 && pg < A.n_pool_pages ? (uint32_t)pg * (uint32_t)A.page_tokens + (tok & (uint32_t)(A.page_tokens - 1)) : NONE;
+            };
+            uint32_t row[2], tok_n[2] = {NONE, NONE}, row_n[2] = {NONE, NONE};
+            int pg_n[2] = {-1, -1};
+            float scl[2], scl_n[2] = {0.0f, 0.0f};
+            if (ok && tj < w.t1) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) tok_n[u] = entry(tj, u);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) row[u] = pool_row(tok_n[u], page(tok_n[u]));
 #pragma unroll
                 for (int u = 0; u < 2; ++u) scl[u] = row[u] != NONE ? A.pscale[row[u]] : 0.0f;
-            };
-            uint32_t row[2];
-            float scl[2];
-            int t = w.t0 + ((g - c0) & (TM_GW - 1));
-            locate(t, row, scl);
-            for (; t < w.t1; t += TM_GW) {
-                const int i = c0 + t - w.t0, s = i % TM_STAGES, use = i / TM_STAGES;
-                if (use > 0) ok = tc::mbar_wait_warp(&bars.k_empty[s], (use & 1) ^ 1, abort_flag, 41, max_polls);
-                if (!ok) break;
-                uint8_t* kbuf = smem + SM_K + s * KSTAGE;
-                uint8_t* rope = kbuf + 4 * KCHUNK;
-                uint32_t bad[2] = {0u, 0u};        // rows of the tree that hold a NaN code
-                if ((t + 1) * TM_TILE > w.s.n) {
-                    // 36 chunks a row: 32 latent, then four of the rope columns by the first four lanes
-#pragma unroll 1
-                    for (int it = 0; it < TM_TILE; ++it) {
-                        const uint32_t r = __shfl_sync(0xffffffffu, it < 32 ? row[0] : row[1], it & 31);
-                        const uint4* src = reinterpret_cast<const uint4*>(A.pool + (r != NONE ? (size_t)r * TM_W : 0));
-                        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-                        uint4 v = r != NONE ? src[lane] : zero, x = r != NONE && lane < 4 ? src[32 + lane] : zero;
-                        bool nan = false;
-                        if (t * TM_TILE + it >= w.s.n) {
-                            uint32_t* p[2] = {&v.x, &x.x};
+            }
+            for (int tb = tj; tb < w.t1 && ok; tb += 4) {
 #pragma unroll
-                            for (int h = 0; h < 2; ++h)
+                for (int u = 0; u < 2; ++u) tok_n[u] = entry(tb + 4, u);
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    // bytes whose low seven bits are all up
-                                    const uint32_t m = (((p[h][k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-                                    nan |= m != 0u;
-                                    p[h][k] &= ~(m * 0xffu);
-                                }
-                        }
-                        if (__ballot_sync(0xffffffffu, nan) && (it & 31) == lane) bad[it >> 5] = 1u;
-                        *reinterpret_cast<uint4*>(kbuf + (lane >> 3) * KCHUNK + tc::sw128_chunk(it, lane & 7)) = v;
-                        if (lane < 4) *reinterpret_cast<uint4*>(rope + sw64_chunk(it, lane)) = x;
-                    }
-                } else {
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
+                for (int k = 0; k < 4; ++k) {
+                    const int t = tb + k;
+                    if (t >= w.t1 || !ok) break;
+                    const int i = c0 + t - w.t0, s = i % TM_STAGES, use = i / TM_STAGES, l0 = 16 * (k & 1);
+                    if (use > 0) ok = tc::mbar_wait_warp(&bars.k_empty[s], (use & 1) ^ 1, abort_flag, 42, max_polls);
+                    if (!ok) break;
+                    uint8_t* kbuf = smem + SM_K + s * KSTAGE;
+                    uint8_t* rope = kbuf + 4 * KCHUNK;
 #pragma unroll 8
-                        for (int it = 0; it < 32; ++it) {
-                            const uint32_t r = __shfl_sync(0xffffffffu, row[u], it);
-                            tc::cp_async16_zfill(tc::smem_u32(kbuf + (lane >> 3) * KCHUNK + tc::sw128_chunk(u * 32 + it, lane & 7)),
-                                                 A.pool + (r != NONE ? (size_t)r * TM_W + lane * 16 : 0), r != NONE ? 16u : 0u);
-                        }
+                    for (int it = 0; it < 16; ++it) {
+                        const uint32_t r = __shfl_sync(0xffffffffu, row[k >> 1], l0 + it);
+                        tc::cp_async16_zfill(tc::smem_u32(kbuf + (lane >> 3) * KCHUNK + tc::sw128_chunk(16 * g + it, lane & 7)),
+                                             A.pool + (r != NONE ? (size_t)r * TM_W + lane * 16 : 0), r != NONE ? 16u : 0u);
                     }
 #pragma unroll
-                    for (int it = 0; it < 8; ++it) {
+                    for (int it = 0; it < 2; ++it) {
                         const int rl = it * 8 + (lane >> 2);
-                        const uint32_t r = __shfl_sync(0xffffffffu, row[it >> 2], rl & 31);
-                        tc::cp_async16_zfill(tc::smem_u32(rope + sw64_chunk(rl, lane & 3)),
+                        const uint32_t r = __shfl_sync(0xffffffffu, row[k >> 1], l0 + rl);
+                        tc::cp_async16_zfill(tc::smem_u32(rope + sw64_chunk(16 * g + rl, lane & 3)),
                                              A.pool + (r != NONE ? (size_t)r * TM_W + TM_KVL + (lane & 3) * 16 : 0), r != NONE ? 16u : 0u);
                     }
-                }
-                tc::cp_async_mbar_arrive_noinc(&bars.k_full[s]);
+                    bool bad = false;              // this lane's row holds a NaN code
+                    if ((t + 1) * TM_TILE > w.s.n) {
+                        // rows of the tree: each lane looks through the chunks that it copied itself, once they are there
+                        tc::cp_async_commit();
+                        tc::cp_async_wait<0>();
+                        auto clear = [&](uint8_t* at) -> bool {
+                            uint4 x = *reinterpret_cast<const uint4*>(at);
+                            // bytes whose low seven bits are all up
+                            auto nan = [](uint32_t v) { return ((v & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };
+                            const uint4 m = make_uint4(nan(x.x), nan(x.y), nan(x.z), nan(x.w));
+                            if (!(m.x | m.y | m.z | m.w)) return false;
+                            x.x &= ~((m.x >> 7) * 0xffu); x.y &= ~((m.y >> 7) * 0xffu); x.z &= ~((m.z >> 7) * 0xffu); x.w &= ~((m.w >> 7) * 0xffu);
+                            *reinterpret_cast<uint4*>(at) = x;
+                            return true;
+                        };
+                        const int first = w.s.n - t * TM_TILE - 16 * g, end = total - t * TM_TILE - 16 * g;
+#pragma unroll 4
+                        for (int it = max(0, first); it < min(16, end); ++it)
+                            if (__any_sync(0xffffffffu, clear(kbuf + (lane >> 3) * KCHUNK + tc::sw128_chunk(16 * g + it, lane & 7))) && (lane & 15) == it) bad = true;
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const bool live = row[u] != NONE && !(scl[u] <= 0.0f);
-                    const float sc = bad[u] ? __int_as_float(0x7fffffff) : scl[u];
-                    float* tp = s_tok + s * TM_TILE + u * 32 + lane;
-                    tp[0] = live ? sc : 0.0f;
-                    tp[TOKPLANE / 4] = live ? __log2f(sc) + TM_POFF : -INFINITY;
-                    // (0 for a NaN: times a weight that is NaN itself where the row is seen, times 0 where it is hidden)
-                    tp[2 * (TOKPLANE / 4)] = live && sc == sc ? __frcp_rn(sc) : 0.0f;
+                        for (int it = 0; it < 2; ++it) {
+                            const int rl = it * 8 + (lane >> 2);
+                            const uint32_t hit = __ballot_sync(0xffffffffu, rl >= first && rl < end && clear(rope + sw64_chunk(16 * g + rl, lane & 3)));
+                            if (((lane & 15) >> 3) == it && ((hit >> (4 * (lane & 7))) & 15u)) bad = true;
+                        }
+                    }
+                    tc::cp_async_mbar_arrive_noinc(&bars.k_full[s]);
+                    if ((lane >> 4) == (k & 1)) token_words(s, 16 * g + (lane & 15), row[k >> 1], scl[k >> 1], bad);
+                    tc::fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&bars.k_full[s]);
+                    if (k == 0) {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) pg_n[u] = page(tok_n[u]);
+                    }
+                    if (k == 1) {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) { row_n[u] = pool_row(tok_n[u], pg_n[u]); scl_n[u] = row_n[u] != NONE ? A.pscale[row_n[u]] : 0.0f; }
+                    }
                 }
-                tc::fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&bars.k_full[s]);
-                locate(t + TM_GW, row, scl);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) { row[u] = row_n[u]; scl[u] = scl_n[u]; }
             }
         }
     } else if (warp == TM_QKW) {
@@ -354,25 +445,52 @@ tree_mma_kernel(TreeArgs A, int* err, uint8_t* scratch, int max_polls) {
             const size_t flat = (size_t)w.s.node0 * A.H + r0;      // first row of the block in q, out and out_lse
             const uint64_t mask = hd < valid ? A.node_mask[w.s.node0 + (r0 + hd) / A.H] : 0ull;
             // ---- q -> two e4m3 terms per row: hi = e4m3(q / s), s = absmax / 448, lo = e4m3(q / s - hi) ----
-            // (warp half th takes that half of the columns; a lane the 128 latent and 16 rope values on its side tb; one shuffle a
-            // word gives each lane one term of both sides, a run of the row of its own tensor-memory lane)
+            // A warp takes sixteen rows and half th of their columns. They arrive as whole 128-byte lines (lanes 8 k .. 8 k + 7 on one row),
+            // are split there and go through shared memory, 64 columns at a time, to the lanes whose tensor-memory row they are. (A
+            // lane reading its own row, a line per load, waited 10,500 cycles for them.)
             {
-                const uint16_t* src = A.q + (flat + (hd < valid ? hd : 0)) * TM_W;
-                const uint4* l4 = reinterpret_cast<const uint4*>(src + th * (TM_KVL / 2) + tb * (TM_KVL / 4));
-                const uint4* r4 = reinterpret_cast<const uint4*>(src + TM_KVL + th * (TM_ROPE / 2) + tb * (TM_ROPE / 4));
+                const uint16_t* q0 = A.q + flat * TM_W;
                 uint4 v[18];
+                const int rq = 16 * sq + (lane >> 3), xq = 16 * sq + (lane >> 2);          // rows of a latent, of a rope load
 #pragma unroll
-                for (int c = 0; c < 18; ++c) v[c] = hd < valid ? (c < 16 ? l4[c] : r4[c - 16]) : make_uint4(0u, 0u, 0u, 0u);
-                uint32_t m = 0u;
+                for (int c = 0; c < 4; ++c)
 #pragma unroll
-                for (int c = 0; c < 18; ++c) m = rv_max_bf16x2(m, rv_absmax8(v[c]));
-                m = rv_max_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                if (tb == 0) s_wmax[th * 64 + hd] = __uint_as_float(m << 16);
+                    for (int k = 0; k < 4; ++k) {
+                        const int r = rq + 4 * k;
+                        v[4 * c + k] = r < valid ? *reinterpret_cast<const uint4*>(q0 + (size_t)r * TM_W + th * (TM_KVL / 2) + c * 64 + (lane & 7) * 8) : make_uint4(0u, 0u, 0u, 0u);
+                    }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int r = xq + 8 * k;
+                    v[16 + k] = r < valid ? *reinterpret_cast<const uint4*>(q0 + (size_t)r * TM_W + TM_KVL + th * (TM_ROPE / 2) + (lane & 3) * 8) : make_uint4(0u, 0u, 0u, 0u);
+                }
+                // largest magnitudes: of latent rows 4 k + lane / 8 and rope rows 8 k + lane / 4, then of row lane % 16
+                uint32_t ml4[4], mx2[2];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    ml4[k] = rv_max_bf16x2(rv_max_bf16x2(rv_absmax8(v[k]), rv_absmax8(v[4 + k])), rv_max_bf16x2(rv_absmax8(v[8 + k]), rv_absmax8(v[12 + k])));
+#pragma unroll
+                    for (int o = 1; o < 8; o <<= 1) ml4[k] = rv_max_bf16x2(ml4[k], __shfl_xor_sync(0xffffffffu, ml4[k], o));
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    mx2[k] = rv_absmax8(v[16 + k]);
+#pragma unroll
+                    for (int o = 1; o < 4; o <<= 1) mx2[k] = rv_max_bf16x2(mx2[k], __shfl_xor_sync(0xffffffffu, mx2[k], o));
+                }
+                {
+                    const int r = lane & 15;
+                    uint32_t a = 0u, x = 0u;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) { const uint32_t y = __shfl_sync(0xffffffffu, ml4[k], 8 * (r & 3)); if ((r >> 2) == k) a = y; }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) { const uint32_t y = __shfl_sync(0xffffffffu, mx2[k], 4 * (r & 7)); if ((r >> 3) == k) x = y; }
+                    if (lane < 16) s_wmax[th * 64 + hd] = __uint_as_float(rv_max_bf16x2(a, x) << 16);
+                }
                 tc::named_barrier(3, TM_SOFTMAX);          // (also: both groups are through with the block before)
-                const float amax = fmaxf(s_wmax[hd], s_wmax[64 + hd]);
-                const float sc = amax > 0.0f ? amax / 448.0f : 1.0f, inv = 1.0f / sc;
-                if (th == 0 && tb == 0) { s_ahi[hd] = sc * A.softmax_scale * 1.4426950408889634f; s_mref[hd] = -INFINITY; }
-                auto codes8 = [&](const uint4 x, uint2& hi, uint2& lo) {
+                auto scale_of = [&](int r) { const float amax = fmaxf(s_wmax[r], s_wmax[64 + r]); return amax > 0.0f ? amax / 448.0f : 1.0f; };
+                if (th == 0 && tb == 0) { s_ahi[hd] = scale_of(hd) * A.softmax_scale * 1.4426950408889634f; s_mref[hd] = -INFINITY; }
+                auto codes8 = [&](const uint4 x, float inv, uint2& hi, uint2& lo) {
                     const uint32_t ww[4] = {x.x, x.y, x.z, x.w};
                     uint16_t ch[4], cl[4];
 #pragma unroll
@@ -385,34 +503,45 @@ tree_mma_kernel(TreeArgs A, int* err, uint8_t* scratch, int max_polls) {
                     hi = make_uint2((uint32_t)ch[0] | ((uint32_t)ch[1] << 16), (uint32_t)ch[2] | ((uint32_t)ch[3] << 16));
                     lo = make_uint2((uint32_t)cl[0] | ((uint32_t)cl[1] << 16), (uint32_t)cl[2] | ((uint32_t)cl[3] << 16));
                 };
-                auto exchange = [&](const uint2 hi, const uint2 lo, uint32_t* first, uint32_t* second) {
-                    const uint2 keep = tb ? lo : hi, give = tb ? hi : lo;
-                    const uint2 got = make_uint2(__shfl_xor_sync(0xffffffffu, give.x, 16), __shfl_xor_sync(0xffffffffu, give.y, 16));
-                    first[0] = tb ? got.x : keep.x; first[1] = tb ? got.y : keep.y;
-                    second[0] = tb ? keep.x : got.x; second[1] = tb ? keep.y : got.y;
-                };
+                // 64 codes of 32 virtual rows (hi 0-15, lo 16-31) in this warp's 2 KiB of the staging, 16-byte chunks swizzled by row
+                uint8_t* buf = smem + SM_OUT + warp * 2048;
+                auto spot = [&](int r, int byte) { return buf + r * 64 + ((((byte >> 4) ^ (r >> 1)) & 3) << 4) + (byte & 15); };
+                if (lane == 0 && sq == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                tc::named_barrier(3, TM_SOFTMAX);          // the staging is free
                 const uint32_t dst = TM_Q + lane_base + th * 64;
+                float inv4[4];
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    uint32_t a0[8], a1[8];
+                for (int k = 0; k < 4; ++k) inv4[k] = 1.0f / scale_of(rq + 4 * k);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < 4; ++c) {
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
                         uint2 hi, lo;
-                        codes8(v[g * 4 + c], hi, lo);
-                        exchange(hi, lo, a0 + 2 * c, a1 + 2 * c);
+                        codes8(v[4 * c + k], inv4[k], hi, lo);
+                        const int r = 4 * k + (lane >> 3);
+                        *reinterpret_cast<uint2*>(spot(r, (lane & 7) * 8)) = hi;
+                        *reinterpret_cast<uint2*>(spot(16 + r, (lane & 7) * 8)) = lo;
                     }
-                    tc::tmem_st8(dst + g * 8, a0);
-                    tc::tmem_st8(dst + 32 + g * 8, a1);
-                }
-                uint32_t a0[4], a1[4];
+                    __syncwarp();
+                    uint32_t a[16];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint2 hi, lo;
-                    codes8(v[16 + c], hi, lo);
-                    exchange(hi, lo, a0 + 2 * c, a1 + 2 * c);
+                    for (int k = 0; k < 4; ++k) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(spot(lane, 16 * k));
+                        a[4 * k] = x.x; a[4 * k + 1] = x.y; a[4 * k + 2] = x.z; a[4 * k + 3] = x.w;
+                    }
+                    tc::tmem_st8(dst + c * 16, a);
+                    tc::tmem_st8(dst + c * 16 + 8, a + 8);
                 }
-                *reinterpret_cast<uint4*>(smem + SM_QR + sw64_chunk(orow, 2 * th)) = make_uint4(a0[0], a0[1], a0[2], a0[3]);
-                *reinterpret_cast<uint4*>(smem + SM_QR + sw64_chunk(orow, 2 * th + 1)) = make_uint4(a1[0], a1[1], a1[2], a1[3]);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {              // rope columns: straight to the operand tile, eight codes at a time
+                    const int r = 8 * k + (lane >> 2);
+                    uint2 hi, lo;
+                    codes8(v[16 + k], 1.0f / scale_of(16 * sq + r), hi, lo);
+                    const int col = th * 32 + (lane & 3) * 8;
+                    *reinterpret_cast<uint2*>(smem + SM_QR + sw64_chunk(sq * 32 + r, col >> 4) + (col & 15)) = hi;
+                    *reinterpret_cast<uint2*>(smem + SM_QR + sw64_chunk(sq * 32 + 16 + r, col >> 4) + (col & 15)) = lo;
+                }
                 tc::tmem_st_wait();
                 tc::fence_proxy_async();
                 tc::tc_fence_before();
@@ -562,14 +691,14 @@ tree_mma_kernel(TreeArgs A, int* err, uint8_t* scratch, int max_polls) {
             tc::tc_fence_after();
             const float l = s_wmax[hd] + s_wmax[64 + hd];
             const bool whole = w.t0 == 0 && w.t1 == w.nt;
+            if (whole && th == 0 && lane < 16) {
+                // (l and O carry 2^5; NaN stays NaN)
+                if (hd < valid && A.out_lse)
+                    A.out_lse[flat + hd] = l == 0.0f ? -INFINITY : (m_ref - TM_POFF) * 0.6931471805599453f + logf(l);
+                s_fac[hd] = l == 0.0f ? 0.0f : 1.0f / l;
+            }
+            tc::named_barrier(1, TM_SOFTMAX);              // (the sums are read: the next block's maxima take their place)
             if (whole) {
-                if (th == 0 && lane < 16) {
-                    // (l and O carry 2^5; NaN stays NaN)
-                    if (hd < valid && A.out_lse)
-                        A.out_lse[flat + hd] = l == 0.0f ? -INFINITY : (m_ref - TM_POFF) * 0.6931471805599453f + logf(l);
-                    s_fac[hd] = l == 0.0f ? 0.0f : 1.0f / l;
-                }
-                tc::named_barrier(1, TM_SOFTMAX);
                 // eight rows at a time through the group's staging, and out as one bulk copy
                 uint16_t* stage = reinterpret_cast<uint16_t*>(smem + SM_OUT + th * 8192);
 #pragma unroll 1
@@ -696,7 +825,15 @@ int rv_tree_mma(const TreeArgs& a, void* scratch, cudaStream_t st) {
     const int sms = rv_sm_count(), grid = sms < RV_SMS ? sms : RV_SMS;   // (the scratch holds the parts of RV_SMS runs)
     rv_drain_error();
     uint8_t* s = reinterpret_cast<uint8_t*>(scratch);
-    rv_launch_dependent(tree_mma_kernel, dim3(grid), dim3(TM_THREADS), (size_t)SM_TOTAL, st, a, reinterpret_cast<int*>(s), s, tc::kMaxPolls);
+    // tensor copies of a page's rows, 16 to 64 of them; smaller pages are gathered row by row
+    const int box = a.page_tokens < 16 ? 0 : (a.page_tokens < TM_TILE ? a.page_tokens : TM_TILE);
+    CUtensorMap latents{}, ropes{};
+    if (box) {
+        const uint64_t rows = (uint64_t)a.n_pool_pages * a.page_tokens;
+        if (int e = rivoli::make_tmap_columns(&latents, a.pool, rows, TM_W, 128, box)) return e;
+        if (int e = rivoli::make_tmap_columns(&ropes, a.pool, rows, TM_W, TM_ROPE, box)) return e;
+    }
+    rv_launch_dependent(tree_mma_kernel, dim3(grid), dim3(TM_THREADS), (size_t)SM_TOTAL, st, a, latents, ropes, box, reinterpret_cast<int*>(s), s, tc::kMaxPolls);
     if (int e = rv_launch_status()) return e;
     rv_launch_dependent(tree_join_kernel, dim3(grid, TM_ROWS / 8), dim3(256), 0, st, (const uint8_t*)s, a.out, a.out_lse);
     return rv_launch_status();
