@@ -5,21 +5,29 @@
 // The arithmetic is that of the decode step's attention (attend_mma.cu): cache rows are consumed as the e4m3 codes they are, q and the
 // softmax weights are two e4m3 terms each (2^-8 relative), a row's scale rides in its weight (P' = weight * scale * 2^5), references
 // lag behind the running maximum by at most 2^3, sums are f32. What differs is the shape of the work. The nodes of a tree share their
-// prefix, so that the rows of a sequence are nodes x heads, 64 to a block, and one tile of the cache serves them all: 240 products and
-// more per byte from a single node on and sixteen times that at sixteen nodes. The kernel is bound by the tensor cores and what feeds
-// them, the cache's tiles come from L2, and what has to be even is the number of (row block, tile) pairs per SM:
-//   * one persistent CTA per SM; the pairs of all sequences, in order, are cut into equal runs, one per CTA. A run that begins or ends
+// prefix, so that the rows of a sequence are nodes x heads, 128 to a block, and one tile of 64 cache rows serves them all: the kernel is
+// bound by the tensor cores and what feeds them.
+//   * A block of 128 rows is a PAIR of CTAs, 64 rows each, and its products are tcgen05 cta_group::2, issued by the pair's first CTA. The
+//     hi and lo terms of 64 rows are the 128 rows that a CTA has in S = Q . K^T (M = 256, N = 64 tokens: 32 of each CTA); O += P' . V is
+//     M = 128 (64 rows of each CTA, both halves of tensor memory's lanes taking half of the columns), N = 256 dims: 128 of each CTA. Each CTA
+//     feeds half of the shared operand and keeps softmax, references and O of its own rows to itself. A tile's 26 instructions take
+//     1,105 cycles (measured back to back: 32 and 66 cycles each), against 1,400 and more for one CTA on its own, whose O^T += V^T . P'
+//     with 64 columns reads shared memory for longer than it multiplies.
+//   * The (row block, tile) pairs of all sequences, in order, are cut into equal runs, one per pair of CTAs. A run that begins or ends
 //     inside a row block leaves that block's (maximum, sum, O) in scratch and a second, small kernel joins the parts; all others are
 //     written directly. No sequence is too long and no batch too ragged for this.
-//   * barriers and their phases run on over the row blocks of a CTA: the gather fetches the next block's tiles while this one's output
-//     is written.
+//   * Barriers and their phases run on over the row blocks: the next block's tiles are fetched while this one's output is written.
+//   * The rows of a tile come as K (the CTA's 32 tokens, all columns; held until S is there) and V (all 64 tokens, the CTA's 256 columns; held
+//     until O is) in rings of their own. Tiles that lie in a dense prefix are tensor copies of page rows, others are gathered.
 // Rows of the tree are tested against each node's mask in the tiles that hold them, the last one or two of a sequence. A hidden row's
-// weight is 0, but 0 x NaN is NaN: NaN codes of tree rows are fetched as 0 and make the row's scale NaN instead, which only reaches the
-// nodes that see it.
+// weight is 0, but 0 x NaN is NaN: NaN codes of tree rows become 0 and make the row's scale NaN instead, which only reaches the nodes
+// that see it.
 //
-// Shared memory: a ring of five tiles of 64 rows (36 KiB), the rope columns of q, P' twice, 16 KiB of staging. Tensor memory: S twice
-// (64 columns each), q (128: its latent columns are the A operand of the QK products), O^T (4 x 64). Warps: 0-7 softmax and epilogue, 8 QK
-// issue, 9 PV issue, 10-13 gather. All waits are bounded (tc_common.cuh).
+// Tensor memory: S twice (64 columns each), q (128: its latent columns are the A operand of the QK products), O (256). Warps: 0-11 softmax
+// and epilogue in three groups that take the tiles in turn, 12 QK issue, 13 PV issue (in the pair's second CTA these two pass on that its
+// K and V are there), 14 gathers K, 15 gathers V. All waits are bounded (tc_common.cuh).
+#include <atomic>
+
 #include "codec.cuh"
 #include "common.cuh"
 #include "quant.cuh"
@@ -29,48 +37,53 @@
 
 namespace {
 
-constexpr int TM_TILE = 64, TM_ROWS = 64;            // cache rows of a tile, (node, head) rows of a block
+constexpr int TM_TILE = 64, TM_ROWS = 64, TM_BLOCK = 2 * TM_ROWS;   // cache rows of a tile; (node, head) rows of a CTA, of a pair
 constexpr int TM_KVL = 512, TM_ROPE = 64, TM_W = TM_KVL + TM_ROPE;
-constexpr int TM_STAGES = 5, TM_GW = 4, TM_SW = 8;
-constexpr int TM_QKW = TM_SW, TM_PVW = TM_SW + 1, TM_GW0 = TM_SW + 2;
-constexpr int TM_THREADS = (TM_GW0 + TM_GW) * 32, TM_SOFTMAX = TM_SW * 32;
+constexpr int TM_OWN = TM_TILE / 2;                  // tokens of a tile whose K a CTA holds
+constexpr int NK = 4, NV = 6, NG = 3;                // stages of K and of V; softmax groups, each with a P' buffer
+constexpr int TM_SW = 4 * NG, TM_QKW = TM_SW, TM_PVW = TM_SW + 1, TM_KW = TM_SW + 2, TM_VW = TM_SW + 3;
+constexpr int TM_THREADS = (TM_VW + 1) * 32, TM_SOFTMAX = TM_SW * 32, TM_GROUP = 128;
 constexpr float TM_POFF = 5.0f, TM_LAG = 3.0f;       // P' = 2^(s - ref + 5) <= 2^8, see attend_mma.cu
-constexpr int TM_MIN_UNITS = 4;                      // tiles a CTA takes at least, while there are few
+constexpr int TM_MIN_UNITS = 4;                      // tiles a pair takes at least, while there are few
+constexpr int TM_PAIRS = RV_SMS / 2;
 
 // tensor memory columns
 constexpr int TMC_S = 0, TMC_Q = 2 * TM_TILE, TMC_O = TMC_Q + TM_KVL / 4;
-static_assert(TMC_O + 4 * TM_ROWS == 512, "tensor memory budget");
+static_assert(TMC_O + 256 == 512, "tensor memory budget");
 
 // shared memory (bytes)
-constexpr int KCHUNK = 8192, KSTAGE = 4 * KCHUNK + 4096;    // four latent chunks [64 rows][128 B], 128-byte swizzle; rope [64][64 B], 64-byte swizzle
-constexpr int SM_K = 0;
-constexpr int SM_QR = SM_K + TM_STAGES * KSTAGE;            // rope columns of q: [128 virtual rows][64 B], 64-byte swizzle
-constexpr int SM_P = SM_QR + 8192;                          // twice {hi, lo} [64 rows][64 tokens], 64-byte swizzle
+constexpr int KCHUNK = TM_OWN * 128, KSTAGE = 4 * KCHUNK + TM_OWN * 64;   // four latent chunks [32 tokens][128 B], 128-byte swizzle; rope [32][64 B], 64-byte swizzle
+constexpr int VCHUNK = TM_TILE * 128, VSTAGE = 2 * VCHUNK;                // two chunks [64 tokens][128 B]: columns 128 rank and 256 + 128 rank on
+constexpr int SM_V = 0;
+constexpr int SM_K = SM_V + NV * VSTAGE;
+constexpr int SM_QR = SM_K + NK * KSTAGE;                   // rope columns of q: [128 virtual rows][64 B], 64-byte swizzle
+constexpr int SM_P = SM_QR + 8192;                          // per group {hi, lo} [64 rows][64 tokens], 64-byte swizzle
 constexpr int PTERM = 4096, PBUF = 2 * PTERM;
-constexpr int SM_OUT = SM_P + 2 * PBUF;                     // staging: two groups of 8 rows x 512 bf16
-constexpr int SM_TOK = SM_OUT + 2 * 8192;                   // f32 [3][stages][64]: scale | log2(scale) + offset | 1 / scale
-constexpr int TOKPLANE = TM_STAGES * TM_TILE * 4;
+constexpr int SM_TOK = SM_P + NG * PBUF;                    // f32 [3][NV][64]: scale | log2(scale) + offset | 1 / scale
+constexpr int TOKPLANE = NV * TM_TILE * 4;
 constexpr int SM_AHI = SM_TOK + 3 * TOKPLANE;               // f32 [64] query scale * softmax scale * log2(e)
-constexpr int SM_WMAX = SM_AHI + 256;                       // f32 [2][64]
-constexpr int SM_FAC = SM_WMAX + 512;                       // f32 [64]
+constexpr int SM_WMAX = SM_AHI + 256;                       // f32 [3][64]
+constexpr int SM_FAC = SM_WMAX + 768;                       // f32 [64]
 constexpr int SM_MREF = SM_FAC + 256;                       // f32 [64]
 constexpr int SM_BARS = SM_MREF + 256;
-constexpr int SM_MISC = SM_BARS + 256;
+constexpr int SM_MISC = SM_BARS + 512;
 constexpr int SM_TOTAL = SM_MISC + 64;
 static_assert(SM_TOTAL <= 232448, "shared memory budget");
-static_assert(SM_QR % 1024 == 0 && SM_P % 1024 == 0 && KSTAGE % 1024 == 0, "operand tiles are 1024-byte aligned");
+static_assert(SM_K % 1024 == 0 && SM_QR % 1024 == 0 && SM_P % 1024 == 0 && KSTAGE % 1024 == 0, "operand tiles are 1024-byte aligned");
 
-constexpr int KFULL = TM_GW * 33;                          // arrivals that fill a stage: the copies of 128 lanes, and each gather warp
+// Barriers marked * are the first CTA's alone: both CTAs arrive there.
 struct Bars {
-    uint64_t k_full[TM_STAGES], k_empty[TM_STAGES], s_full[2], s_empty[2], p_full[2], pv_done[2], dec[2], q_full;
+    uint64_t k_full[NK], k_peer[NK] /* * */, k_empty[NK], v_full[NV], v_peer[NV] /* * */, v_empty[NV], tok_full[NV], s_full[NG], s_empty[2] /* * */,
+        p_full[NG] /* * */, pv_done[NG], dec[NG], q_full /* * */;
 };
-static_assert(sizeof(Bars) <= 256, "barrier block");
+static_assert(sizeof(Bars) <= 512, "barrier block");
+constexpr int FULL = 33;                                    // arrivals that fill a stage: the copies of 32 lanes, and the gathering warp
 
-// scratch: error word (256 bytes) | per CTA the block it is the first of, for the joining kernel | (reference, sum) of parts | O of parts
-constexpr int SLOTS = 2 * RV_SMS;                           // a CTA leaves at most the end of one block and the beginning of another
+// scratch: error word (256 bytes) | per pair the block it has the beginning of, for the joining kernel | (reference, sum) of parts | O of parts
+constexpr int SLOTS = 2 * TM_PAIRS;                         // a pair leaves at most the end of one block and the beginning of another
 struct Head { int32_t row0, valid, parts, pad; };
-constexpr size_t SC_HEAD = 256, SC_ML = SC_HEAD + RV_SMS * sizeof(Head), SC_O = (SC_ML + (size_t)SLOTS * TM_ROWS * 8 + 255) / 256 * 256;
-constexpr size_t SC_TOTAL = SC_O + (size_t)SLOTS * TM_ROWS * TM_KVL * 4;
+constexpr size_t SC_HEAD = 256, SC_ML = SC_HEAD + TM_PAIRS * sizeof(Head), SC_O = (SC_ML + (size_t)SLOTS * TM_BLOCK * 8 + 255) / 256 * 256;
+constexpr size_t SC_TOTAL = SC_O + (size_t)SLOTS * TM_BLOCK * TM_KVL * 4;
 
 __device__ __forceinline__ uint32_t sw64_chunk(uint32_t row, uint32_t chunk) { return row * 64u + ((chunk ^ ((row >> 1) & 3u)) << 4); }
 __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes, uint32_t layout) {
@@ -82,10 +95,38 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo_bytes
     d |= (uint64_t)layout << 61;   // 2 = 128-byte swizzle, 4 = 64-byte swizzle
     return d;
 }
-
 __device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(tc::smem_u32(bar)), "r"(n) : "memory");
 }
+// One arrival on the first CTA's barrier, from either CTA (`at`: its address there).
+__device__ __forceinline__ uint32_t in_first(const void* p) {
+    uint32_t at;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(tc::smem_u32(p)));
+    return at;
+}
+__device__ __forceinline__ void arrive_first(uint32_t at) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at) : "memory");
+}
+// The bounded wait for what the other CTA did.
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code, int max_polls) {
+    const uint32_t a = tc::smem_u32(bar);
+    bool done = false;
+    for (int it = 0; it < max_polls && !done; ++it) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(a), "r"(parity) : "memory");
+        done = ok != 0;
+        if (!done && (it & 63) == 63 && *abort_flag) break;
+    }
+    if (!done && !*abort_flag) *abort_flag = code;
+    return __all_sync(0xffffffffu, done);
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Bytes of a word whose low seven bits are all up (NaN codes), as their top bits.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t v) { return ((v & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
 // A walk over a run of (row block, tile) pairs. Units are numbered tile by tile, block by block, sequence by sequence.
 struct Walk {
@@ -95,7 +136,7 @@ struct Walk {
     TreeSeq s;
 };
 __device__ __forceinline__ void units_of(const TreeArgs& A, const TreeSeq& s, int& nt, int& nrb) {
-    nrb = (s.T * A.H + TM_ROWS - 1) / TM_ROWS;
+    nrb = (s.T * A.H + TM_BLOCK - 1) / TM_BLOCK;
     nt = s.T ? (s.n + s.T + TM_TILE - 1) / TM_TILE : 0;
 }
 __device__ __forceinline__ bool walk_segment(const TreeArgs& A, Walk& w) {
@@ -113,7 +154,7 @@ __device__ __forceinline__ void walk_on(const TreeArgs& A, Walk& w) {
     w.t0 = 0;
     if (++w.rb == w.nrb) { w.rb = 0; w.nrb = 0; }
 }
-// First unit of CTA g's run.
+// First unit of pair g's run.
 __device__ __forceinline__ long long run_begin(long long total, int g, int n) { return total * g / n; }
 
 __global__ void __launch_bounds__(TM_THREADS, 1)
@@ -128,33 +169,39 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
     float* s_mref = reinterpret_cast<float*>(smem + SM_MREF);
     uint32_t* tmem_base_s = reinterpret_cast<uint32_t*>(smem + SM_MISC);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + SM_MISC + 4);
-    int* s_run = reinterpret_cast<int*>(smem + SM_MISC + 8);               // b, rb, t0 of the run's beginning
+    int* s_run = reinterpret_cast<int*>(smem + SM_MISC + 8);               // b, rb, t0 of the run's beginning, number of runs
     long long* s_units = reinterpret_cast<long long*>(smem + SM_MISC + 24);   // its units, all units
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int pair = blockIdx.x >> 1, rank = blockIdx.x & 1;               // (clusters of two along x)
     if (tid == 0) {
 #pragma unroll
-        for (int s = 0; s < TM_STAGES; ++s) { tc::mbar_init(&bars.k_full[s], KFULL); tc::mbar_init(&bars.k_empty[s], 1); }
+        for (int s = 0; s < NK; ++s) { tc::mbar_init(&bars.k_full[s], FULL); tc::mbar_init(&bars.k_peer[s], 1); tc::mbar_init(&bars.k_empty[s], 1); }
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            tc::mbar_init(&bars.s_full[s], 2); tc::mbar_init(&bars.s_empty[s], TM_SW / 2);
-            tc::mbar_init(&bars.p_full[s], TM_SOFTMAX / 2); tc::mbar_init(&bars.pv_done[s], 1); tc::mbar_init(&bars.dec[s], TM_SW / 2);
+        for (int s = 0; s < NV; ++s) {
+            tc::mbar_init(&bars.v_full[s], FULL); tc::mbar_init(&bars.v_peer[s], 1); tc::mbar_init(&bars.v_empty[s], 1);
+            tc::mbar_init(&bars.tok_full[s], 1);
         }
-        tc::mbar_init(&bars.q_full, TM_SOFTMAX);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) tc::mbar_init(&bars.s_empty[s], 8);
+#pragma unroll
+        for (int s = 0; s < NG; ++s) { tc::mbar_init(&bars.s_full[s], 1); tc::mbar_init(&bars.p_full[s], 8); tc::mbar_init(&bars.pv_done[s], 1); tc::mbar_init(&bars.dec[s], 4); }
+        tc::mbar_init(&bars.q_full, 2 * TM_SW);
         tc::mbar_init_fence();
         *abort_flag = 0;
     }
-    if (warp == TM_QKW) tc::tmem_alloc<512>(tmem_base_s);
+    if (warp == TM_QKW) tc::tmem_alloc2(tmem_base_s);
     tc::fence_proxy_async();
     tc::tc_fence_before();
     __syncthreads();
+    cluster_sync();                                    // barriers and columns of both CTAs are there
     tc::tc_fence_after();
     const uint32_t tmem = *tmem_base_s;
     const uint32_t TM_S0 = tmem + TMC_S, TM_Q = tmem + TMC_Q, TM_O = tmem + TMC_O;
     rv_grid_dep_wait();
     rv_grid_dep_trigger();
 
-    // ------------------------------ the CTA's run ------------------------------------------------
+    // ------------------------------ the pair's run -----------------------------------------------
     if (warp == 0) {
         auto scan = [&](int b, long long& inc) {   // units of sequence b, and of all of its 32 up to it
             int nt = 0, nrb = 0;
@@ -167,7 +214,7 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
         };
         long long total = 0, inc = 0, mine = 0;
         for (int b0 = 0; b0 < A.B; b0 += 32) { mine = scan(b0 + lane, inc); total += __shfl_sync(0xffffffffu, inc, 31); }
-        const int n = (int)max(1LL, min((long long)gridDim.x, total / TM_MIN_UNITS)), g = blockIdx.x;
+        const int n = (int)max(1LL, min((long long)(gridDim.x / 2), total / TM_MIN_UNITS)), g = pair;
         const long long u0 = g < n ? run_begin(total, g, n) : total, u1 = g < n ? run_begin(total, g + 1, n) : total;
         if (lane == 0) { s_units[0] = u1 - u0; s_units[1] = total; s_run[0] = A.B; s_run[1] = s_run[2] = 0; s_run[3] = n; }
         __syncwarp();
@@ -189,18 +236,15 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
     w.nt = w.nrb = 0;
     if (w.left > 0) { w.s = tree_seq(A, w.b); units_of(A, w.s, w.nt, w.nrb); }
 
-    if (warp >= TM_GW0) {
+    if (warp == TM_KW || warp == TM_VW) {
         // ------------------------------ gather ---------------------------------------------------
-        // Tiles that lie wholly in a dense prefix are a few tensor copies (a page's rows each), a tile per warp in turn. Tiles of a row
-        // list, and those that hold rows of the tree or end inside, are gathered by all four warps together, sixteen rows each: the
-        // copies go row by row with 32 lanes on 32 consecutive 16-byte chunks (one warp per tile took 5,200 cycles to issue them, and a
-        // stage was held for that long more: 2,500 cycles a tile with five stages). No warp waits for its copies: they signal the
-        // stage themselves. Rows past the end and on unmapped pages are written as zeros.
-        const int g = warp - TM_GW0, shift = rv_log2(A.page_tokens);
+        // Warp 14 fetches K (this CTA's 32 tokens of a tile) and writes the scales of all 64, warp 15 fetches V. Neither waits for its
+        // copies: they signal the stage themselves. Rows past the end and on unmapped pages are written as zeros.
+        const bool is_k = warp == TM_KW;
+        const int shift = rv_log2(A.page_tokens);
         constexpr uint32_t NONE = 0xffffffffu;
         bool ok = true;
-        int c0 = 0;                                // tiles of the CTA before this segment
-        // scale, log2 and reciprocal of a token of stage s
+        int c0 = 0;                                // tiles of the pair before this segment
         auto token_words = [&](int s, int slot, uint32_t r, float scl, bool nan) {
             const bool live = r != NONE && !(scl <= 0.0f);
             const float sc = nan ? __int_as_float(0x7fffffff) : scl;
@@ -212,70 +256,16 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
         };
         for (; ok && walk_segment(A, w); c0 += w.t1 - w.t0, walk_on(A, w)) {
             const int total = w.s.n + w.s.T;
-            {   // the block's queries on their way to L2: they are read when the softmax warps come to this segment
-                const int r0 = w.rb * TM_ROWS, bytes = min(TM_ROWS, w.s.T * A.H - r0) * TM_W * 2;
+            {   // the queries of the CTA's rows on their way to L2: they are read when the softmax warps come to this segment
+                const int r0 = w.rb * TM_BLOCK + rank * TM_ROWS, bytes = min(TM_ROWS, w.s.T * A.H - r0) * TM_W * 2;
                 const char* at = reinterpret_cast<const char*>(A.q + ((size_t)w.s.node0 * A.H + r0) * TM_W);
-                for (int o = (g * 32 + lane) * 128; o < bytes; o += TM_GW * 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + o));
+                for (int o = ((is_k ? 0 : 32) + lane) * 128; o < bytes; o += 64 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + o));
             }
             const int tj = box_rows && !w.s.listed ? max(w.t0, min(w.t1, w.s.n / TM_TILE)) : w.t0;   // tiles from here on are gathered
-            {
-                const int32_t* table = A.block_table + (size_t)w.b * A.max_pages;
-                auto page_of = [&](int t, int k) -> int {     // page of the k-th box of tile t; -1: none
-                    const int lp = (t * TM_TILE + k * box_rows) >> shift;
-                    const int pg = t < tj && lp < A.max_pages ? table[lp] : -1;
-                    return pg >= 0 && pg < A.n_pool_pages ? pg : -1;
-                };
-                auto row_of = [&](int t, int pg, int u) -> uint32_t {   // pool row of the lane's u-th token
-                    const int slot = u * 32 + lane, mine = __shfl_sync(0xffffffffu, pg, slot / box_rows);
-                    return mine >= 0 ? (uint32_t)mine * (uint32_t)A.page_tokens + (uint32_t)((t * TM_TILE + slot) & (A.page_tokens - 1)) : NONE;
-                };
-                const int boxes = tj > w.t0 ? TM_TILE / box_rows : 0;
-                int t = w.t0 + ((g - c0) & (TM_GW - 1));
-                int pg = -1, pg_next = -1;
-                float scl[2] = {0.0f, 0.0f};
-                if (boxes) {
-                    if (lane < boxes) { pg = page_of(t, lane); pg_next = page_of(t + TM_GW, lane); }
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) { const uint32_t r = row_of(t, pg, u); if (r != NONE) scl[u] = A.pscale[r]; }
-                }
-                for (; t < tj; t += TM_GW) {
-                    const int i = c0 + t - w.t0, s = i % TM_STAGES, use = i / TM_STAGES;
-                    if (use > 0) ok = tc::mbar_wait_warp(&bars.k_empty[s], (use & 1) ^ 1, abort_flag, 41, max_polls);
-                    if (!ok) break;
-                    const uint32_t kbuf = tc::smem_u32(smem + SM_K + s * KSTAGE);
-                    const uint32_t mapped = __ballot_sync(0xffffffffu, lane < boxes && pg >= 0);
-                    if (lane == 0) tc::mbar_arrive_expect_tx(&bars.k_full[s], __popc(mapped) * box_rows * TM_W);
-                    __syncwarp();
-                    if (lane < boxes && pg >= 0) {
-                        const int y = pg * A.page_tokens + ((t * TM_TILE + lane * box_rows) & (A.page_tokens - 1));
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            tc::tma_load_2d(kbuf + c * KCHUNK + lane * box_rows * 128, &latents, c * 128, y, &bars.k_full[s]);
-                        tc::tma_load_2d(kbuf + 4 * KCHUNK + lane * box_rows * 64, &ropes, TM_KVL, y, &bars.k_full[s]);
-                    }
-                    if (mapped != (boxes == 32 ? ~0u : (1u << boxes) - 1)) {       // pages that are not there: zeros
-                        for (int x = lane; x < TM_TILE * 36; x += 32) {
-                            const int r = x / 36, c = x - r * 36;
-                            if ((mapped >> (r / box_rows)) & 1) continue;
-                            *reinterpret_cast<uint4*>(smem + SM_K + s * KSTAGE + (c < 32 ? (c >> 3) * KCHUNK + tc::sw128_chunk(r, c & 7) : 4 * KCHUNK + sw64_chunk(r, c - 32))) =
-                                make_uint4(0u, 0u, 0u, 0u);
-                        }
-                        tc::fence_proxy_async();
-                    }
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) token_words(s, u * 32 + lane, row_of(t, pg, u), scl[u], false);
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_n(&bars.k_full[s], KFULL - 1);
-                    pg = pg_next;
-                    pg_next = lane < boxes ? page_of(t + 2 * TM_GW, lane) : -1;
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) { const uint32_t r = row_of(t + TM_GW, pg, u); scl[u] = r != NONE ? A.pscale[r] : 0.0f; }
-                }
-            }
-            // Four tiles at a time: a lane resolves one row of each of two of them. The words of the chain entry -> page -> scale are
-            // asked for a batch ahead, a level behind each of the batch's first tiles, and used a tile later at the earliest.
-            auto entry = [&](int tb, int u) -> uint32_t {
-                const int t = tb + 2 * u + (lane >> 4), j = t * TM_TILE + 16 * g + (lane & 15);
+            // A lane's two tokens of a tile are 2 x 32 rows apart by 32: entry -> page -> pool row -> scale. The words are asked for a tile
+            // ahead each.
+            auto entry = [&](int t, int u) -> uint32_t {
+                const int j = t * TM_TILE + u * 32 + lane;
                 return t < w.t1 && j < total ? tree_token(A, w.s, w.b, j) : NONE;
             };
             auto page = [&](uint32_t tok) -> int {
@@ -284,168 +274,245 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
             auto pool_row = [&](uint32_t tok, int pg) -> uint32_t {
                 return pg >= 0 && pg < A.n_pool_pages ? (uint32_t)pg * (uint32_t)A.page_tokens + (tok & (uint32_t)(A.page_tokens - 1)) : NONE;
             };
-            uint32_t row[2], tok_n[2] = {NONE, NONE}, row_n[2] = {NONE, NONE};
-            int pg_n[2] = {-1, -1};
-            float scl[2], scl_n[2] = {0.0f, 0.0f};
-            if (ok && tj < w.t1) {
+            uint32_t row[2], tok1[2], tok2[2];     // rows of tile t; entries of tiles t + 1 and t + 2
+            int pg1[2];                            // pages of tile t + 1
+            float scl[2];                          // scales of tile t
 #pragma unroll
-                for (int u = 0; u < 2; ++u) tok_n[u] = entry(tj, u);
+            for (int u = 0; u < 2; ++u) { row[u] = entry(w.t0, u); tok1[u] = entry(w.t0 + 1, u); tok2[u] = entry(w.t0 + 2, u); }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) row[u] = pool_row(tok_n[u], page(tok_n[u]));
+            for (int u = 0; u < 2; ++u) { row[u] = pool_row(row[u], page(row[u])); pg1[u] = page(tok1[u]); }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) scl[u] = row[u] != NONE ? A.pscale[row[u]] : 0.0f;
-            }
-            for (int tb = tj; tb < w.t1 && ok; tb += 4) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u) tok_n[u] = entry(tb + 4, u);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int t = tb + k;
-                    if (t >= w.t1 || !ok) break;
-                    const int i = c0 + t - w.t0, s = i % TM_STAGES, use = i / TM_STAGES, l0 = 16 * (k & 1);
-                    if (use > 0) ok = tc::mbar_wait_warp(&bars.k_empty[s], (use & 1) ^ 1, abort_flag, 42, max_polls);
-                    if (!ok) break;
-                    uint8_t* kbuf = smem + SM_K + s * KSTAGE;
-                    uint8_t* rope = kbuf + 4 * KCHUNK;
+            for (int u = 0; u < 2; ++u) scl[u] = is_k && row[u] != NONE ? A.pscale[row[u]] : 0.0f;
+            for (int t = w.t0; t < w.t1; ++t) {
+                const int i = c0 + t - w.t0, sv = i % NV, usev = i / NV;
+                const int s = is_k ? i % NK : sv, use = is_k ? i / NK : usev;
+                uint64_t* full = is_k ? &bars.k_full[s] : &bars.v_full[s];
+                if (usev > 0) ok = tc::mbar_wait_warp(&bars.v_empty[sv], (usev & 1) ^ 1, abort_flag, 41, max_polls);   // (K: for the token words)
+                if (ok && is_k && use > 0) ok = tc::mbar_wait_warp(&bars.k_empty[s], (use & 1) ^ 1, abort_flag, 42, max_polls);
+                if (!ok) break;
+                uint8_t* buf = smem + (is_k ? SM_K + s * KSTAGE : SM_V + s * VSTAGE);
+                const bool tree_rows = (t + 1) * TM_TILE > w.s.n;
+                uint32_t bad[2] = {0u, 0u};        // this lane's rows that hold a NaN code
+                if (is_k && tree_rows) {
+                    // rows of the tree: 32 lanes look through a row at a time
+                    const int first = max(0, w.s.n - t * TM_TILE), end = min(TM_TILE, total - t * TM_TILE);
 #pragma unroll 8
-                    for (int it = 0; it < 16; ++it) {
-                        const uint32_t r = __shfl_sync(0xffffffffu, row[k >> 1], l0 + it);
-                        tc::cp_async16_zfill(tc::smem_u32(kbuf + (lane >> 3) * KCHUNK + tc::sw128_chunk(16 * g + it, lane & 7)),
-                                             A.pool + (r != NONE ? (size_t)r * TM_W + lane * 16 : 0), r != NONE ? 16u : 0u);
+                    for (int it = first; it < end; ++it) {
+                        const uint32_t r = __shfl_sync(0xffffffffu, it < 32 ? row[0] : row[1], it & 31);
+                        const uint4* src = reinterpret_cast<const uint4*>(A.pool + (r != NONE ? (size_t)r * TM_W : 0));
+                        uint4 v = src[lane], x = src[lane < 4 ? 32 + lane : 0];
+                        const uint32_t m = nan_bytes(v.x) | nan_bytes(v.y) | nan_bytes(v.z) | nan_bytes(v.w) |
+                                           (lane < 4 ? nan_bytes(x.x) | nan_bytes(x.y) | nan_bytes(x.z) | nan_bytes(x.w) : 0u);
+                        if (__any_sync(0xffffffffu, m != 0u) && (it & 31) == lane) bad[it >> 5] = 1u;
                     }
+                }
+                if (is_k) {
 #pragma unroll
-                    for (int it = 0; it < 2; ++it) {
-                        const int rl = it * 8 + (lane >> 2);
-                        const uint32_t r = __shfl_sync(0xffffffffu, row[k >> 1], l0 + rl);
-                        tc::cp_async16_zfill(tc::smem_u32(rope + sw64_chunk(16 * g + rl, lane & 3)),
-                                             A.pool + (r != NONE ? (size_t)r * TM_W + TM_KVL + (lane & 3) * 16 : 0), r != NONE ? 16u : 0u);
+                    for (int u = 0; u < 2; ++u) token_words(sv, u * 32 + lane, row[u], scl[u], bad[u] != 0u);
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&bars.tok_full[sv]);
+                }
+                if (t < tj) {
+                    // tensor copies: box k holds tokens k * box_rows on, of the CTA's 32 (K) or of all (V)
+                    const int boxes = (is_k ? TM_OWN : TM_TILE) / box_rows, slot = (is_k ? rank * TM_OWN : 0) + lane * box_rows;
+                    const uint32_t r0 = __shfl_sync(0xffffffffu, row[0], slot & 31), r1 = __shfl_sync(0xffffffffu, row[1], slot & 31);
+                    const uint32_t y = (slot & 32) ? r1 : r0;
+                    const bool mine = lane < boxes && y != NONE;
+                    const uint32_t mapped = __ballot_sync(0xffffffffu, mine);
+                    if (lane == 0) tc::mbar_arrive_expect_tx(full, __popc(mapped) * box_rows * (is_k ? TM_W : 256));
+                    __syncwarp();
+                    const uint32_t at = tc::smem_u32(buf);
+                    if (mine && is_k) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) tc::tma_load_2d(at + c * KCHUNK + lane * box_rows * 128, &latents, c * 128, (int)y, full);
+                        tc::tma_load_2d(at + 4 * KCHUNK + lane * box_rows * 64, &ropes, TM_KVL, (int)y, full);
+                    } else if (mine) {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) tc::tma_load_2d(at + c * VCHUNK + lane * box_rows * 128, &latents, (2 * c + rank) * 128, (int)y, full);
                     }
-                    bool bad = false;              // this lane's row holds a NaN code
-                    if ((t + 1) * TM_TILE > w.s.n) {
-                        // rows of the tree: each lane looks through the chunks that it copied itself, once they are there
-                        tc::cp_async_commit();
-                        tc::cp_async_wait<0>();
-                        auto clear = [&](uint8_t* at) -> bool {
-                            uint4 x = *reinterpret_cast<const uint4*>(at);
-                            // bytes whose low seven bits are all up
-                            auto nan = [](uint32_t v) { return ((v & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };
-                            const uint4 m = make_uint4(nan(x.x), nan(x.y), nan(x.z), nan(x.w));
-                            if (!(m.x | m.y | m.z | m.w)) return false;
-                            x.x &= ~((m.x >> 7) * 0xffu); x.y &= ~((m.y >> 7) * 0xffu); x.z &= ~((m.z >> 7) * 0xffu); x.w &= ~((m.w >> 7) * 0xffu);
-                            *reinterpret_cast<uint4*>(at) = x;
-                            return true;
-                        };
-                        const int first = w.s.n - t * TM_TILE - 16 * g, end = total - t * TM_TILE - 16 * g;
-#pragma unroll 4
-                        for (int it = max(0, first); it < min(16, end); ++it)
-                            if (__any_sync(0xffffffffu, clear(kbuf + (lane >> 3) * KCHUNK + tc::sw128_chunk(16 * g + it, lane & 7))) && (lane & 15) == it) bad = true;
-#pragma unroll
-                        for (int it = 0; it < 2; ++it) {
-                            const int rl = it * 8 + (lane >> 2);
-                            const uint32_t hit = __ballot_sync(0xffffffffu, rl >= first && rl < end && clear(rope + sw64_chunk(16 * g + rl, lane & 3)));
-                            if (((lane & 15) >> 3) == it && ((hit >> (4 * (lane & 7))) & 15u)) bad = true;
+                    if (__popc(mapped) != boxes) {             // pages that are not there: zeros
+                        const int chunks = is_k ? 36 : 16, rows = is_k ? TM_OWN : TM_TILE;
+                        for (int x = lane; x < rows * chunks; x += 32) {
+                            const int r = x / chunks, c = x - r * chunks;
+                            if ((mapped >> (r / box_rows)) & 1) continue;
+                            *reinterpret_cast<uint4*>(buf + (!is_k ? (c >> 3) * VCHUNK + tc::sw128_chunk(r, c & 7) : c < 32 ? (c >> 3) * KCHUNK + tc::sw128_chunk(r, c & 7)
+                                                                                                                              : 4 * KCHUNK + sw64_chunk(r, c - 32))) = make_uint4(0u, 0u, 0u, 0u);
                         }
                     }
-                    tc::cp_async_mbar_arrive_noinc(&bars.k_full[s]);
-                    if ((lane >> 4) == (k & 1)) token_words(s, 16 * g + (lane & 15), row[k >> 1], scl[k >> 1], bad);
                     tc::fence_proxy_async();
                     __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&bars.k_full[s]);
-                    if (k == 0) {
+                    if (lane == 0) mbar_arrive_n(full, FULL - 1);
+                } else {
+                    if (is_k) {
+                        const uint32_t own = rank ? row[1] : row[0];
+#pragma unroll 8
+                        for (int it = 0; it < TM_OWN; ++it) {
+                            const uint32_t r = __shfl_sync(0xffffffffu, own, it);
+                            tc::cp_async16_zfill(tc::smem_u32(buf + (lane >> 3) * KCHUNK + tc::sw128_chunk(it, lane & 7)),
+                                                 A.pool + (r != NONE ? (size_t)r * TM_W + lane * 16 : 0), r != NONE ? 16u : 0u);
+                        }
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) pg_n[u] = page(tok_n[u]);
-                    }
-                    if (k == 1) {
+                        for (int it = 0; it < 4; ++it) {
+                            const int rl = it * 8 + (lane >> 2);
+                            const uint32_t r = __shfl_sync(0xffffffffu, own, rl);
+                            tc::cp_async16_zfill(tc::smem_u32(buf + 4 * KCHUNK + sw64_chunk(rl, lane & 3)),
+                                                 A.pool + (r != NONE ? (size_t)r * TM_W + TM_KVL + (lane & 3) * 16 : 0), r != NONE ? 16u : 0u);
+                        }
+                    } else {
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) { row_n[u] = pool_row(tok_n[u], pg_n[u]); scl_n[u] = row_n[u] != NONE ? A.pscale[row_n[u]] : 0.0f; }
+                        for (int u = 0; u < 2; ++u) {
+#pragma unroll 8
+                            for (int it = 0; it < 16; ++it) {          // two rows an instruction, 16 chunks each
+                                const int rl = 2 * it + (lane >> 4), c = lane & 15;
+                                const uint32_t r = __shfl_sync(0xffffffffu, row[u], rl);
+                                tc::cp_async16_zfill(tc::smem_u32(buf + (c >> 3) * VCHUNK + tc::sw128_chunk(u * 32 + rl, c & 7)),
+                                                     A.pool + (r != NONE ? (size_t)r * TM_W + (2 * (c >> 3) + rank) * 128 + (c & 7) * 16 : 0), r != NONE ? 16u : 0u);
+                            }
+                        }
                     }
+                    if (tree_rows) {
+                        // NaN codes become 0: each lane looks through what it copied itself, once it is there (zeros in rows of the
+                        // prefix too would be wrong: those are seen by all)
+                        tc::cp_async_commit();
+                        tc::cp_async_wait<0>();
+                        auto clear = [&](uint8_t* at) {
+                            uint4 x = *reinterpret_cast<const uint4*>(at);
+                            const uint4 m = make_uint4(nan_bytes(x.x), nan_bytes(x.y), nan_bytes(x.z), nan_bytes(x.w));
+                            if (!(m.x | m.y | m.z | m.w)) return;
+                            x.x &= ~((m.x >> 7) * 0xffu); x.y &= ~((m.y >> 7) * 0xffu); x.z &= ~((m.z >> 7) * 0xffu); x.w &= ~((m.w >> 7) * 0xffu);
+                            *reinterpret_cast<uint4*>(at) = x;
+                        };
+                        const int first = w.s.n - t * TM_TILE - (is_k ? rank * TM_OWN : 0);
+                        if (is_k) {
+#pragma unroll 4
+                            for (int it = max(0, first); it < TM_OWN; ++it) clear(buf + (lane >> 3) * KCHUNK + tc::sw128_chunk(it, lane & 7));
+#pragma unroll
+                            for (int it = 0; it < 4; ++it)
+                                if (it * 8 + (lane >> 2) >= first) clear(buf + 4 * KCHUNK + sw64_chunk(it * 8 + (lane >> 2), lane & 3));
+                        } else {
+#pragma unroll 4
+                            for (int it = 0; it < 32; ++it)
+                                if (2 * it + (lane >> 4) >= first) clear(buf + ((lane & 15) >> 3) * VCHUNK + tc::sw128_chunk(2 * it + (lane >> 4), lane & 7));
+                        }
+                    }
+                    tc::cp_async_mbar_arrive_noinc(full);
+                    tc::fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(full);
                 }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) { row[u] = row_n[u]; scl[u] = scl_n[u]; }
+                for (int u = 0; u < 2; ++u) {
+                    row[u] = pool_row(tok1[u], pg1[u]);
+                    tok1[u] = tok2[u];
+                    pg1[u] = page(tok2[u]);
+                    tok2[u] = entry(t + 3, u);
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) scl[u] = is_k && row[u] != NONE ? A.pscale[row[u]] : 0.0f;
             }
         }
-    } else if (warp == TM_QKW) {
-        // ------------------------------ QK issuer: S(i) = Q . K(i)^T -----------------------------
-        const uint32_t id_qk = tc::idesc_e4m3(128, TM_TILE, 0, 0);
-        const uint64_t d_qr = smem_desc(tc::smem_u32(smem + SM_QR), 16, 512, 4);
-        bool ok = true;
-        int i = 0, seg = 0;
-        for (; ok && walk_segment(A, w); walk_on(A, w), ++seg) {
-            ok = tc::mbar_wait_warp(&bars.q_full, seg & 1, abort_flag, 51, max_polls);
-            for (int t = w.t0; t < w.t1 && ok; ++t, ++i) {
-                const int s = i % TM_STAGES, use = i / TM_STAGES, sb = i & 1;
-                ok = tc::mbar_wait_warp(&bars.k_full[s], use & 1, abort_flag, 52, max_polls) &&
-                     tc::mbar_wait_warp(&bars.s_empty[sb], ((i >> 1) & 1) ^ 1, abort_flag, 53, max_polls);
-                if (!ok) break;
-                tc::fence_proxy_async();   // the copies wrote through the generic proxy, the products read through the async one
-                tc::tc_fence_after();
-                const uint64_t d_k = smem_desc(tc::smem_u32(smem + SM_K + s * KSTAGE), 16, 1024, 2);
-                const uint64_t d_rope = smem_desc(tc::smem_u32(smem + SM_K + s * KSTAGE + 4 * KCHUNK), 16, 512, 4);
-                const uint32_t d = TM_S0 + sb * TM_TILE;
-                if (tc::elect_one()) {
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) tc::mma_f8(d, d_qr + (uint64_t)(k * 2), d_rope + (uint64_t)(k * 2), id_qk, k != 0);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            tc::mma_f8_ta(d, TM_Q + (uint32_t)(c * 32 + k * 8), d_k + (uint64_t)((c * KCHUNK + k * 32) >> 4), id_qk, 1);
-                    tc::mma_commit(&bars.s_full[sb]);
-                    tc::mbar_arrive(&bars.s_full[sb]);   // hands the token words on: this thread has seen k_full
+    } else if (warp == TM_QKW || warp == TM_PVW) {
+        if (rank == 1) {
+            // ------------------------------ the second CTA: its stages are full -------------------
+            uint64_t* full = warp == TM_QKW ? bars.k_full : bars.v_full;
+            const uint32_t peer = in_first(warp == TM_QKW ? bars.k_peer : bars.v_peer);
+            const int stages = warp == TM_QKW ? NK : NV;
+            bool ok = true;
+            int s = 0, phase = 0;
+            for (; ok && walk_segment(A, w); walk_on(A, w))
+                for (int t = w.t0; t < w.t1; ++t) {
+                    ok = tc::mbar_wait_warp(&full[s], phase, abort_flag, 57, max_polls);
+                    if (!ok) break;
+                    tc::fence_proxy_async();
+                    if (lane == 0) arrive_first(peer + s * 8);
+                    if (++s == stages) { s = 0; phase ^= 1; }
                 }
-                __syncwarp();
-            }
-        }
-    } else if (warp == TM_PVW) {
-        // ------------------------------ PV issuer: O^T += V(i)^T . P'(i) --------------------------
-        const uint32_t id_pv = tc::idesc_e4m3(128, TM_ROWS, 1, 0);
-        bool ok = true;
-        int i = 0;
-        for (; ok && walk_segment(A, w); walk_on(A, w)) {
-            for (int t = w.t0; t < w.t1 && ok; ++t, ++i) {
-                const int s = i % TM_STAGES, pb = i & 1;
-                ok = tc::mbar_wait_warp(&bars.p_full[pb], (i >> 1) & 1, abort_flag, 54, max_polls);
-                if (!ok) break;
-                tc::fence_proxy_async();
-                tc::tc_fence_after();
-                const uint64_t d_v = smem_desc(tc::smem_u32(smem + SM_K + s * KSTAGE), KCHUNK, 1024, 2);
-                const uint64_t d_phi = smem_desc(tc::smem_u32(smem + SM_P + pb * PBUF), 16, 512, 4);
-                const uint64_t d_plo = smem_desc(tc::smem_u32(smem + SM_P + pb * PBUF + PTERM), 16, 512, 4);
-                if (tc::elect_one()) {
+        } else if (warp == TM_QKW) {
+            // ------------------------------ QK issuer: S(i) = Q . K(i)^T -------------------------
+            const uint32_t id_qk = tc::idesc_e4m3(256, TM_TILE, 0, 0);
+            const uint64_t d_qr = smem_desc(tc::smem_u32(smem + SM_QR), 16, 512, 4);
+            bool ok = true;
+            int i = 0, seg = 0;
+            for (; ok && walk_segment(A, w); walk_on(A, w), ++seg) {
+                ok = wait_cluster(&bars.q_full, seg & 1, abort_flag, 51, max_polls);
+                for (int t = w.t0; t < w.t1 && ok; ++t, ++i) {
+                    const int s = i % NK, use = i / NK, sb = i & 1;
+                    ok = tc::mbar_wait_warp(&bars.k_full[s], use & 1, abort_flag, 52, max_polls) &&
+                         wait_cluster(&bars.k_peer[s], use & 1, abort_flag, 56, max_polls) &&
+                         wait_cluster(&bars.s_empty[sb], ((i >> 1) & 1) ^ 1, abort_flag, 53, max_polls);
+                    if (!ok) break;
+                    tc::fence_proxy_async();   // copies that wrote through the generic proxy, the products read through the async one
+                    tc::tc_fence_after();
+                    const uint64_t d_k = smem_desc(tc::smem_u32(smem + SM_K + s * KSTAGE), 16, 1024, 2);
+                    const uint64_t d_rope = smem_desc(tc::smem_u32(smem + SM_K + s * KSTAGE + 4 * KCHUNK), 16, 512, 4);
+                    const uint32_t d = TM_S0 + sb * TM_TILE;
+                    if (tc::elect_one()) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                        for (int k = 0; k < 2; ++k) tc::mma2_f8(d, d_qr + (uint64_t)(k * 2), d_rope + (uint64_t)(k * 2), id_qk, k != 0);
 #pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            tc::mma_f8(TM_O + c * 64, d_v + (uint64_t)((c * KCHUNK + k * 4096) >> 4), d_phi + (uint64_t)(k * 2), id_pv, t > w.t0 || k != 0);
+                        for (int c = 0; c < 4; ++c)
 #pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            tc::mma_f8(TM_O + c * 64, d_v + (uint64_t)((c * KCHUNK + k * 4096) >> 4), d_plo + (uint64_t)(k * 2), id_pv, 1);
+                            for (int k = 0; k < 4; ++k)
+                                tc::mma2_f8_ta(d, TM_Q + (uint32_t)(c * 32 + k * 8), d_k + (uint64_t)((c * KCHUNK + k * 32) >> 4), id_qk, 1);
+                        tc::commit2(&bars.k_empty[s]);
+                        tc::commit2(&bars.s_full[i % NG]);
                     }
-                    tc::mma_commit(&bars.k_empty[s]);
-                    tc::mma_commit(&bars.pv_done[pb]);
+                    __syncwarp();
                 }
-                __syncwarp();
+            }
+        } else {
+            // ------------------------------ PV issuer: O += P'(i) . V(i) --------------------------
+            const uint32_t id_pv = tc::idesc_e4m3(128, 256, 0, 1);
+            bool ok = true;
+            int i = 0;
+            for (; ok && walk_segment(A, w); walk_on(A, w)) {
+                for (int t = w.t0; t < w.t1 && ok; ++t, ++i) {
+                    const int s = i % NV, use = i / NV, pb = i % NG;
+                    ok = tc::mbar_wait_warp(&bars.v_full[s], use & 1, abort_flag, 58, max_polls) &&
+                         wait_cluster(&bars.v_peer[s], use & 1, abort_flag, 59, max_polls) &&
+                         wait_cluster(&bars.p_full[pb], (i / NG) & 1, abort_flag, 54, max_polls);
+                    if (!ok) break;
+                    tc::fence_proxy_async();
+                    tc::tc_fence_after();
+                    const uint64_t d_v = smem_desc(tc::smem_u32(smem + SM_V + s * VSTAGE), VCHUNK, 1024, 2);
+                    const uint64_t d_p = smem_desc(tc::smem_u32(smem + SM_P + pb * PBUF), 16, 512, 4);
+                    if (tc::elect_one()) {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)        // p_hi, then p_lo, 32 tokens each time
+                                tc::mma2_f8(TM_O + c * 128, d_p + (uint64_t)(((k >> 1) * PTERM >> 4) + (k & 1) * 2), d_v + (uint64_t)((c * VCHUNK + (k & 1) * 4096) >> 4), id_pv,
+                                        t > w.t0 || k != 0);
+                        tc::commit2(&bars.v_empty[s]);
+                        tc::commit2(&bars.pv_done[pb]);
+                    }
+                    __syncwarp();
+                }
             }
         }
     } else {
         // ------------------------------ queries, softmax, epilogue -------------------------------
         // S: a thread is a tensor-memory lane, one term of one row: lanes 0-15 of warp s % 4 hold the hi terms of rows 16 s .. + 15,
-        // lanes 16-31 their lo terms. One shuffle per score adds the two and leaves each lane half of the tokens of its row. The
-        // groups of four warps take the tiles in turn.
+        // lanes 16-31 their lo terms. One shuffle per score adds the two and leaves each lane half of the tokens of its row.
+        // O: lanes 0-63 hold rows 0-63 in columns 0-127 of each 256 dims, lanes 64-127 the same rows in the other 128.
         const int sq = warp & 3, th = warp >> 2, tb = lane >> 4;
         const int hd = 16 * sq + (lane & 15);
-        const int orow = sq * 32 + lane;                   // O^T: this thread's dim of each 128-dim block
+        const int orow = (sq * 32 + lane) & 63;            // O: this thread's row
+        const int srow = sq * 32 + lane;                   // its row of the virtual ones
         const uint32_t lane_base = ((uint32_t)(sq * 32)) << 16;
-        constexpr int GROUP = TM_SOFTMAX / 2;
-        auto give_up = [&]() { (void)tc::barrier_any(6 + th, GROUP, true); (void)tc::barrier_any(8 + th, GROUP, true); };
-        int i0 = 0;                                        // tiles of the CTA before this segment
+        const uint32_t q_full = in_first(&bars.q_full), s_empty = in_first(bars.s_empty), p_full = in_first(bars.p_full);
+        auto give_up = [&]() { (void)tc::barrier_any(6 + th, TM_GROUP, true); (void)tc::barrier_any(9 + th, TM_GROUP, true); };
+        // O has taken tile i. A parity tells a phase from the one before it only: a group asks for its own tile first, whose predecessor
+        // in the barrier it has seen, and then for another's within the NG behind it.
+        auto pv_done = [&](int i) { return tc::mbar_wait_warp(&bars.pv_done[i % NG], (i / NG) & 1, abort_flag, 63, max_polls); };
+        int i0 = 0;                                        // tiles of the pair before this segment
         bool failed = false;
         for (; !failed && walk_segment(A, w); i0 += w.t1 - w.t0, walk_on(A, w)) {
-            const int rows_all = w.s.T * A.H, r0 = w.rb * TM_ROWS, valid = min(TM_ROWS, rows_all - r0);
-            const size_t flat = (size_t)w.s.node0 * A.H + r0;      // first row of the block in q, out and out_lse
+            const int rows_all = w.s.T * A.H, r0 = w.rb * TM_BLOCK + rank * TM_ROWS, valid = max(0, min(TM_ROWS, rows_all - r0));
+            const size_t flat = (size_t)w.s.node0 * A.H + r0;      // first row of the CTA in q, out and out_lse
             const uint64_t mask = hd < valid ? A.node_mask[w.s.node0 + (r0 + hd) / A.H] : 0ull;
             // ---- q -> two e4m3 terms per row: hi = e4m3(q / s), s = absmax / 448, lo = e4m3(q / s - hi) ----
-            // A warp takes sixteen rows and half th of their columns. They arrive as whole 128-byte lines (lanes 8 k .. 8 k + 7 on one row),
+            // A warp of the first two groups takes sixteen rows and half th of their columns. They arrive as whole 128-byte lines (lanes 8 k .. 8 k + 7 on one row),
             // are split there and go through shared memory, 64 columns at a time, to the lanes whose tensor-memory row they are. (A
             // lane reading its own row, a line per load, waited 10,500 cycles for them.)
             {
@@ -457,12 +524,12 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const int r = rq + 4 * k;
-                        v[4 * c + k] = r < valid ? *reinterpret_cast<const uint4*>(q0 + (size_t)r * TM_W + th * (TM_KVL / 2) + c * 64 + (lane & 7) * 8) : make_uint4(0u, 0u, 0u, 0u);
+                        v[4 * c + k] = r < valid && th < 2 ? *reinterpret_cast<const uint4*>(q0 + (size_t)r * TM_W + th * (TM_KVL / 2) + c * 64 + (lane & 7) * 8) : make_uint4(0u, 0u, 0u, 0u);
                     }
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const int r = xq + 8 * k;
-                    v[16 + k] = r < valid ? *reinterpret_cast<const uint4*>(q0 + (size_t)r * TM_W + TM_KVL + th * (TM_ROPE / 2) + (lane & 3) * 8) : make_uint4(0u, 0u, 0u, 0u);
+                    v[16 + k] = r < valid && th < 2 ? *reinterpret_cast<const uint4*>(q0 + (size_t)r * TM_W + TM_KVL + th * (TM_ROPE / 2) + (lane & 3) * 8) : make_uint4(0u, 0u, 0u, 0u);
                 }
                 // largest magnitudes: of latent rows 4 k + lane / 8 and rope rows 8 k + lane / 4, then of row lane % 16
                 uint32_t ml4[4], mx2[2];
@@ -485,9 +552,9 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                     for (int k = 0; k < 4; ++k) { const uint32_t y = __shfl_sync(0xffffffffu, ml4[k], 8 * (r & 3)); if ((r >> 2) == k) a = y; }
 #pragma unroll
                     for (int k = 0; k < 2; ++k) { const uint32_t y = __shfl_sync(0xffffffffu, mx2[k], 4 * (r & 7)); if ((r >> 3) == k) x = y; }
-                    if (lane < 16) s_wmax[th * 64 + hd] = __uint_as_float(rv_max_bf16x2(a, x) << 16);
+                    if (lane < 16 && th < 2) s_wmax[th * 64 + hd] = __uint_as_float(rv_max_bf16x2(a, x) << 16);
                 }
-                tc::named_barrier(3, TM_SOFTMAX);          // (also: both groups are through with the block before)
+                tc::named_barrier(3, TM_SOFTMAX);          // (also: all groups are through with the block before)
                 auto scale_of = [&](int r) { const float amax = fmaxf(s_wmax[r], s_wmax[64 + r]); return amax > 0.0f ? amax / 448.0f : 1.0f; };
                 if (th == 0 && tb == 0) { s_ahi[hd] = scale_of(hd) * A.softmax_scale * 1.4426950408889634f; s_mref[hd] = -INFINITY; }
                 auto codes8 = [&](const uint4 x, float inv, uint2& hi, uint2& lo) {
@@ -503,49 +570,50 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                     hi = make_uint2((uint32_t)ch[0] | ((uint32_t)ch[1] << 16), (uint32_t)ch[2] | ((uint32_t)ch[3] << 16));
                     lo = make_uint2((uint32_t)cl[0] | ((uint32_t)cl[1] << 16), (uint32_t)cl[2] | ((uint32_t)cl[3] << 16));
                 };
-                // 64 codes of 32 virtual rows (hi 0-15, lo 16-31) in this warp's 2 KiB of the staging, 16-byte chunks swizzled by row
-                uint8_t* buf = smem + SM_OUT + warp * 2048;
+                // 64 codes of 32 virtual rows (hi 0-15, lo 16-31) in this warp's 2 KiB of the idle P' buffers, 16-byte chunks swizzled by row
+                uint8_t* buf = smem + SM_P + (warp & 7) * 2048;
                 auto spot = [&](int r, int byte) { return buf + r * 64 + ((((byte >> 4) ^ (r >> 1)) & 3) << 4) + (byte & 15); };
-                if (lane == 0 && sq == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                tc::named_barrier(3, TM_SOFTMAX);          // the staging is free
-                const uint32_t dst = TM_Q + lane_base + th * 64;
-                float inv4[4];
+                if (th < 2) {
+                    const uint32_t dst = TM_Q + lane_base + th * 64;
+                    float inv4[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) inv4[k] = 1.0f / scale_of(rq + 4 * k);
+                    for (int k = 0; k < 4; ++k) inv4[k] = 1.0f / scale_of(rq + 4 * k);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    __syncwarp();
+                    for (int c = 0; c < 4; ++c) {
+                        __syncwarp();
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
+                        for (int k = 0; k < 4; ++k) {
+                            uint2 hi, lo;
+                            codes8(v[4 * c + k], inv4[k], hi, lo);
+                            const int r = 4 * k + (lane >> 3);
+                            *reinterpret_cast<uint2*>(spot(r, (lane & 7) * 8)) = hi;
+                            *reinterpret_cast<uint2*>(spot(16 + r, (lane & 7) * 8)) = lo;
+                        }
+                        __syncwarp();
+                        uint32_t a[16];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint4 x = *reinterpret_cast<const uint4*>(spot(lane, 16 * k));
+                            a[4 * k] = x.x; a[4 * k + 1] = x.y; a[4 * k + 2] = x.z; a[4 * k + 3] = x.w;
+                        }
+                        tc::tmem_st8(dst + c * 16, a);
+                        tc::tmem_st8(dst + c * 16 + 8, a + 8);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {              // rope columns: straight to the operand tile, eight codes at a time
+                        const int r = 8 * k + (lane >> 2);
                         uint2 hi, lo;
-                        codes8(v[4 * c + k], inv4[k], hi, lo);
-                        const int r = 4 * k + (lane >> 3);
-                        *reinterpret_cast<uint2*>(spot(r, (lane & 7) * 8)) = hi;
-                        *reinterpret_cast<uint2*>(spot(16 + r, (lane & 7) * 8)) = lo;
+                        codes8(v[16 + k], 1.0f / scale_of(16 * sq + r), hi, lo);
+                        const int col = th * 32 + (lane & 3) * 8;
+                        *reinterpret_cast<uint2*>(smem + SM_QR + sw64_chunk(sq * 32 + r, col >> 4) + (col & 15)) = hi;
+                        *reinterpret_cast<uint2*>(smem + SM_QR + sw64_chunk(sq * 32 + 16 + r, col >> 4) + (col & 15)) = lo;
                     }
-                    __syncwarp();
-                    uint32_t a[16];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(spot(lane, 16 * k));
-                        a[4 * k] = x.x; a[4 * k + 1] = x.y; a[4 * k + 2] = x.z; a[4 * k + 3] = x.w;
-                    }
-                    tc::tmem_st8(dst + c * 16, a);
-                    tc::tmem_st8(dst + c * 16 + 8, a + 8);
-                }
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {              // rope columns: straight to the operand tile, eight codes at a time
-                    const int r = 8 * k + (lane >> 2);
-                    uint2 hi, lo;
-                    codes8(v[16 + k], 1.0f / scale_of(16 * sq + r), hi, lo);
-                    const int col = th * 32 + (lane & 3) * 8;
-                    *reinterpret_cast<uint2*>(smem + SM_QR + sw64_chunk(sq * 32 + r, col >> 4) + (col & 15)) = hi;
-                    *reinterpret_cast<uint2*>(smem + SM_QR + sw64_chunk(sq * 32 + 16 + r, col >> 4) + (col & 15)) = lo;
                 }
                 tc::tmem_st_wait();
                 tc::fence_proxy_async();
                 tc::tc_fence_before();
-                tc::mbar_arrive(&bars.q_full);
+                __syncwarp();
+                if (lane == 0) arrive_first(q_full);
                 tc::named_barrier(3, TM_SOFTMAX);          // the row scales and references are read by other warps than wrote them
             }
 
@@ -554,23 +622,24 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
             float l_acc = 0.0f, m_ref = -INFINITY;
             const int i1 = i0 + (w.t1 - w.t0);
             bool ok = true;
-            for (int i = i0 + ((th ^ i0) & 1); i < i1; i += 2) {
-                const int s = i % TM_STAGES, j0 = (w.t0 + i - i0) * TM_TILE;
-                ok = tc::mbar_wait_warp(&bars.s_full[th], (i >> 1) & 1, abort_flag, 62, max_polls);
+            for (int i = i0 + (th + 2 * NG - i0 % NG) % NG; i < i1; i += NG) {
+                const int sv = i % NV, j0 = (w.t0 + i - i0) * TM_TILE, sb = i & 1;
+                ok = tc::mbar_wait_warp(&bars.tok_full[sv], (i / NV) & 1, abort_flag, 61, max_polls) &&
+                     tc::mbar_wait_warp(&bars.s_full[th], (i / NG) & 1, abort_flag, 62, max_polls);
                 if (!ok) { give_up(); break; }
                 tc::tc_fence_after();
-                const float4* ti = reinterpret_cast<const float4*>(s_tok + s * TM_TILE + 16 * tb);
+                const float4* ti = reinterpret_cast<const float4*>(s_tok + sv * TM_TILE + 16 * tb);
                 float s2[32];
                 float mx = -INFINITY;
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
                     uint32_t r[32];
-                    tc::tmem_ld32(TM_S0 + th * TM_TILE + lane_base + 32 * hf, r);
+                    tc::tmem_ld32(TM_S0 + sb * TM_TILE + lane_base + 32 * hf, r);
                     tc::tmem_ld_wait();
                     if (hf == 1) {
                         tc::tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) tc::mbar_arrive(&bars.s_empty[th]);
+                        if (lane == 0) arrive_first(s_empty + sb * 8);
                     }
 #pragma unroll
                     for (int j4 = 0; j4 < 4; ++j4) {
@@ -597,15 +666,52 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                         mx = fmaxf(mx, s2[j]);
                     }
                 }
-                // the references as the tile before left them (the other group's)
+                // P' as two e4m3 terms (through f16) at reference m; l_t takes the plain weights. A row that has seen nothing has no
+                // reference: its scores are all -inf and weigh 0.
+                uint32_t hi_w[8], lo_w[8];
+                float l_t;
+                auto weights = [&](float m) {
+                    l_t = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 ti4 = ti[2 * (TOKPLANE / 16) + 8 * (j >> 4) + ((j & 15) >> 2)];
+                        const float inv4[4] = {ti4.x, ti4.y, ti4.z, ti4.w};
+                        uint32_t chs[2], cls[2];
+#pragma unroll
+                        for (int e = 0; e < 4; e += 2) {
+                            float p0, p1;
+                            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(s2[j + e] - m));
+                            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(s2[j + e + 1] - m));
+                            l_t = fmaf(p0, inv4[e], l_t);
+                            l_t = fmaf(p1, inv4[e + 1], l_t);
+                            const __half2 ph = __floats2half2_rn(p0, p1);
+                            const uint32_t phb = *reinterpret_cast<const uint32_t*>(&ph);
+                            uint16_t ch, cl;
+                            uint32_t hfb;
+                            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(ch) : "r"(phb));
+                            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hfb) : "h"(ch));
+                            const __half2 res = __hsub2(ph, *reinterpret_cast<const __half2*>(&hfb));
+                            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(cl) : "r"(*reinterpret_cast<const uint32_t*>(&res)));
+                            chs[e >> 1] = ch; cls[e >> 1] = cl;
+                        }
+                        hi_w[j >> 2] = chs[0] | (chs[1] << 16);
+                        lo_w[j >> 2] = cls[0] | (cls[1] << 16);
+                    }
+                };
+                // The weights at the reference as it was a tile or two ago, before it is known whether it stands: it nearly always does,
+                // and what is waited for below passes meanwhile.
+                const float m_spec = m_ref == -INFINITY ? 0.0f : m_ref;
+                weights(m_spec);
+                // the references as the tile before left them (another group's)
+                const int gb = (i + NG - 1) % NG;
                 if (i > i0) {
-                    ok = tc::mbar_wait_warp(&bars.dec[th ^ 1], ((i - 1) >> 1) & 1, abort_flag, 65, max_polls);
+                    ok = tc::mbar_wait_warp(&bars.dec[gb], ((i - 1) / NG) & 1, abort_flag, 65, max_polls);
                     if (!ok) { give_up(); break; }
                     const float m_now = s_mref[hd];
                     if (m_now != m_ref) { l_acc *= exp2f(m_ref - m_now); m_ref = m_now; }
                 }
                 // As long as no score exceeds its row's reference by more than the lag the references stand: one barrier with an OR.
-                if (tc::barrier_any(6 + th, GROUP, mx - m_ref > TM_LAG + TM_POFF)) {
+                if (tc::barrier_any(6 + th, TM_GROUP, mx - m_ref > TM_LAG + TM_POFF)) {
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                     float fac = 1.0f;
                     {
@@ -614,18 +720,20 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                         else if (tm > m_ref) { fac = exp2f(m_ref - tm); m_ref = tm; }
                         if (lane < 16) { s_fac[hd] = fac; s_mref[hd] = m_ref; }
                     }
-                    if (tc::barrier_any(8 + th, GROUP, false)) { ok = false; break; }
-                    if (i > i0) ok = tc::mbar_wait_warp(&bars.pv_done[th ^ 1], ((i - 1) >> 1) & 1, abort_flag, 63, max_polls);
-                    if (!ok) { if (i + 2 < i1) give_up(); break; }
+                    if (tc::barrier_any(9 + th, TM_GROUP, false)) { ok = false; break; }
+                    if (i >= i0 + NG) ok = pv_done(i - NG);
+                    if (ok && i > i0) ok = pv_done(i - 1);
+                    if (!ok) { if (i + NG < i1) give_up(); break; }
                     tc::tc_fence_after();
-                    if (i > i0) {                          // O^T to the new references
+                    if (i > i0) {                          // O to the new references
+                        const float f = s_fac[orow];
                         uint32_t r[32];
 #pragma unroll 1
                         for (int c = 0; c < 8; ++c) {
                             tc::tmem_ld32(TM_O + lane_base + c * 32, r);
                             tc::tmem_ld_wait();
 #pragma unroll
-                            for (int h = 0; h < 32; ++h) r[h] = __float_as_uint(__uint_as_float(r[h]) * s_fac[(c & 1) * 32 + h]);
+                            for (int h = 0; h < 32; ++h) r[h] = __float_as_uint(__uint_as_float(r[h]) * f);
                             tc::tmem_st32(TM_O + lane_base + c * 32, r);
                         }
                         tc::tmem_st_wait();
@@ -635,38 +743,12 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                 }
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&bars.dec[th]);
-                // P' as two e4m3 terms (through f16); l takes the plain weight. A row that has seen nothing has no reference: its
-                // scores are all -inf and weigh 0.
                 const float m_use = m_ref == -INFINITY ? 0.0f : m_ref;
-                uint32_t hi_w[8], lo_w[8];
-#pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    const float4 ti4 = ti[2 * (TOKPLANE / 16) + 8 * (j >> 4) + ((j & 15) >> 2)];
-                    const float inv4[4] = {ti4.x, ti4.y, ti4.z, ti4.w};
-                    uint32_t chs[2], cls[2];
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        float p0, p1;
-                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(s2[j + e] - m_use));
-                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(s2[j + e + 1] - m_use));
-                        l_acc = fmaf(p0, inv4[e], l_acc);
-                        l_acc = fmaf(p1, inv4[e + 1], l_acc);
-                        const __half2 ph = __floats2half2_rn(p0, p1);
-                        const uint32_t phb = *reinterpret_cast<const uint32_t*>(&ph);
-                        uint16_t ch, cl;
-                        uint32_t hfb;
-                        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(ch) : "r"(phb));
-                        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hfb) : "h"(ch));
-                        const __half2 res = __hsub2(ph, *reinterpret_cast<const __half2*>(&hfb));
-                        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(cl) : "r"(*reinterpret_cast<const uint32_t*>(&res)));
-                        chs[e >> 1] = ch; cls[e >> 1] = cl;
-                    }
-                    hi_w[j >> 2] = chs[0] | (chs[1] << 16);
-                    lo_w[j >> 2] = cls[0] | (cls[1] << 16);
-                }
+                if (__any_sync(0xffffffffu, m_use != m_spec)) weights(m_use);
+                l_acc += l_t;
                 // the buffer was read by the products of this group's tile before
-                if (i >= i0 + 2) ok = tc::mbar_wait_warp(&bars.pv_done[th], ((i - 2) >> 1) & 1, abort_flag, 64, max_polls);
-                if (!ok) { if (i + 2 < i1) give_up(); break; }
+                if (i >= i0 + NG) ok = pv_done(i - NG);
+                if (!ok) { if (i + NG < i1) give_up(); break; }
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
                     uint8_t* prow = smem + SM_P + th * PBUF + sw64_chunk(hd, 2 * hf + tb);
@@ -674,108 +756,91 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                     *reinterpret_cast<uint4*>(prow + PTERM) = make_uint4(lo_w[4 * hf], lo_w[4 * hf + 1], lo_w[4 * hf + 2], lo_w[4 * hf + 3]);
                 }
                 tc::fence_proxy_async();
-                tc::mbar_arrive(&bars.p_full[th]);
+                __syncwarp();
+                if (lane == 0) arrive_first(p_full + th * 8);
             }
 
             // ---- epilogue of the segment ----
-            // l per row: its four threads (two lanes 16 apart in a warp of each group) meet at the last reference
-            if (ok) ok = tc::mbar_wait_warp(&bars.pv_done[(i1 - 1) & 1], ((i1 - 1) >> 1) & 1, abort_flag, 66, max_polls);
+            // l per row: its six threads (two lanes 16 apart in a warp of each group) meet at the last reference
+            const int own = i1 - 1 - (i1 - 1 - th + NG) % NG;  // this group's last tile
+            if (ok && own >= i0) ok = pv_done(own);
+            if (ok) ok = pv_done(i1 - 1);
             failed = tc::barrier_any(1, TM_SOFTMAX, !ok);  // (all leave the loop over segments together)
+            const float m_last = s_mref[hd];
             {
-                const float m_now = s_mref[hd];
-                if (m_now != m_ref) { l_acc *= exp2f(m_ref - m_now); m_ref = m_now; }
+                if (m_last != m_ref) l_acc *= exp2f(m_ref - m_last);
                 const float mine = l_acc + __shfl_xor_sync(0xffffffffu, l_acc, 16);
                 if (lane < 16) s_wmax[th * 64 + hd] = mine;
             }
             tc::named_barrier(1, TM_SOFTMAX);
             tc::tc_fence_after();
-            const float l = s_wmax[hd] + s_wmax[64 + hd];
             const bool whole = w.t0 == 0 && w.t1 == w.nt;
-            if (whole && th == 0 && lane < 16) {
+            const int slot = 2 * pair + (w.t0 == 0 ? 1 : 0);
+            if (th == 0 && lane < 16) {
                 // (l and O carry 2^5; NaN stays NaN)
-                if (hd < valid && A.out_lse)
-                    A.out_lse[flat + hd] = l == 0.0f ? -INFINITY : (m_ref - TM_POFF) * 0.6931471805599453f + logf(l);
+                const float l = s_wmax[hd] + s_wmax[64 + hd] + s_wmax[128 + hd];
+                if (!whole) reinterpret_cast<float2*>(scratch + SC_ML)[slot * TM_BLOCK + rank * TM_ROWS + hd] = make_float2(m_last, l);
+                else if (hd < valid && A.out_lse) A.out_lse[flat + hd] = l == 0.0f ? -INFINITY : (m_last - TM_POFF) * 0.6931471805599453f + logf(l);
                 s_fac[hd] = l == 0.0f ? 0.0f : 1.0f / l;
             }
             tc::named_barrier(1, TM_SOFTMAX);              // (the sums are read: the next block's maxima take their place)
-            if (whole) {
-                // eight rows at a time through the group's staging, and out as one bulk copy
-                uint16_t* stage = reinterpret_cast<uint16_t*>(smem + SM_OUT + th * 8192);
+            {
+                // a row's 32 columns at a time: 64 bytes of bf16, or a part's 128 of f32 as they are, for the joining kernel
+                const float inv_l = s_fac[orow];
+                float* po = reinterpret_cast<float*>(scratch + SC_O) + ((size_t)slot * TM_BLOCK + rank * TM_ROWS + orow) * TM_KVL;
+                uint16_t* to = A.out + (flat + orow) * TM_KVL;
 #pragma unroll 1
-                for (int g = 0; g < 4; ++g) {
-                    const int hg = th * 32 + g * 8;
-                    uint32_t r[4][8];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tc::tmem_ld8(TM_O + lane_base + c * 64 + hg, r[c]);
+                for (int c = th; c < 8; c += NG) {
+                    const int dim = 256 * (c >> 2) + 128 * (sq >> 1) + 32 * (c & 3);
+                    uint32_t r[32];
+                    tc::tmem_ld32(TM_O + lane_base + c * 32, r);
                     tc::tmem_ld_wait();
-                    if (sq == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                    tc::named_barrier(4 + th, GROUP);      // the staging is free
-                    const float4 f0 = *reinterpret_cast<const float4*>(s_fac + hg), f1 = *reinterpret_cast<const float4*>(s_fac + hg + 4);
-                    const float inv_l[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
-                    uint16_t* sp = stage + orow;
+                    if (!whole) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                        for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4*>(po + dim + 4 * k) = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
+                    } else if (orow < valid) {
 #pragma unroll
-                        for (int k = 0; k < 8; k += 2) {
-                            uint32_t w2;
-                            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w2) : "f"(__uint_as_float(r[c][k + 1]) * inv_l[k + 1]), "f"(__uint_as_float(r[c][k]) * inv_l[k]));
-                            sp[k * TM_KVL + c * 128] = (uint16_t)w2;
-                            sp[(k + 1) * TM_KVL + c * 128] = (uint16_t)(w2 >> 16);
+                        for (int k = 0; k < 4; ++k) {
+                            uint32_t p[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p[e]) : "f"(__uint_as_float(r[8 * k + 2 * e + 1]) * inv_l), "f"(__uint_as_float(r[8 * k + 2 * e]) * inv_l));
+                            *reinterpret_cast<uint4*>(to + dim + 8 * k) = make_uint4(p[0], p[1], p[2], p[3]);
                         }
-                    tc::fence_proxy_async();
-                    tc::named_barrier(4 + th, GROUP);
-                    const int n = min(8, valid - hg);
-                    if (sq == 0 && lane == 0 && n > 0) {
-                        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
-                                     ::"l"(A.out + (flat + hg) * TM_KVL), "r"(tc::smem_u32(stage)), "r"(n * TM_KVL * 2) : "memory");
-                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }
                 }
-            } else {
-                // a part: O as it is, its references and sums, for the joining kernel
-                const int slot = 2 * blockIdx.x + (w.t0 == 0 ? 1 : 0);
-                if (th == 0 && lane < 16)
-                    reinterpret_cast<float2*>(scratch + SC_ML)[slot * TM_ROWS + hd] = make_float2(m_ref, l);
-                float* po = reinterpret_cast<float*>(scratch + SC_O) + (size_t)slot * TM_ROWS * TM_KVL;
-#pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t r[32];
-                    tc::tmem_ld32(TM_O + lane_base + c * 64 + th * 32, r);
-                    tc::tmem_ld_wait();
-#pragma unroll
-                    for (int h = 0; h < 32; ++h)
-                        po[(size_t)(th * 32 + h) * TM_KVL + c * 128 + orow] = __uint_as_float(r[h]);
-                }
-                if (w.t0 == 0 && tid == 0) {
-                    // this CTA has the block's beginning: which runs hold the rest
-                    const long long total = s_units[1], end = run_begin(total, blockIdx.x + 1, s_run[3]) + (w.nt - w.t1) - 1;   // the block's last unit
-                    int last = (int)(end * s_run[3] / total);
-                    while (run_begin(total, last + 1, s_run[3]) <= end) ++last;
-                    Head h{(int32_t)flat, valid, last - (int)blockIdx.x + 1, 0};
-                    reinterpret_cast<Head*>(scratch + SC_HEAD)[blockIdx.x] = h;
-                    w.left = -1;                           // (told; the walk ends here in any case)
-                }
+            }
+            if (!whole && w.t0 == 0 && tid == 0 && rank == 0) {
+                // this pair has the block's beginning: which runs hold the rest
+                const long long total = s_units[1], end = run_begin(total, pair + 1, s_run[3]) + (w.nt - w.t1) - 1;   // the block's last unit
+                int last = (int)(end * s_run[3] / total);
+                while (run_begin(total, last + 1, s_run[3]) <= end) ++last;
+                Head h{(int32_t)flat, min(TM_BLOCK, rows_all - r0), last - pair + 1, 0};
+                reinterpret_cast<Head*>(scratch + SC_HEAD)[pair] = h;
+                w.left = -1;                               // (told; the walk ends here in any case)
             }
             tc::tc_fence_before();
         }
-        if (sq == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         // no block begins in this run and ends in another: nothing for the joining kernel
-        if (tid == 0 && w.left >= 0) {
+        if (tid == 0 && rank == 0 && w.left >= 0) {
             Head h{0, 0, 0, 0};
-            reinterpret_cast<Head*>(scratch + SC_HEAD)[blockIdx.x] = h;
+            reinterpret_cast<Head*>(scratch + SC_HEAD)[pair] = h;
         }
     }
 
     tc::tc_fence_before();
     __syncthreads();
+    if (warp == TM_QKW) tc::settle(*abort_flag);
+    __syncthreads();
+    cluster_sync();                                    // neither CTA leaves while the other's products may read its shared memory
     if (warp == TM_QKW) {
         tc::settle(*abort_flag);
-        tc::tmem_dealloc<512>(tmem);
+        tc::tmem_dealloc2(tmem);
     }
     if (tid == 0 && *abort_flag) atomicCAS(err, 0, *abort_flag);
 }
 
-// Joins the parts of the row block whose beginning CTA blockIdx.x of the kernel before left, eight of its rows per block: a warp per row.
+// Joins the parts of the row block whose beginning pair blockIdx.x of the kernel before left, eight of its rows per block: a warp per row.
 __global__ void __launch_bounds__(256)
 tree_join_kernel(const uint8_t* scratch, uint16_t* out, float* out_lse) {
     rv_grid_dep_wait();
@@ -786,16 +851,16 @@ tree_join_kernel(const uint8_t* scratch, uint16_t* out, float* out_lse) {
     auto slot = [&](int p) { return p == 0 ? 2 * g + 1 : 2 * (g + p); };
     const float2* ml = reinterpret_cast<const float2*>(scratch + SC_ML);
     float m = -INFINITY, l = 0.0f;
-    for (int p = 0; p < h.parts; ++p) m = fmaxf(m, ml[slot(p) * TM_ROWS + row].x);
+    for (int p = 0; p < h.parts; ++p) m = fmaxf(m, ml[slot(p) * TM_BLOCK + row].x);
     float4 acc[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) acc[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int p = 0; p < h.parts; ++p) {
-        const float2 part = ml[slot(p) * TM_ROWS + row];
+        const float2 part = ml[slot(p) * TM_BLOCK + row];
         if (part.x == -INFINITY && part.y == 0.0f) continue;       // the part saw nothing
         const float f = exp2f(part.x - m);
         l += part.y * f;
-        const float4* o = reinterpret_cast<const float4*>(scratch + SC_O) + ((size_t)slot(p) * TM_ROWS + row) * (TM_KVL / 4);
+        const float4* o = reinterpret_cast<const float4*>(scratch + SC_O) + ((size_t)slot(p) * TM_BLOCK + row) * (TM_KVL / 4);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             const float4 x = o[c * 32 + lane];
@@ -820,21 +885,49 @@ tree_join_kernel(const uint8_t* scratch, uint16_t* out, float* out_lse) {
 bool rv_tree_mma_supported(const DsaGeom* g) { return g->kv_lora == TM_KVL && g->rope_dim == TM_ROPE; }
 size_t rv_tree_mma_scratch_bytes() { return SC_TOTAL; }
 
+// Pairs that are resident at once: their runs are as long as each other, and a pair that had to wait for another's SMs would double the time.
+static int tree_pairs() {
+    static std::atomic<int> known{0};
+    int n = known.load(std::memory_order_relaxed);
+    if (n) return n;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(RV_SMS); cfg.blockDim = dim3(TM_THREADS); cfg.dynamicSmemBytes = SM_TOTAL;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, tree_mma_kernel, &cfg) != cudaSuccess || n <= 0) {
+        (void)cudaGetLastError();
+        return rv_sm_count() / 2 < TM_PAIRS ? rv_sm_count() / 2 : TM_PAIRS;
+    }
+    n = n < TM_PAIRS ? n : TM_PAIRS;                   // (the scratch holds the parts of so many runs)
+    known.store(n, std::memory_order_relaxed);
+    return n;
+}
+
 int rv_tree_mma(const TreeArgs& a, void* scratch, cudaStream_t st) {
     rv_allow_smem<tree_mma_kernel>(SM_TOTAL);
-    const int sms = rv_sm_count(), grid = sms < RV_SMS ? sms : RV_SMS;   // (the scratch holds the parts of RV_SMS runs)
+    const int pairs = tree_pairs();
     rv_drain_error();
     uint8_t* s = reinterpret_cast<uint8_t*>(scratch);
-    // tensor copies of a page's rows, 16 to 64 of them; smaller pages are gathered row by row
-    const int box = a.page_tokens < 16 ? 0 : (a.page_tokens < TM_TILE ? a.page_tokens : TM_TILE);
+    // tensor copies of a page's rows, 16 or 32 of them; smaller pages are gathered row by row
+    const int box = a.page_tokens < 16 ? 0 : (a.page_tokens < TM_OWN ? a.page_tokens : TM_OWN);
     CUtensorMap latents{}, ropes{};
     if (box) {
         const uint64_t rows = (uint64_t)a.n_pool_pages * a.page_tokens;
         if (int e = rivoli::make_tmap_columns(&latents, a.pool, rows, TM_W, 128, box)) return e;
         if (int e = rivoli::make_tmap_columns(&ropes, a.pool, rows, TM_W, TM_ROPE, box)) return e;
     }
-    rv_launch_dependent(tree_mma_kernel, dim3(grid), dim3(TM_THREADS), (size_t)SM_TOTAL, st, a, latents, ropes, box, reinterpret_cast<int*>(s), s, tc::kMaxPolls);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * pairs)); cfg.blockDim = dim3(TM_THREADS); cfg.dynamicSmemBytes = (size_t)SM_TOTAL; cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = 2; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 2;
+    (void)cudaLaunchKernelEx(&cfg, tree_mma_kernel, a, latents, ropes, box, reinterpret_cast<int*>(s), s, (int)tc::kMaxPolls);
     if (int e = rv_launch_status()) return e;
-    rv_launch_dependent(tree_join_kernel, dim3(grid, TM_ROWS / 8), dim3(256), 0, st, (const uint8_t*)s, a.out, a.out_lse);
+    rv_launch_dependent(tree_join_kernel, dim3(pairs, TM_BLOCK / 8), dim3(256), 0, st, (const uint8_t*)s, a.out, a.out_lse);
     return rv_launch_status();
 }
