@@ -20,8 +20,8 @@
 //   * The rows of a tile come as K (the CTA's 32 tokens, all columns; held until S is there) and V (all 64 tokens, the CTA's 256 columns; held
 //     until O is) in rings of their own. Tiles that lie in a dense prefix are tensor copies of page rows, others are gathered.
 // Rows of the tree are tested against each node's mask in the tiles that hold them, the last one or two of a sequence. A hidden row's
-// weight is 0, but 0 x NaN is NaN: NaN codes of tree rows become 0 and make the row's scale NaN instead, which only reaches the nodes
-// that see it.
+// weight is 0, but 0 x NaN is NaN: in V, NaN codes of tree rows become 0 (in K they make a score NaN, which the mask takes away from the
+// nodes that do not see the row, and from them alone).
 //
 // Tensor memory: S twice (64 columns each), q (128: its latent columns are the A operand of the QK products), O (256). Warps: 0-11 softmax
 // and epilogue in three groups that take the tiles in turn, 12 QK issue, 13 PV issue (in the pair's second CTA these two pass on that its
@@ -59,9 +59,9 @@ constexpr int SM_K = SM_V + NV * VSTAGE;
 constexpr int SM_QR = SM_K + NK * KSTAGE;                   // rope columns of q: [128 virtual rows][64 B], 64-byte swizzle
 constexpr int SM_P = SM_QR + 8192;                          // per group {hi, lo} [64 rows][64 tokens], 64-byte swizzle
 constexpr int PTERM = 4096, PBUF = 2 * PTERM;
-constexpr int SM_TOK = SM_P + NG * PBUF;                    // f32 [3][NV][64]: scale | log2(scale) + offset | 1 / scale
-constexpr int TOKPLANE = NV * TM_TILE * 4;
-constexpr int SM_AHI = SM_TOK + 3 * TOKPLANE;               // f32 [64] query scale * softmax scale * log2(e)
+constexpr int SM_TOK = SM_P + NG * PBUF;                    // f32 [NV][64]: the tokens' scales
+constexpr int SM_SEE = SM_TOK + NV * TM_TILE * 4;           // u64 [NV][2]: tokens that are there; tokens whose scale is no number
+constexpr int SM_AHI = SM_SEE + NV * 16;                    // f32 [64] query scale * softmax scale * log2(e)
 constexpr int SM_WMAX = SM_AHI + 256;                       // f32 [3][64]
 constexpr int SM_FAC = SM_WMAX + 768;                       // f32 [64]
 constexpr int SM_MREF = SM_FAC + 256;                       // f32 [64]
@@ -98,35 +98,46 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo_bytes
 __device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(tc::smem_u32(bar)), "r"(n) : "memory");
 }
-// One arrival on the first CTA's barrier, from either CTA (`at`: its address there).
+// One arrival on the first CTA's barrier, from either CTA (`at`: its address there). What it announces is shared and tensor memory of the
+// arriving CTA, which the products read there, through the async proxy and behind this thread's fences: release at the CTA's scope is
+// what that takes. (With the scopes of arrivals and waits at the cluster, which orders global memory too, every one of these cost a
+// thousand cycles and more: 3,700 cycles a tile.)
 __device__ __forceinline__ uint32_t in_first(const void* p) {
     uint32_t at;
     asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(tc::smem_u32(p)));
     return at;
 }
 __device__ __forceinline__ void arrive_first(uint32_t at) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(at) : "memory");
 }
-// The bounded wait for what the other CTA did.
-__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code, int max_polls) {
+// The bounded wait of a warp, in few instructions: the kernel's loops have to stay in the instruction cache. (With every wait unrolled, the
+// weights there twice and the query conversion in one piece, 192 KiB of code, each of a tile's steps waited for its instructions, and a
+// tile took 3,700 cycles.)
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code, int max_polls) {
     const uint32_t a = tc::smem_u32(bar);
-    bool done = false;
-    for (int it = 0; it < max_polls && !done; ++it) {
-        uint32_t ok;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+    uint32_t ok;
+    int left = max_polls;
+#pragma unroll 1
+    do {
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                      : "=r"(ok) : "r"(a), "r"(parity) : "memory");
-        done = ok != 0;
-        if (!done && (it & 63) == 63 && *abort_flag) break;
-    }
-    if (!done && !*abort_flag) *abort_flag = code;
-    return __all_sync(0xffffffffu, done);
+    } while (!ok && --left > 0 && ((left & 63) || !*abort_flag));
+    if (__all_sync(0xffffffffu, ok != 0)) return true;
+    if (!*abort_flag) *abort_flag = code;
+    return false;
 }
+// Two f32 in a register pair: the packed forms round each as usual.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack(float lo, float hi) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi)); return r; }
+__device__ __forceinline__ float2 unpack(f2 v) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v)); return r; }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Bytes of a word whose low seven bits are all up (NaN codes), as their top bits.
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t v) { return ((v & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+// A word of codes with 0 for NaN (bytes whose low seven bits are all up).
+__device__ __forceinline__ uint32_t no_nan(uint32_t v) { return v & ~(((((v & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu); }
 
 // A walk over a run of (row block, tile) pairs. Units are numbered tile by tile, block by block, sequence by sequence.
 struct Walk {
@@ -163,6 +174,7 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
     extern __shared__ __align__(1024) uint8_t smem[];
     Bars& bars = *reinterpret_cast<Bars*>(smem + SM_BARS);
     float* s_tok = reinterpret_cast<float*>(smem + SM_TOK);
+    uint4* s_see = reinterpret_cast<uint4*>(smem + SM_SEE);
     float* s_ahi = reinterpret_cast<float*>(smem + SM_AHI);
     float* s_wmax = reinterpret_cast<float*>(smem + SM_WMAX);
     float* s_fac = reinterpret_cast<float*>(smem + SM_FAC);
@@ -240,107 +252,85 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
         // ------------------------------ gather ---------------------------------------------------
         // Warp 14 fetches K (this CTA's 32 tokens of a tile) and writes the scales of all 64, warp 15 fetches V. Neither waits for its
         // copies: they signal the stage themselves. Rows past the end and on unmapped pages are written as zeros.
+        // A lane resolves two tokens of a tile, 32 apart: entry -> page -> pool row -> scale, each level asked for a tile or more before it
+        // is used (the loads come back through queues that the copies have filled).
         const bool is_k = warp == TM_KW;
         const int shift = rv_log2(A.page_tokens);
         constexpr uint32_t NONE = 0xffffffffu;
         bool ok = true;
-        int c0 = 0;                                // tiles of the pair before this segment
-        auto token_words = [&](int s, int slot, uint32_t r, float scl, bool nan) {
-            const bool live = r != NONE && !(scl <= 0.0f);
-            const float sc = nan ? __int_as_float(0x7fffffff) : scl;
-            float* tp = s_tok + s * TM_TILE + slot;
-            tp[0] = live ? sc : 0.0f;
-            tp[TOKPLANE / 4] = live ? __log2f(sc) + TM_POFF : -INFINITY;
-            // (0 for a NaN: times a weight that is NaN itself where the row is seen, times 0 where it is hidden)
-            tp[2 * (TOKPLANE / 4)] = live && sc == sc ? __frcp_rn(sc) : 0.0f;
-        };
-        for (; ok && walk_segment(A, w); c0 += w.t1 - w.t0, walk_on(A, w)) {
+        int s = 0, use = 0, sv = 0, usev = 0;      // stage and use of it; of V's ring, whose depth the token words share
+        const int depth = is_k ? NK : NV;
+        for (; ok && walk_segment(A, w); walk_on(A, w)) {
             const int total = w.s.n + w.s.T;
             {   // the queries of the CTA's rows on their way to L2: they are read when the softmax warps come to this segment
                 const int r0 = w.rb * TM_BLOCK + rank * TM_ROWS, bytes = min(TM_ROWS, w.s.T * A.H - r0) * TM_W * 2;
                 const char* at = reinterpret_cast<const char*>(A.q + ((size_t)w.s.node0 * A.H + r0) * TM_W);
+#pragma unroll 1
                 for (int o = ((is_k ? 0 : 32) + lane) * 128; o < bytes; o += 64 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + o));
             }
             const int tj = box_rows && !w.s.listed ? max(w.t0, min(w.t1, w.s.n / TM_TILE)) : w.t0;   // tiles from here on are gathered
-            // A lane's two tokens of a tile are 2 x 32 rows apart by 32: entry -> page -> pool row -> scale. The words are asked for a tile
-            // ahead each.
+            const int32_t* table = A.block_table + (size_t)w.b * A.max_pages;
             auto entry = [&](int t, int u) -> uint32_t {
                 const int j = t * TM_TILE + u * 32 + lane;
                 return t < w.t1 && j < total ? tree_token(A, w.s, w.b, j) : NONE;
             };
-            auto page = [&](uint32_t tok) -> int {
-                return tok != NONE && (tok >> shift) < (uint32_t)A.max_pages ? A.block_table[(size_t)w.b * A.max_pages + (tok >> shift)] : -1;
-            };
+            auto page = [&](uint32_t tok) -> int { return tok != NONE && (tok >> shift) < (uint32_t)A.max_pages ? table[tok >> shift] : -1; };
             auto pool_row = [&](uint32_t tok, int pg) -> uint32_t {
                 return pg >= 0 && pg < A.n_pool_pages ? (uint32_t)pg * (uint32_t)A.page_tokens + (tok & (uint32_t)(A.page_tokens - 1)) : NONE;
             };
-            uint32_t row[2], tok1[2], tok2[2];     // rows of tile t; entries of tiles t + 1 and t + 2
-            int pg1[2];                            // pages of tile t + 1
+            auto scale = [&](uint32_t r) -> float { return is_k && r != NONE ? A.pscale[r] : 0.0f; };
+            uint32_t row[2], row1[2], tok2[2];     // pool rows of tiles t and t + 1; entries of tile t + 2
             float scl[2];                          // scales of tile t
 #pragma unroll
-            for (int u = 0; u < 2; ++u) { row[u] = entry(w.t0, u); tok1[u] = entry(w.t0 + 1, u); tok2[u] = entry(w.t0 + 2, u); }
+            for (int u = 0; u < 2; ++u) { row[u] = entry(w.t0, u); row1[u] = entry(w.t0 + 1, u); tok2[u] = entry(w.t0 + 2, u); }
 #pragma unroll
-            for (int u = 0; u < 2; ++u) { row[u] = pool_row(row[u], page(row[u])); pg1[u] = page(tok1[u]); }
+            for (int u = 0; u < 2; ++u) { row[u] = pool_row(row[u], page(row[u])); row1[u] = pool_row(row1[u], page(row1[u])); }
 #pragma unroll
-            for (int u = 0; u < 2; ++u) scl[u] = is_k && row[u] != NONE ? A.pscale[row[u]] : 0.0f;
+            for (int u = 0; u < 2; ++u) scl[u] = scale(row[u]);
+#pragma unroll 1
             for (int t = w.t0; t < w.t1; ++t) {
-                const int i = c0 + t - w.t0, sv = i % NV, usev = i / NV;
-                const int s = is_k ? i % NK : sv, use = is_k ? i / NK : usev;
-                uint64_t* full = is_k ? &bars.k_full[s] : &bars.v_full[s];
-                if (usev > 0) ok = tc::mbar_wait_warp(&bars.v_empty[sv], (usev & 1) ^ 1, abort_flag, 41, max_polls);   // (K: for the token words)
-                if (ok && is_k && use > 0) ok = tc::mbar_wait_warp(&bars.k_empty[s], (use & 1) ^ 1, abort_flag, 42, max_polls);
+                float scl1[2];
+                int pg2[2];
+                uint32_t tok3[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) { scl1[u] = scale(row1[u]); pg2[u] = page(tok2[u]); tok3[u] = entry(t + 3, u); }
+                uint64_t* full = (is_k ? bars.k_full : bars.v_full) + s;
+                if (usev > 0) ok = wait_for(&bars.v_empty[sv], (usev & 1) ^ 1, abort_flag, 41, max_polls);   // (K: for the token words)
+                if (ok && is_k && use > 0) ok = wait_for(&bars.k_empty[s], (use & 1) ^ 1, abort_flag, 42, max_polls);
                 if (!ok) break;
                 uint8_t* buf = smem + (is_k ? SM_K + s * KSTAGE : SM_V + s * VSTAGE);
-                const bool tree_rows = (t + 1) * TM_TILE > w.s.n;
-                uint32_t bad[2] = {0u, 0u};        // this lane's rows that hold a NaN code
-                if (is_k && tree_rows) {
-                    // rows of the tree: 32 lanes look through a row at a time
-                    const int first = max(0, w.s.n - t * TM_TILE), end = min(TM_TILE, total - t * TM_TILE);
-#pragma unroll 8
-                    for (int it = first; it < end; ++it) {
-                        const uint32_t r = __shfl_sync(0xffffffffu, it < 32 ? row[0] : row[1], it & 31);
-                        const uint4* src = reinterpret_cast<const uint4*>(A.pool + (r != NONE ? (size_t)r * TM_W : 0));
-                        uint4 v = src[lane], x = src[lane < 4 ? 32 + lane : 0];
-                        const uint32_t m = nan_bytes(v.x) | nan_bytes(v.y) | nan_bytes(v.z) | nan_bytes(v.w) |
-                                           (lane < 4 ? nan_bytes(x.x) | nan_bytes(x.y) | nan_bytes(x.z) | nan_bytes(x.w) : 0u);
-                        if (__any_sync(0xffffffffu, m != 0u) && (it & 31) == lane) bad[it >> 5] = 1u;
-                    }
-                }
-                if (is_k) {
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) token_words(sv, u * 32 + lane, row[u], scl[u], bad[u] != 0u);
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&bars.tok_full[sv]);
-                }
+                const uint32_t at = tc::smem_u32(buf);
                 if (t < tj) {
                     // tensor copies: box k holds tokens k * box_rows on, of the CTA's 32 (K) or of all (V)
                     const int boxes = (is_k ? TM_OWN : TM_TILE) / box_rows, slot = (is_k ? rank * TM_OWN : 0) + lane * box_rows;
-                    const uint32_t r0 = __shfl_sync(0xffffffffu, row[0], slot & 31), r1 = __shfl_sync(0xffffffffu, row[1], slot & 31);
-                    const uint32_t y = (slot & 32) ? r1 : r0;
+                    const uint32_t y0 = __shfl_sync(0xffffffffu, row[0], slot & 31), y1 = __shfl_sync(0xffffffffu, row[1], slot & 31);
+                    const uint32_t y = (slot & 32) ? y1 : y0;
                     const bool mine = lane < boxes && y != NONE;
                     const uint32_t mapped = __ballot_sync(0xffffffffu, mine);
                     if (lane == 0) tc::mbar_arrive_expect_tx(full, __popc(mapped) * box_rows * (is_k ? TM_W : 256));
                     __syncwarp();
-                    const uint32_t at = tc::smem_u32(buf);
-                    if (mine && is_k) {
+                    if (mine) {
+                        if (is_k) {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) tc::tma_load_2d(at + c * KCHUNK + lane * box_rows * 128, &latents, c * 128, (int)y, full);
-                        tc::tma_load_2d(at + 4 * KCHUNK + lane * box_rows * 64, &ropes, TM_KVL, (int)y, full);
-                    } else if (mine) {
+                            for (int c = 0; c < 4; ++c) tc::tma_load_2d(at + c * KCHUNK + lane * box_rows * 128, &latents, c * 128, (int)y, full);
+                            tc::tma_load_2d(at + 4 * KCHUNK + lane * box_rows * 64, &ropes, TM_KVL, (int)y, full);
+                        } else {
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) tc::tma_load_2d(at + c * VCHUNK + lane * box_rows * 128, &latents, (2 * c + rank) * 128, (int)y, full);
+                            for (int c = 0; c < 2; ++c) tc::tma_load_2d(at + c * VCHUNK + lane * box_rows * 128, &latents, (2 * c + rank) * 128, (int)y, full);
+                        }
                     }
                     if (__popc(mapped) != boxes) {             // pages that are not there: zeros
                         const int chunks = is_k ? 36 : 16, rows = is_k ? TM_OWN : TM_TILE;
+#pragma unroll 1
                         for (int x = lane; x < rows * chunks; x += 32) {
                             const int r = x / chunks, c = x - r * chunks;
                             if ((mapped >> (r / box_rows)) & 1) continue;
                             *reinterpret_cast<uint4*>(buf + (!is_k ? (c >> 3) * VCHUNK + tc::sw128_chunk(r, c & 7) : c < 32 ? (c >> 3) * KCHUNK + tc::sw128_chunk(r, c & 7)
                                                                                                                               : 4 * KCHUNK + sw64_chunk(r, c - 32))) = make_uint4(0u, 0u, 0u, 0u);
                         }
+                        tc::fence_proxy_async();
+                        __syncwarp();
                     }
-                    tc::fence_proxy_async();
-                    __syncwarp();
                     if (lane == 0) mbar_arrive_n(full, FULL - 1);
                 } else {
                     if (is_k) {
@@ -348,51 +338,35 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
 #pragma unroll 8
                         for (int it = 0; it < TM_OWN; ++it) {
                             const uint32_t r = __shfl_sync(0xffffffffu, own, it);
-                            tc::cp_async16_zfill(tc::smem_u32(buf + (lane >> 3) * KCHUNK + tc::sw128_chunk(it, lane & 7)),
+                            tc::cp_async16_zfill(at + (lane >> 3) * KCHUNK + tc::sw128_chunk(it, lane & 7),
                                                  A.pool + (r != NONE ? (size_t)r * TM_W + lane * 16 : 0), r != NONE ? 16u : 0u);
                         }
 #pragma unroll
                         for (int it = 0; it < 4; ++it) {
                             const int rl = it * 8 + (lane >> 2);
                             const uint32_t r = __shfl_sync(0xffffffffu, own, rl);
-                            tc::cp_async16_zfill(tc::smem_u32(buf + 4 * KCHUNK + sw64_chunk(rl, lane & 3)),
+                            tc::cp_async16_zfill(at + 4 * KCHUNK + sw64_chunk(rl, lane & 3),
                                                  A.pool + (r != NONE ? (size_t)r * TM_W + TM_KVL + (lane & 3) * 16 : 0), r != NONE ? 16u : 0u);
                         }
                     } else {
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
+                        const int c = lane & 15;
+                        const uint8_t* from = A.pool + (2 * (c >> 3) + rank) * 128 + (c & 7) * 16;
 #pragma unroll 8
-                            for (int it = 0; it < 16; ++it) {          // two rows an instruction, 16 chunks each
-                                const int rl = 2 * it + (lane >> 4), c = lane & 15;
-                                const uint32_t r = __shfl_sync(0xffffffffu, row[u], rl);
-                                tc::cp_async16_zfill(tc::smem_u32(buf + (c >> 3) * VCHUNK + tc::sw128_chunk(u * 32 + rl, c & 7)),
-                                                     A.pool + (r != NONE ? (size_t)r * TM_W + (2 * (c >> 3) + rank) * 128 + (c & 7) * 16 : 0), r != NONE ? 16u : 0u);
-                            }
+                        for (int it = 0; it < 32; ++it) {              // two rows an instruction, 16 chunks each
+                            const int rl = 2 * it + (lane >> 4);
+                            const uint32_t r = __shfl_sync(0xffffffffu, it < 16 ? row[0] : row[1], rl & 31);
+                            tc::cp_async16_zfill(at + (c >> 3) * VCHUNK + tc::sw128_chunk(rl, c & 7), r != NONE ? from + (size_t)r * TM_W : A.pool, r != NONE ? 16u : 0u);
                         }
-                    }
-                    if (tree_rows) {
-                        // NaN codes become 0: each lane looks through what it copied itself, once it is there (zeros in rows of the
-                        // prefix too would be wrong: those are seen by all)
-                        tc::cp_async_commit();
-                        tc::cp_async_wait<0>();
-                        auto clear = [&](uint8_t* at) {
-                            uint4 x = *reinterpret_cast<const uint4*>(at);
-                            const uint4 m = make_uint4(nan_bytes(x.x), nan_bytes(x.y), nan_bytes(x.z), nan_bytes(x.w));
-                            if (!(m.x | m.y | m.z | m.w)) return;
-                            x.x &= ~((m.x >> 7) * 0xffu); x.y &= ~((m.y >> 7) * 0xffu); x.z &= ~((m.z >> 7) * 0xffu); x.w &= ~((m.w >> 7) * 0xffu);
-                            *reinterpret_cast<uint4*>(at) = x;
-                        };
-                        const int first = w.s.n - t * TM_TILE - (is_k ? rank * TM_OWN : 0);
-                        if (is_k) {
-#pragma unroll 4
-                            for (int it = max(0, first); it < TM_OWN; ++it) clear(buf + (lane >> 3) * KCHUNK + tc::sw128_chunk(it, lane & 7));
-#pragma unroll
-                            for (int it = 0; it < 4; ++it)
-                                if (it * 8 + (lane >> 2) >= first) clear(buf + 4 * KCHUNK + sw64_chunk(it * 8 + (lane >> 2), lane & 3));
-                        } else {
-#pragma unroll 4
-                            for (int it = 0; it < 32; ++it)
-                                if (2 * it + (lane >> 4) >= first) clear(buf + ((lane & 15) >> 3) * VCHUNK + tc::sw128_chunk(2 * it + (lane >> 4), lane & 7));
+                        if ((t + 1) * TM_TILE > w.s.n) {
+                            // rows of the tree: each lane looks through what it copied itself, once it is there
+                            tc::cp_async_commit();
+                            tc::cp_async_wait<0>();
+#pragma unroll 1
+                            for (int it = 0; it < 32; ++it) {
+                                const int rl = 2 * it + (lane >> 4);
+                                uint4* v = reinterpret_cast<uint4*>(buf + (c >> 3) * VCHUNK + tc::sw128_chunk(rl, c & 7));
+                                if (t * TM_TILE + rl >= w.s.n) { const uint4 x = *v; *v = make_uint4(no_nan(x.x), no_nan(x.y), no_nan(x.z), no_nan(x.w)); }
+                            }
                         }
                     }
                     tc::cp_async_mbar_arrive_noinc(full);
@@ -400,15 +374,23 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(full);
                 }
+                if (is_k) {
+                    uint32_t there[2], wild[2];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    row[u] = pool_row(tok1[u], pg1[u]);
-                    tok1[u] = tok2[u];
-                    pg1[u] = page(tok2[u]);
-                    tok2[u] = entry(t + 3, u);
+                    for (int u = 0; u < 2; ++u) {
+                        const bool odd = !(scl[u] < INFINITY), live = row[u] != NONE && !(scl[u] <= 0.0f);   // odd: NaN, or infinite
+                        s_tok[sv * TM_TILE + u * 32 + lane] = !live ? 0.0f : odd ? 1.0f : scl[u];
+                        there[u] = __ballot_sync(0xffffffffu, live);
+                        wild[u] = __ballot_sync(0xffffffffu, live && odd);
+                    }
+                    if (lane == 0) s_see[sv] = make_uint4(there[0], there[1], wild[0], wild[1]);
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&bars.tok_full[sv]);
                 }
+                if (++s == depth) { s = 0; ++use; }
+                if (++sv == NV) { sv = 0; ++usev; }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) scl[u] = is_k && row[u] != NONE ? A.pscale[row[u]] : 0.0f;
+                for (int u = 0; u < 2; ++u) { row[u] = row1[u]; scl[u] = scl1[u]; row1[u] = pool_row(tok2[u], pg2[u]); tok2[u] = tok3[u]; }
             }
         }
     } else if (warp == TM_QKW || warp == TM_PVW) {
@@ -421,7 +403,7 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
             int s = 0, phase = 0;
             for (; ok && walk_segment(A, w); walk_on(A, w))
                 for (int t = w.t0; t < w.t1; ++t) {
-                    ok = tc::mbar_wait_warp(&full[s], phase, abort_flag, 57, max_polls);
+                    ok = wait_for(&full[s], phase, abort_flag, 57, max_polls);
                     if (!ok) break;
                     tc::fence_proxy_async();
                     if (lane == 0) arrive_first(peer + s * 8);
@@ -434,12 +416,12 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
             bool ok = true;
             int i = 0, seg = 0;
             for (; ok && walk_segment(A, w); walk_on(A, w), ++seg) {
-                ok = wait_cluster(&bars.q_full, seg & 1, abort_flag, 51, max_polls);
+                ok = wait_for(&bars.q_full, seg & 1, abort_flag, 51, max_polls);
                 for (int t = w.t0; t < w.t1 && ok; ++t, ++i) {
                     const int s = i % NK, use = i / NK, sb = i & 1;
-                    ok = tc::mbar_wait_warp(&bars.k_full[s], use & 1, abort_flag, 52, max_polls) &&
-                         wait_cluster(&bars.k_peer[s], use & 1, abort_flag, 56, max_polls) &&
-                         wait_cluster(&bars.s_empty[sb], ((i >> 1) & 1) ^ 1, abort_flag, 53, max_polls);
+                    ok = wait_for(&bars.k_full[s], use & 1, abort_flag, 52, max_polls) &&
+                         wait_for(&bars.k_peer[s], use & 1, abort_flag, 56, max_polls) &&
+                         wait_for(&bars.s_empty[sb], ((i >> 1) & 1) ^ 1, abort_flag, 53, max_polls);
                     if (!ok) break;
                     tc::fence_proxy_async();   // copies that wrote through the generic proxy, the products read through the async one
                     tc::tc_fence_after();
@@ -468,9 +450,9 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
             for (; ok && walk_segment(A, w); walk_on(A, w)) {
                 for (int t = w.t0; t < w.t1 && ok; ++t, ++i) {
                     const int s = i % NV, use = i / NV, pb = i % NG;
-                    ok = tc::mbar_wait_warp(&bars.v_full[s], use & 1, abort_flag, 58, max_polls) &&
-                         wait_cluster(&bars.v_peer[s], use & 1, abort_flag, 59, max_polls) &&
-                         wait_cluster(&bars.p_full[pb], (i / NG) & 1, abort_flag, 54, max_polls);
+                    ok = wait_for(&bars.v_full[s], use & 1, abort_flag, 58, max_polls) &&
+                         wait_for(&bars.v_peer[s], use & 1, abort_flag, 59, max_polls) &&
+                         wait_for(&bars.p_full[pb], (i / NG) & 1, abort_flag, 54, max_polls);
                     if (!ok) break;
                     tc::fence_proxy_async();
                     tc::tc_fence_after();
@@ -492,25 +474,27 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
         }
     } else {
         // ------------------------------ queries, softmax, epilogue -------------------------------
-        // S: a thread is a tensor-memory lane, one term of one row: lanes 0-15 of warp s % 4 hold the hi terms of rows 16 s .. + 15,
-        // lanes 16-31 their lo terms. One shuffle per score adds the two and leaves each lane half of the tokens of its row.
+        // S: lanes 0-15 of a warp's quarter hold the hi terms of 16 rows, lanes 16-31 their lo terms. Read 16 lanes at a time in the
+        // fragment form (a thread gets two neighbouring columns of rows lane / 4 and lane / 4 + 8 per eight columns), hi and lo come to the
+        // same registers of the same thread: the sum takes no exchange. A thread has 16 tokens of two rows.
         // O: lanes 0-63 hold rows 0-63 in columns 0-127 of each 256 dims, lanes 64-127 the same rows in the other 128.
         const int sq = warp & 3, th = warp >> 2, tb = lane >> 4;
-        const int hd = 16 * sq + (lane & 15);
+        const int hd = 16 * sq + (lane & 15);              // a row of the conversion and of the epilogue's sums
+        const int ra = 16 * sq + (lane >> 2), rb = ra + 8, tq = 2 * (lane & 3);   // rows and first token of the scores
         const int orow = (sq * 32 + lane) & 63;            // O: this thread's row
-        const int srow = sq * 32 + lane;                   // its row of the virtual ones
         const uint32_t lane_base = ((uint32_t)(sq * 32)) << 16;
         const uint32_t q_full = in_first(&bars.q_full), s_empty = in_first(bars.s_empty), p_full = in_first(bars.p_full);
         auto give_up = [&]() { (void)tc::barrier_any(6 + th, TM_GROUP, true); (void)tc::barrier_any(9 + th, TM_GROUP, true); };
         // O has taken tile i. A parity tells a phase from the one before it only: a group asks for its own tile first, whose predecessor
         // in the barrier it has seen, and then for another's within the NG behind it.
-        auto pv_done = [&](int i) { return tc::mbar_wait_warp(&bars.pv_done[i % NG], (i / NG) & 1, abort_flag, 63, max_polls); };
+        auto pv_done = [&](int i) { return wait_for(&bars.pv_done[i % NG], (i / NG) & 1, abort_flag, 63, max_polls); };
         int i0 = 0;                                        // tiles of the pair before this segment
         bool failed = false;
         for (; !failed && walk_segment(A, w); i0 += w.t1 - w.t0, walk_on(A, w)) {
             const int rows_all = w.s.T * A.H, r0 = w.rb * TM_BLOCK + rank * TM_ROWS, valid = max(0, min(TM_ROWS, rows_all - r0));
             const size_t flat = (size_t)w.s.node0 * A.H + r0;      // first row of the CTA in q, out and out_lse
-            const uint64_t mask = hd < valid ? A.node_mask[w.s.node0 + (r0 + hd) / A.H] : 0ull;
+            const uint64_t mask_a = ra < valid ? A.node_mask[w.s.node0 + (r0 + ra) / A.H] : 0ull;
+            const uint64_t mask_b = rb < valid ? A.node_mask[w.s.node0 + (r0 + rb) / A.H] : 0ull;
             // ---- q -> two e4m3 terms per row: hi = e4m3(q / s), s = absmax / 448, lo = e4m3(q / s - hi) ----
             // A warp of the first two groups takes sixteen rows and half th of their columns. They arrive as whole 128-byte lines (lanes 8 k .. 8 k + 7 on one row),
             // are split there and go through shared memory, 64 columns at a time, to the lanes whose tensor-memory row they are. (A
@@ -578,13 +562,13 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                     float inv4[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) inv4[k] = 1.0f / scale_of(rq + 4 * k);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {              // (a loop: code that runs once is waited for)
                         __syncwarp();
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             uint2 hi, lo;
-                            codes8(v[4 * c + k], inv4[k], hi, lo);
+                            codes8(v[k], inv4[k], hi, lo);
                             const int r = 4 * k + (lane >> 3);
                             *reinterpret_cast<uint2*>(spot(r, (lane & 7) * 8)) = hi;
                             *reinterpret_cast<uint2*>(spot(16 + r, (lane & 7) * 8)) = lo;
@@ -598,12 +582,14 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                         }
                         tc::tmem_st8(dst + c * 16, a);
                         tc::tmem_st8(dst + c * 16 + 8, a + 8);
+#pragma unroll
+                        for (int k = 0; k < 14; ++k) v[k] = v[k + 4];
                     }
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {              // rope columns: straight to the operand tile, eight codes at a time
                         const int r = 8 * k + (lane >> 2);
                         uint2 hi, lo;
-                        codes8(v[16 + k], 1.0f / scale_of(16 * sq + r), hi, lo);
+                        codes8(v[k], 1.0f / scale_of(16 * sq + r), hi, lo);
                         const int col = th * 32 + (lane & 3) * 8;
                         *reinterpret_cast<uint2*>(smem + SM_QR + sw64_chunk(sq * 32 + r, col >> 4) + (col & 15)) = hi;
                         *reinterpret_cast<uint2*>(smem + SM_QR + sw64_chunk(sq * 32 + 16 + r, col >> 4) + (col & 15)) = lo;
@@ -618,23 +604,25 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
             }
 
             // ---- the tiles ----
-            const float a_h = s_ahi[hd];
-            float l_acc = 0.0f, m_ref = -INFINITY;
+            const float a_a = s_ahi[ra], a_b = s_ahi[rb];
+            float l_a = 0.0f, l_b = 0.0f, m_a = -INFINITY, m_b = -INFINITY;   // sums, and the references they are at
             const int i1 = i0 + (w.t1 - w.t0);
             bool ok = true;
+#pragma unroll 1
             for (int i = i0 + (th + 2 * NG - i0 % NG) % NG; i < i1; i += NG) {
                 const int sv = i % NV, j0 = (w.t0 + i - i0) * TM_TILE, sb = i & 1;
-                ok = tc::mbar_wait_warp(&bars.tok_full[sv], (i / NV) & 1, abort_flag, 61, max_polls) &&
-                     tc::mbar_wait_warp(&bars.s_full[th], (i / NG) & 1, abort_flag, 62, max_polls);
+                ok = wait_for(&bars.tok_full[sv], (i / NV) & 1, abort_flag, 61, max_polls) && wait_for(&bars.s_full[th], (i / NG) & 1, abort_flag, 62, max_polls);
                 if (!ok) { give_up(); break; }
                 tc::tc_fence_after();
-                const float4* ti = reinterpret_cast<const float4*>(s_tok + sv * TM_TILE + 16 * tb);
-                float s2[32];
-                float mx = -INFINITY;
+                // x: scores in log2 units; [k][row][token tq + e] of each run k of eight tokens
+                f2 x[16];
+                const f2* sc = reinterpret_cast<const f2*>(s_tok + sv * TM_TILE + tq);   // [4 k]: scales of run k's two tokens
+                const uint32_t s_at = TM_S0 + sb * TM_TILE + lane_base;
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    uint32_t r[32];
-                    tc::tmem_ld32(TM_S0 + sb * TM_TILE + lane_base + 32 * hf, r);
+                    uint32_t hi[16], lo[16];
+                    tc::tmem_ld16x256(s_at + 32 * hf, hi);
+                    tc::tmem_ld16x256(s_at + (16u << 16) + 32 * hf, lo);
                     tc::tmem_ld_wait();
                     if (hf == 1) {
                         tc::tc_fence_before();
@@ -642,118 +630,152 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                         if (lane == 0) arrive_first(s_empty + sb * 8);
                     }
 #pragma unroll
-                    for (int j4 = 0; j4 < 4; ++j4) {
-                        const float4 ts = ti[8 * hf + j4], tc2 = ti[TOKPLANE / 16 + 8 * hf + j4];
-                        const float sc4[4] = {ts.x, ts.y, ts.z, ts.w}, c24[4] = {tc2.x, tc2.y, tc2.z, tc2.w};
+                    for (int j = 0; j < 8; ++j)
+                        x[8 * hf + j] = add2(pack(__uint_as_float(hi[2 * j]), __uint_as_float(hi[2 * j + 1])), pack(__uint_as_float(lo[2 * j]), __uint_as_float(lo[2 * j + 1])));
+                }
+                const uint4 see = s_see[sv];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int j = 4 * j4 + e;
-                            const float mine = __uint_as_float(tb ? r[16 + j] : r[j]);
-                            const float give = __uint_as_float(tb ? r[j] : r[16 + j]);
-                            const float raw = mine + __shfl_xor_sync(0xffffffffu, give, 16);
-                            // rows past the end are zeros with an additive -inf: their weights are exactly 0
-                            s2[16 * hf + j] = fmaf(raw, a_h * sc4[e], c24[e]);
-                            mx = fmaxf(mx, s2[16 * hf + j]);
-                        }
+                for (int k = 0; k < 8; ++k) {
+                    const f2 c = sc[4 * k];
+                    x[2 * k] = mul2(x[2 * k], mul2(pack(a_a, a_a), c));
+                    x[2 * k + 1] = mul2(x[2 * k + 1], mul2(pack(a_b, a_b), c));
+                }
+                if (j0 + TM_TILE > w.s.n || (see.x & see.y) != ~0u || (see.z | see.w)) {
+                    // rows of the tree, rows that are not there, scales that are no numbers: what a node does not see scores -inf
+                    const uint64_t there = (uint64_t)see.y << 32 | see.x, wild = ((uint64_t)see.w << 32 | see.z) >> tq;
+                    const uint64_t va = (tree_visible(mask_a, w.s.T, w.s.n, j0) & there) >> tq, vb = (tree_visible(mask_b, w.s.T, w.s.n, j0) & there) >> tq;
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const uint64_t v = (k & 1) ? vb : va;
+                        float2 y = unpack(x[k]);
+                        const int bit = 8 * (k >> 1);
+                        y.x = !((v >> bit) & 1) ? -INFINITY : (wild >> bit) & 1 ? NAN : y.x;
+                        y.y = !((v >> (bit + 1)) & 1) ? -INFINITY : (wild >> (bit + 1)) & 1 ? NAN : y.y;
+                        x[k] = pack(y.x, y.y);
                     }
                 }
-                if (j0 + TM_TILE > w.s.n) {                // rows of the tree: what the mask hides weighs 0
-                    const uint64_t see = tree_visible(mask, w.s.T, w.s.n, j0) >> (16 * tb);
-                    mx = -INFINITY;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        if (!((see >> (j < 16 ? j : 16 + j)) & 1)) s2[j] = -INFINITY;
-                        mx = fmaxf(mx, s2[j]);
-                    }
-                }
-                // P' as two e4m3 terms (through f16) at reference m; l_t takes the plain weights. A row that has seen nothing has no
-                // reference: its scores are all -inf and weigh 0.
-                uint32_t hi_w[8], lo_w[8];
-                float l_t;
-                auto weights = [&](float m) {
-                    l_t = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 ti4 = ti[2 * (TOKPLANE / 16) + 8 * (j >> 4) + ((j & 15) >> 2)];
-                        const float inv4[4] = {ti4.x, ti4.y, ti4.z, ti4.w};
-                        uint32_t chs[2], cls[2];
-#pragma unroll
-                        for (int e = 0; e < 4; e += 2) {
-                            float p0, p1;
-                            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(s2[j + e] - m));
-                            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(s2[j + e + 1] - m));
-                            l_t = fmaf(p0, inv4[e], l_t);
-                            l_t = fmaf(p1, inv4[e + 1], l_t);
-                            const __half2 ph = __floats2half2_rn(p0, p1);
-                            const uint32_t phb = *reinterpret_cast<const uint32_t*>(&ph);
-                            uint16_t ch, cl;
-                            uint32_t hfb;
-                            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(ch) : "r"(phb));
-                            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hfb) : "h"(ch));
-                            const __half2 res = __hsub2(ph, *reinterpret_cast<const __half2*>(&hfb));
-                            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(cl) : "r"(*reinterpret_cast<const uint32_t*>(&res)));
-                            chs[e >> 1] = ch; cls[e >> 1] = cl;
-                        }
-                        hi_w[j >> 2] = chs[0] | (chs[1] << 16);
-                        lo_w[j >> 2] = cls[0] | (cls[1] << 16);
-                    }
-                };
-                // The weights at the reference as it was a tile or two ago, before it is known whether it stands: it nearly always does,
-                // and what is waited for below passes meanwhile.
-                const float m_spec = m_ref == -INFINITY ? 0.0f : m_ref;
-                weights(m_spec);
-                // the references as the tile before left them (another group's)
-                const int gb = (i + NG - 1) % NG;
-                if (i > i0) {
-                    ok = tc::mbar_wait_warp(&bars.dec[gb], ((i - 1) / NG) & 1, abort_flag, 65, max_polls);
-                    if (!ok) { give_up(); break; }
-                    const float m_now = s_mref[hd];
-                    if (m_now != m_ref) { l_acc *= exp2f(m_ref - m_now); m_ref = m_now; }
-                }
-                // As long as no score exceeds its row's reference by more than the lag the references stand: one barrier with an OR.
-                if (tc::barrier_any(6 + th, TM_GROUP, mx - m_ref > TM_LAG + TM_POFF)) {
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                    float fac = 1.0f;
-                    {
-                        const float tm = mx - TM_POFF;
-                        if (m_ref == -INFINITY) { if (tm > -INFINITY) m_ref = tm; }
-                        else if (tm > m_ref) { fac = exp2f(m_ref - tm); m_ref = tm; }
-                        if (lane < 16) { s_fac[hd] = fac; s_mref[hd] = m_ref; }
-                    }
-                    if (tc::barrier_any(9 + th, TM_GROUP, false)) { ok = false; break; }
-                    if (i >= i0 + NG) ok = pv_done(i - NG);
-                    if (ok && i > i0) ok = pv_done(i - 1);
-                    if (!ok) { if (i + NG < i1) give_up(); break; }
-                    tc::tc_fence_after();
-                    if (i > i0) {                          // O to the new references
-                        const float f = s_fac[orow];
-                        uint32_t r[32];
+                // The weights at the references as they were a tile or two ago, before it is known whether those stand: they nearly always
+                // do, and what is waited for meanwhile passes. If not, once more.
+                uint32_t hi_w[8], lo_w[8];                 // codes of the pairs of run k: row a's in the low half, row b's in the high one
+                float lt_a, lt_b;
+                bool again = false, left = false;
 #pragma unroll 1
-                        for (int c = 0; c < 8; ++c) {
-                            tc::tmem_ld32(TM_O + lane_base + c * 32, r);
-                            tc::tmem_ld_wait();
+                for (;;) {
+                    // P' = 2^(x - ref + 5) * scale as two e4m3 terms (through f16); the sums take 2^(x - ref + 5)
+                    const float ka = m_a == -INFINITY ? 0.0f : TM_POFF - m_a, kb = m_b == -INFINITY ? 0.0f : TM_POFF - m_b;
+                    f2 la = 0ull, lb = 0ull;
+                    __half2 top = __float2half2_rn(0.0f);
 #pragma unroll
-                            for (int h = 0; h < 32; ++h) r[h] = __float_as_uint(__uint_as_float(r[h]) * f);
-                            tc::tmem_st32(TM_O + lane_base + c * 32, r);
+                    for (int k = 0; k < 8; ++k) {
+                        const volatile f2* cv = sc;
+                        const f2 c8 = cv[4 * k];
+                        uint32_t ch[2], cl[2];
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const float2 t = unpack(add2(x[2 * k + r], r ? pack(kb, kb) : pack(ka, ka)));
+                            float w0, w1;
+                            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w0) : "f"(t.x));
+                            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w1) : "f"(t.y));
+                            const f2 ww = pack(w0, w1);
+                            if (r) lb = add2(lb, ww); else la = add2(la, ww);
+                            const float2 p = unpack(mul2(ww, c8));
+                            const __half2 ph = __floats2half2_rn(p.x, p.y);
+                            top = __hmax2(top, ph);
+                            const uint32_t phb = *reinterpret_cast<const uint32_t*>(&ph);
+                            uint16_t c, d;
+                            uint32_t back;
+                            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(c) : "r"(phb));
+                            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(c));
+                            const __half2 rest = __hsub2(ph, *reinterpret_cast<const __half2*>(&back));
+                            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(d) : "r"(*reinterpret_cast<const uint32_t*>(&rest)));
+                            ch[r] = c; cl[r] = d;
                         }
-                        tc::tmem_st_wait();
+                        hi_w[k] = ch[0] | (ch[1] << 16);
+                        lo_w[k] = cl[0] | (cl[1] << 16);
                     }
-                    l_acc *= fac;
-                    tc::tc_fence_before();
-                }
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&bars.dec[th]);
-                const float m_use = m_ref == -INFINITY ? 0.0f : m_ref;
-                if (__any_sync(0xffffffffu, m_use != m_spec)) weights(m_use);
-                l_acc += l_t;
-                // the buffer was read by the products of this group's tile before
-                if (i >= i0 + NG) ok = pv_done(i - NG);
-                if (!ok) { if (i + NG < i1) give_up(); break; }
+                    const float2 sa = unpack(la), sbb = unpack(lb);
+                    lt_a = sa.x + sa.y; lt_b = sbb.x + sbb.y;
+                    if (again) break;
+                    const float was_a = m_a, was_b = m_b;
+                    // the references as the tile before left them (another group's)
+                    const int gb = th ? th - 1 : NG - 1;
+                    if (i > i0) {
+                        ok = wait_for(&bars.dec[gb], ((i - 1) / NG) & 1, abort_flag, 65, max_polls);
+                        const float na = s_mref[ra], nb = s_mref[rb];
+                        if (na != m_a) { l_a *= exp2f(m_a - na); m_a = na; }
+                        if (nb != m_b) { l_b *= exp2f(m_b - nb); m_b = nb; }
+                    }
+                    // They stand as long as no P' exceeds 2^(5 + 3) by them (one barrier with an OR), and a row that has none sees nothing.
+                    bool grown = i == i0 || __any_sync(0xffffffffu, m_a != was_a || m_b != was_b);
+                    if (!grown) {
+                        const float2 t2 = __half22float2(top);
+                        grown = fmaxf(t2.x, t2.y) > 256.0f;
+                        if (m_a == -INFINITY || m_b == -INFINITY) {
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    uint8_t* prow = smem + SM_P + th * PBUF + sw64_chunk(hd, 2 * hf + tb);
-                    *reinterpret_cast<uint4*>(prow) = make_uint4(hi_w[4 * hf], hi_w[4 * hf + 1], hi_w[4 * hf + 2], hi_w[4 * hf + 3]);
-                    *reinterpret_cast<uint4*>(prow + PTERM) = make_uint4(lo_w[4 * hf], lo_w[4 * hf + 1], lo_w[4 * hf + 2], lo_w[4 * hf + 3]);
+                            for (int k = 0; k < 16; ++k) { const float2 y = unpack(x[k]); grown |= ((k & 1) ? m_b : m_a) == -INFINITY && fmaxf(y.x, y.y) > -INFINITY; }
+                        }
+                    }
+                    if (tc::barrier_any(6 + th, TM_GROUP, grown || !ok)) {
+                        // the largest x + log2(scale) of a row is what P' goes by
+                        float ta = -INFINITY, tb2 = -INFINITY;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float2 s2 = unpack(sc[4 * k]), ya = unpack(x[2 * k]), yb = unpack(x[2 * k + 1]);
+                            const float g0 = __log2f(s2.x), g1 = __log2f(s2.y);
+                            ta = fmaxf(ta, fmaxf(ya.x + g0, ya.y + g1)); tb2 = fmaxf(tb2, fmaxf(yb.x + g0, yb.y + g1));
+                        }
+#pragma unroll
+                        for (int o = 1; o < 4; o <<= 1) { ta = fmaxf(ta, __shfl_xor_sync(0xffffffffu, ta, o)); tb2 = fmaxf(tb2, __shfl_xor_sync(0xffffffffu, tb2, o)); }
+                        // a reference that stands keeps its lag; any that does not takes all of the growth
+                        auto move = [](float& m, float top_now) -> float {
+                            float f = 1.0f;
+                            if (m == -INFINITY) { if (top_now > -INFINITY) m = top_now; }
+                            else if (top_now > m + TM_LAG) { f = exp2f(m - top_now); m = top_now; }
+                            return f;
+                        };
+                        const float fa = move(m_a, ta), fb = move(m_b, tb2);
+                        if (tq == 0) { s_fac[ra] = fa; s_mref[ra] = m_a; s_fac[rb] = fb; s_mref[rb] = m_b; }
+                        left = tc::barrier_any(9 + th, TM_GROUP, !ok);
+                        const float f = s_fac[orow];
+                        if (!left && i > i0 && __any_sync(0xffffffffu, f != 1.0f)) {       // O to the new references
+                            if (i >= i0 + NG) ok = pv_done(i - NG);
+                            if (ok) ok = pv_done(i - 1);
+                            tc::tc_fence_after();
+                            uint32_t r[32];
+#pragma unroll 1
+                            for (int c = 0; c < 8; ++c) {
+                                tc::tmem_ld32(TM_O + lane_base + c * 32, r);
+                                tc::tmem_ld_wait();
+#pragma unroll
+                                for (int h = 0; h < 32; ++h) r[h] = __float_as_uint(__uint_as_float(r[h]) * f);
+                                tc::tmem_st32(TM_O + lane_base + c * 32, r);
+                            }
+                            tc::tmem_st_wait();
+                            tc::tc_fence_before();
+                        }
+                        l_a *= fa; l_b *= fb;
+                    }
+                    __syncwarp();
+                    if (left) break;
+                    if (lane == 0) tc::mbar_arrive(&bars.dec[th]);
+                    if (!__any_sync(0xffffffffu, m_a != was_a || m_b != was_b)) break;
+                    again = true;
+                }
+                if (left) { ok = false; break; }                   // (the group has agreed on it)
+                if (ok && i >= i0 + NG) ok = pv_done(i - NG);      // the buffer was read by the products of this group's tile before
+                if (!ok) { if (i + NG < i1) give_up(); break; }
+                l_a += lt_a; l_b += lt_b;
+                {
+                    uint8_t* prow = smem + SM_P + th * PBUF + ra * 64 + tq;
+                    const int sx = (ra >> 1) & 3;              // (the same for row b, 512 bytes on)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        uint8_t* at = prow + ((((k >> 1) ^ sx) << 4) + (k & 1) * 8);
+                        *reinterpret_cast<uint16_t*>(at) = (uint16_t)hi_w[k];
+                        *reinterpret_cast<uint16_t*>(at + 512) = (uint16_t)(hi_w[k] >> 16);
+                        *reinterpret_cast<uint16_t*>(at + PTERM) = (uint16_t)lo_w[k];
+                        *reinterpret_cast<uint16_t*>(at + PTERM + 512) = (uint16_t)(lo_w[k] >> 16);
+                    }
                 }
                 tc::fence_proxy_async();
                 __syncwarp();
@@ -761,16 +783,19 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
             }
 
             // ---- epilogue of the segment ----
-            // l per row: its six threads (two lanes 16 apart in a warp of each group) meet at the last reference
+            // l per row: its twelve threads (four neighbouring lanes in a warp of each group) meet at the last reference
             const int own = i1 - 1 - (i1 - 1 - th + NG) % NG;  // this group's last tile
             if (ok && own >= i0) ok = pv_done(own);
             if (ok) ok = pv_done(i1 - 1);
             failed = tc::barrier_any(1, TM_SOFTMAX, !ok);  // (all leave the loop over segments together)
             const float m_last = s_mref[hd];
             {
-                if (m_last != m_ref) l_acc *= exp2f(m_ref - m_last);
-                const float mine = l_acc + __shfl_xor_sync(0xffffffffu, l_acc, 16);
-                if (lane < 16) s_wmax[th * 64 + hd] = mine;
+                const float na = s_mref[ra], nb = s_mref[rb];
+                if (na != m_a) l_a *= exp2f(m_a - na);
+                if (nb != m_b) l_b *= exp2f(m_b - nb);
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) { l_a += __shfl_xor_sync(0xffffffffu, l_a, o); l_b += __shfl_xor_sync(0xffffffffu, l_b, o); }
+                if (tq == 0) { s_wmax[th * 64 + ra] = l_a; s_wmax[th * 64 + rb] = l_b; }
             }
             tc::named_barrier(1, TM_SOFTMAX);
             tc::tc_fence_after();
