@@ -23,9 +23,9 @@
 // weight is 0, but 0 x NaN is NaN: in V, NaN codes of tree rows become 0 (in K they make a score NaN, which the mask takes away from the
 // nodes that do not see the row, and from them alone).
 //
-// Tensor memory: S twice (64 columns each), q (128: its latent columns are the A operand of the QK products), O (256). Warps: 0-11 softmax
-// and epilogue in three groups that take the tiles in turn, 12 QK issue, 13 PV issue (in the pair's second CTA these two pass on that its
-// K and V are there), 14 gathers K, 15 gathers V. All waits are bounded (tc_common.cuh).
+// Tensor memory: S twice (64 columns each), q (128: its latent columns are the A operand of the QK products), O (256). Warps: 0-7 softmax
+// and epilogue in two groups that take the tiles in turn, 8 QK issue, 9 PV issue (in the pair's second CTA these two pass on that its K and
+// V are there), 10-12 gather K, 13-15 V. All waits are bounded (tc_common.cuh).
 #include <atomic>
 
 #include "codec.cuh"
@@ -40,10 +40,10 @@ namespace {
 constexpr int TM_TILE = 64, TM_ROWS = 64, TM_BLOCK = 2 * TM_ROWS;   // cache rows of a tile; (node, head) rows of a CTA, of a pair
 constexpr int TM_KVL = 512, TM_ROPE = 64, TM_W = TM_KVL + TM_ROPE;
 constexpr int TM_OWN = TM_TILE / 2;                  // tokens of a tile whose K a CTA holds
-constexpr int NK = 4, NV = 6, NG = 3;                // stages of K and of V; softmax groups, each with a P' buffer
-constexpr int TM_SW = 4 * NG, TM_QKW = TM_SW, TM_PVW = TM_SW + 1, TM_KW = TM_SW + 2, TM_VW = TM_SW + 3;
-constexpr int TM_THREADS = (TM_VW + 1) * 32, TM_SOFTMAX = TM_SW * 32, TM_GROUP = 128;
-constexpr float TM_POFF = 5.0f, TM_LAG = 3.0f;       // P' = 2^(s - ref + 5) <= 2^8, see attend_mma.cu
+constexpr int NK = 5, NV = 6, NG = 2, GW = 3;        // stages of K and of V; softmax groups, each with a P' buffer; warps that gather K, and V
+constexpr int TM_SW = 4 * NG, TM_QKW = TM_SW, TM_PVW = TM_SW + 1, TM_KW = TM_SW + 2, TM_VW = TM_KW + GW;
+constexpr int TM_THREADS = (TM_VW + GW) * 32, TM_SOFTMAX = TM_SW * 32, TM_GROUP = 128;
+constexpr float TM_POFF = 5.0f, TM_MOST = 256.0f;    // P' = 2^(s - ref + 5) <= 2^8: references lag by 2^3 at most, see attend_mma.cu
 constexpr int TM_MIN_UNITS = 4;                      // tiles a pair takes at least, while there are few
 constexpr int TM_PAIRS = RV_SMS / 2;
 
@@ -62,8 +62,8 @@ constexpr int PTERM = 4096, PBUF = 2 * PTERM;
 constexpr int SM_TOK = SM_P + NG * PBUF;                    // f32 [NV][64]: the tokens' scales
 constexpr int SM_SEE = SM_TOK + NV * TM_TILE * 4;           // u64 [NV][2]: tokens that are there; tokens whose scale is no number
 constexpr int SM_AHI = SM_SEE + NV * 16;                    // f32 [64] query scale * softmax scale * log2(e)
-constexpr int SM_WMAX = SM_AHI + 256;                       // f32 [3][64]
-constexpr int SM_FAC = SM_WMAX + 768;                       // f32 [64]
+constexpr int SM_WMAX = SM_AHI + 256;                       // f32 [NG][64]
+constexpr int SM_FAC = SM_WMAX + NG * 256;                  // f32 [64]
 constexpr int SM_MREF = SM_FAC + 256;                       // f32 [64]
 constexpr int SM_BARS = SM_MREF + 256;
 constexpr int SM_MISC = SM_BARS + 512;
@@ -248,25 +248,26 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
     w.nt = w.nrb = 0;
     if (w.left > 0) { w.s = tree_seq(A, w.b); units_of(A, w.s, w.nt, w.nrb); }
 
-    if (warp == TM_KW || warp == TM_VW) {
+    if (warp >= TM_KW) {
         // ------------------------------ gather ---------------------------------------------------
-        // Warp 14 fetches K (this CTA's 32 tokens of a tile) and writes the scales of all 64, warp 15 fetches V. Neither waits for its
-        // copies: they signal the stage themselves. Rows past the end and on unmapped pages are written as zeros.
+        // Three warps fetch K (this CTA's 32 tokens of a tile) and write the scales of all 64, three fetch V, a tile in turn. None waits
+        // for its copies: they signal the stage themselves. Rows past the end and on unmapped pages are written as zeros.
         // A lane resolves two tokens of a tile, 32 apart: entry -> page -> pool row -> scale, each level asked for a tile or more before it
         // is used (the loads come back through queues that the copies have filled).
-        const bool is_k = warp == TM_KW;
+        const bool is_k = warp < TM_VW;
         const int shift = rv_log2(A.page_tokens);
         constexpr uint32_t NONE = 0xffffffffu;
         bool ok = true;
-        int s = 0, use = 0, sv = 0, usev = 0;      // stage and use of it; of V's ring, whose depth the token words share
-        const int depth = is_k ? NK : NV;
+        const int g = warp - (is_k ? TM_KW : TM_VW), depth = is_k ? NK : NV;
+        int s = g, use = 0, sv = g, usev = 0;      // stage and use of it; of V's ring, whose depth the token words share
+        int turn = g;                              // tiles of the next segment before this warp's first
         for (; ok && walk_segment(A, w); walk_on(A, w)) {
             const int total = w.s.n + w.s.T;
             {   // the queries of the CTA's rows on their way to L2: they are read when the softmax warps come to this segment
                 const int r0 = w.rb * TM_BLOCK + rank * TM_ROWS, bytes = min(TM_ROWS, w.s.T * A.H - r0) * TM_W * 2;
                 const char* at = reinterpret_cast<const char*>(A.q + ((size_t)w.s.node0 * A.H + r0) * TM_W);
 #pragma unroll 1
-                for (int o = ((is_k ? 0 : 32) + lane) * 128; o < bytes; o += 64 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + o));
+                for (int o = ((warp - TM_KW) * 32 + lane) * 128; o < bytes; o += 2 * GW * 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + o));
             }
             const int tj = box_rows && !w.s.listed ? max(w.t0, min(w.t1, w.s.n / TM_TILE)) : w.t0;   // tiles from here on are gathered
             const int32_t* table = A.block_table + (size_t)w.b * A.max_pages;
@@ -279,101 +280,26 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                 return pg >= 0 && pg < A.n_pool_pages ? (uint32_t)pg * (uint32_t)A.page_tokens + (tok & (uint32_t)(A.page_tokens - 1)) : NONE;
             };
             auto scale = [&](uint32_t r) -> float { return is_k && r != NONE ? A.pscale[r] : 0.0f; };
-            uint32_t row[2], row1[2], tok2[2];     // pool rows of tiles t and t + 1; entries of tile t + 2
+            uint32_t row[2], row1[2], tok2[2];     // pool rows of this warp's tile t and its next; entries of the one after
+            int t = w.t0 + turn;
             float scl[2];                          // scales of tile t
 #pragma unroll
-            for (int u = 0; u < 2; ++u) { row[u] = entry(w.t0, u); row1[u] = entry(w.t0 + 1, u); tok2[u] = entry(w.t0 + 2, u); }
+            for (int u = 0; u < 2; ++u) { row[u] = entry(t, u); row1[u] = entry(t + GW, u); tok2[u] = entry(t + 2 * GW, u); }
 #pragma unroll
             for (int u = 0; u < 2; ++u) { row[u] = pool_row(row[u], page(row[u])); row1[u] = pool_row(row1[u], page(row1[u])); }
 #pragma unroll
             for (int u = 0; u < 2; ++u) scl[u] = scale(row[u]);
-#pragma unroll 1
-            for (int t = w.t0; t < w.t1; ++t) {
-                float scl1[2];
-                int pg2[2];
-                uint32_t tok3[2];
+            float scl1[2];
+            int pg2[2];
+            uint32_t tok3[2];
+            // A stage of one's own ring (K: and of the token words') is free; the loads that later tiles need are on their way before it is.
+            auto begin = [&](int t) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) { scl1[u] = scale(row1[u]); pg2[u] = page(tok2[u]); tok3[u] = entry(t + 3, u); }
-                uint64_t* full = (is_k ? bars.k_full : bars.v_full) + s;
-                if (usev > 0) ok = wait_for(&bars.v_empty[sv], (usev & 1) ^ 1, abort_flag, 41, max_polls);   // (K: for the token words)
+                for (int u = 0; u < 2; ++u) { scl1[u] = scale(row1[u]); pg2[u] = page(tok2[u]); tok3[u] = entry(t + 3 * GW, u); }
+                if (usev > 0) ok = wait_for(&bars.v_empty[sv], (usev & 1) ^ 1, abort_flag, 41, max_polls);
                 if (ok && is_k && use > 0) ok = wait_for(&bars.k_empty[s], (use & 1) ^ 1, abort_flag, 42, max_polls);
-                if (!ok) break;
-                uint8_t* buf = smem + (is_k ? SM_K + s * KSTAGE : SM_V + s * VSTAGE);
-                const uint32_t at = tc::smem_u32(buf);
-                if (t < tj) {
-                    // tensor copies: box k holds tokens k * box_rows on, of the CTA's 32 (K) or of all (V)
-                    const int boxes = (is_k ? TM_OWN : TM_TILE) / box_rows, slot = (is_k ? rank * TM_OWN : 0) + lane * box_rows;
-                    const uint32_t y0 = __shfl_sync(0xffffffffu, row[0], slot & 31), y1 = __shfl_sync(0xffffffffu, row[1], slot & 31);
-                    const uint32_t y = (slot & 32) ? y1 : y0;
-                    const bool mine = lane < boxes && y != NONE;
-                    const uint32_t mapped = __ballot_sync(0xffffffffu, mine);
-                    if (lane == 0) tc::mbar_arrive_expect_tx(full, __popc(mapped) * box_rows * (is_k ? TM_W : 256));
-                    __syncwarp();
-                    if (mine) {
-                        if (is_k) {
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) tc::tma_load_2d(at + c * KCHUNK + lane * box_rows * 128, &latents, c * 128, (int)y, full);
-                            tc::tma_load_2d(at + 4 * KCHUNK + lane * box_rows * 64, &ropes, TM_KVL, (int)y, full);
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < 2; ++c) tc::tma_load_2d(at + c * VCHUNK + lane * box_rows * 128, &latents, (2 * c + rank) * 128, (int)y, full);
-                        }
-                    }
-                    if (__popc(mapped) != boxes) {             // pages that are not there: zeros
-                        const int chunks = is_k ? 36 : 16, rows = is_k ? TM_OWN : TM_TILE;
-#pragma unroll 1
-                        for (int x = lane; x < rows * chunks; x += 32) {
-                            const int r = x / chunks, c = x - r * chunks;
-                            if ((mapped >> (r / box_rows)) & 1) continue;
-                            *reinterpret_cast<uint4*>(buf + (!is_k ? (c >> 3) * VCHUNK + tc::sw128_chunk(r, c & 7) : c < 32 ? (c >> 3) * KCHUNK + tc::sw128_chunk(r, c & 7)
-                                                                                                                              : 4 * KCHUNK + sw64_chunk(r, c - 32))) = make_uint4(0u, 0u, 0u, 0u);
-                        }
-                        tc::fence_proxy_async();
-                        __syncwarp();
-                    }
-                    if (lane == 0) mbar_arrive_n(full, FULL - 1);
-                } else {
-                    if (is_k) {
-                        const uint32_t own = rank ? row[1] : row[0];
-#pragma unroll 8
-                        for (int it = 0; it < TM_OWN; ++it) {
-                            const uint32_t r = __shfl_sync(0xffffffffu, own, it);
-                            tc::cp_async16_zfill(at + (lane >> 3) * KCHUNK + tc::sw128_chunk(it, lane & 7),
-                                                 A.pool + (r != NONE ? (size_t)r * TM_W + lane * 16 : 0), r != NONE ? 16u : 0u);
-                        }
-#pragma unroll
-                        for (int it = 0; it < 4; ++it) {
-                            const int rl = it * 8 + (lane >> 2);
-                            const uint32_t r = __shfl_sync(0xffffffffu, own, rl);
-                            tc::cp_async16_zfill(at + 4 * KCHUNK + sw64_chunk(rl, lane & 3),
-                                                 A.pool + (r != NONE ? (size_t)r * TM_W + TM_KVL + (lane & 3) * 16 : 0), r != NONE ? 16u : 0u);
-                        }
-                    } else {
-                        const int c = lane & 15;
-                        const uint8_t* from = A.pool + (2 * (c >> 3) + rank) * 128 + (c & 7) * 16;
-#pragma unroll 8
-                        for (int it = 0; it < 32; ++it) {              // two rows an instruction, 16 chunks each
-                            const int rl = 2 * it + (lane >> 4);
-                            const uint32_t r = __shfl_sync(0xffffffffu, it < 16 ? row[0] : row[1], rl & 31);
-                            tc::cp_async16_zfill(at + (c >> 3) * VCHUNK + tc::sw128_chunk(rl, c & 7), r != NONE ? from + (size_t)r * TM_W : A.pool, r != NONE ? 16u : 0u);
-                        }
-                        if ((t + 1) * TM_TILE > w.s.n) {
-                            // rows of the tree: each lane looks through what it copied itself, once it is there
-                            tc::cp_async_commit();
-                            tc::cp_async_wait<0>();
-#pragma unroll 1
-                            for (int it = 0; it < 32; ++it) {
-                                const int rl = 2 * it + (lane >> 4);
-                                uint4* v = reinterpret_cast<uint4*>(buf + (c >> 3) * VCHUNK + tc::sw128_chunk(rl, c & 7));
-                                if (t * TM_TILE + rl >= w.s.n) { const uint4 x = *v; *v = make_uint4(no_nan(x.x), no_nan(x.y), no_nan(x.z), no_nan(x.w)); }
-                            }
-                        }
-                    }
-                    tc::cp_async_mbar_arrive_noinc(full);
-                    tc::fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(full);
-                }
+            };
+            auto end = [&]() {
                 if (is_k) {
                     uint32_t there[2], wild[2];
 #pragma unroll
@@ -387,11 +313,103 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(&bars.tok_full[sv]);
                 }
-                if (++s == depth) { s = 0; ++use; }
-                if (++sv == NV) { sv = 0; ++usev; }
+                if ((s += GW) >= depth) { s -= depth; ++use; }
+                if ((sv += GW) >= NV) { sv -= NV; ++usev; }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) { row[u] = row1[u]; scl[u] = scl1[u]; row1[u] = pool_row(tok2[u], pg2[u]); tok2[u] = tok3[u]; }
+            };
+            // Tensor copies: box k holds tokens k * box_rows on, of the CTA's 32 (K) or of all (V).
+            const int boxes = tj > w.t0 ? (is_k ? TM_OWN : TM_TILE) / box_rows : 0, slot = (is_k ? rank * TM_OWN : 0) + lane * box_rows;
+#pragma unroll 1
+            for (; t < tj; t += GW) {
+                begin(t);
+                if (!ok) break;
+                uint64_t* full = (is_k ? bars.k_full : bars.v_full) + s;
+                const uint32_t at = tc::smem_u32(smem) + (is_k ? SM_K + s * KSTAGE : SM_V + s * VSTAGE);
+                const uint32_t y0 = __shfl_sync(0xffffffffu, row[0], slot & 31), y1 = __shfl_sync(0xffffffffu, row[1], slot & 31);
+                const uint32_t y = (slot & 32) ? y1 : y0;
+                const bool mine = lane < boxes && y != NONE;
+                const uint32_t mapped = __ballot_sync(0xffffffffu, mine);
+                if (lane == 0) tc::mbar_arrive_expect_tx(full, __popc(mapped) * box_rows * (is_k ? TM_W : 256));
+                __syncwarp();
+                if (mine) {
+                    if (is_k) {
+                        const uint32_t to = at + lane * box_rows * 128;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) tc::tma_load_2d(to + c * KCHUNK, &latents, c * 128, (int)y, full);
+                        tc::tma_load_2d(at + 4 * KCHUNK + lane * box_rows * 64, &ropes, TM_KVL, (int)y, full);
+                    } else {
+                        const uint32_t to = at + lane * box_rows * 128;
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) tc::tma_load_2d(to + c * VCHUNK, &latents, (2 * c + rank) * 128, (int)y, full);
+                    }
+                }
+                if (__builtin_expect(__popc(mapped) != boxes, 0)) {        // pages that are not there: zeros
+                    uint8_t* buf = smem + (is_k ? SM_K + s * KSTAGE : SM_V + s * VSTAGE);
+                    const int chunks = is_k ? 36 : 16, rows = is_k ? TM_OWN : TM_TILE;
+#pragma unroll 1
+                    for (int x = lane; x < rows * chunks; x += 32) {
+                        const int r = x / chunks, c = x - r * chunks;
+                        if ((mapped >> (r / box_rows)) & 1) continue;
+                        *reinterpret_cast<uint4*>(buf + (!is_k ? (c >> 3) * VCHUNK + tc::sw128_chunk(r, c & 7) : c < 32 ? (c >> 3) * KCHUNK + tc::sw128_chunk(r, c & 7)
+                                                                                                                          : 4 * KCHUNK + sw64_chunk(r, c - 32))) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    tc::fence_proxy_async();
+                    __syncwarp();
+                }
+                if (lane == 0) mbar_arrive_n(full, FULL - 1);
+                end();
             }
+#pragma unroll 1
+            for (; t < w.t1 && ok; t += GW) {
+                begin(t);
+                if (!ok) break;
+                uint64_t* full = (is_k ? bars.k_full : bars.v_full) + s;
+                uint8_t* buf = smem + (is_k ? SM_K + s * KSTAGE : SM_V + s * VSTAGE);
+                const uint32_t at = tc::smem_u32(buf);
+                if (is_k) {
+                    const uint32_t own = rank ? row[1] : row[0];
+#pragma unroll 8
+                    for (int it = 0; it < TM_OWN; ++it) {
+                        const uint32_t r = __shfl_sync(0xffffffffu, own, it);
+                        tc::cp_async16_zfill(at + (lane >> 3) * KCHUNK + tc::sw128_chunk(it, lane & 7),
+                                             A.pool + (r != NONE ? (size_t)r * TM_W + lane * 16 : 0), r != NONE ? 16u : 0u);
+                    }
+#pragma unroll
+                    for (int it = 0; it < 4; ++it) {
+                        const int rl = it * 8 + (lane >> 2);
+                        const uint32_t r = __shfl_sync(0xffffffffu, own, rl);
+                        tc::cp_async16_zfill(at + 4 * KCHUNK + sw64_chunk(rl, lane & 3),
+                                             A.pool + (r != NONE ? (size_t)r * TM_W + TM_KVL + (lane & 3) * 16 : 0), r != NONE ? 16u : 0u);
+                    }
+                } else {
+                    const int c = lane & 15;
+                    const uint8_t* from = A.pool + (2 * (c >> 3) + rank) * 128 + (c & 7) * 16;
+#pragma unroll 8
+                    for (int it = 0; it < 32; ++it) {                  // two rows an instruction, 16 chunks each
+                        const int rl = 2 * it + (lane >> 4);
+                        const uint32_t r = __shfl_sync(0xffffffffu, it < 16 ? row[0] : row[1], rl & 31);
+                        tc::cp_async16_zfill(at + (c >> 3) * VCHUNK + tc::sw128_chunk(rl, c & 7), r != NONE ? from + (size_t)r * TM_W : A.pool, r != NONE ? 16u : 0u);
+                    }
+                    if ((t + 1) * TM_TILE > w.s.n) {
+                        // rows of the tree: each lane looks through what it copied itself, once it is there
+                        tc::cp_async_commit();
+                        tc::cp_async_wait<0>();
+#pragma unroll 4
+                        for (int it = 0; it < 32; ++it) {
+                            const int rl = 2 * it + (lane >> 4);
+                            uint4* v = reinterpret_cast<uint4*>(buf + (c >> 3) * VCHUNK + tc::sw128_chunk(rl, c & 7));
+                            if (t * TM_TILE + rl >= w.s.n) { const uint4 x = *v; *v = make_uint4(no_nan(x.x), no_nan(x.y), no_nan(x.z), no_nan(x.w)); }
+                        }
+                    }
+                }
+                tc::cp_async_mbar_arrive_noinc(full);
+                tc::fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(full);
+                end();
+            }
+            turn = t - w.t1;
         }
     } else if (warp == TM_QKW || warp == TM_PVW) {
         if (rank == 1) {
@@ -414,13 +432,13 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
             const uint32_t id_qk = tc::idesc_e4m3(256, TM_TILE, 0, 0);
             const uint64_t d_qr = smem_desc(tc::smem_u32(smem + SM_QR), 16, 512, 4);
             bool ok = true;
-            int i = 0, seg = 0;
+            int i = 0, seg = 0, s = 0, phase = 0, g = 0;
             for (; ok && walk_segment(A, w); walk_on(A, w), ++seg) {
                 ok = wait_for(&bars.q_full, seg & 1, abort_flag, 51, max_polls);
+#pragma unroll 1
                 for (int t = w.t0; t < w.t1 && ok; ++t, ++i) {
-                    const int s = i % NK, use = i / NK, sb = i & 1;
-                    ok = wait_for(&bars.k_full[s], use & 1, abort_flag, 52, max_polls) &&
-                         wait_for(&bars.k_peer[s], use & 1, abort_flag, 56, max_polls) &&
+                    const int sb = i & 1;
+                    ok = wait_for(&bars.k_full[s], phase, abort_flag, 52, max_polls) && wait_for(&bars.k_peer[s], phase, abort_flag, 56, max_polls) &&
                          wait_for(&bars.s_empty[sb], ((i >> 1) & 1) ^ 1, abort_flag, 53, max_polls);
                     if (!ok) break;
                     tc::fence_proxy_async();   // copies that wrote through the generic proxy, the products read through the async one
@@ -437,22 +455,23 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                             for (int k = 0; k < 4; ++k)
                                 tc::mma2_f8_ta(d, TM_Q + (uint32_t)(c * 32 + k * 8), d_k + (uint64_t)((c * KCHUNK + k * 32) >> 4), id_qk, 1);
                         tc::commit2(&bars.k_empty[s]);
-                        tc::commit2(&bars.s_full[i % NG]);
+                        tc::commit2(&bars.s_full[g]);
                     }
                     __syncwarp();
+                    if (++s == NK) { s = 0; phase ^= 1; }
+                    if (++g == NG) g = 0;
                 }
             }
         } else {
             // ------------------------------ PV issuer: O += P'(i) . V(i) --------------------------
             const uint32_t id_pv = tc::idesc_e4m3(128, 256, 0, 1);
             bool ok = true;
-            int i = 0;
+            int s = 0, phase = 0, pb = 0, p_phase = 0;
             for (; ok && walk_segment(A, w); walk_on(A, w)) {
-                for (int t = w.t0; t < w.t1 && ok; ++t, ++i) {
-                    const int s = i % NV, use = i / NV, pb = i % NG;
-                    ok = wait_for(&bars.v_full[s], use & 1, abort_flag, 58, max_polls) &&
-                         wait_for(&bars.v_peer[s], use & 1, abort_flag, 59, max_polls) &&
-                         wait_for(&bars.p_full[pb], (i / NG) & 1, abort_flag, 54, max_polls);
+#pragma unroll 1
+                for (int t = w.t0; t < w.t1 && ok; ++t) {
+                    ok = wait_for(&bars.v_full[s], phase, abort_flag, 58, max_polls) && wait_for(&bars.v_peer[s], phase, abort_flag, 59, max_polls) &&
+                         wait_for(&bars.p_full[pb], p_phase, abort_flag, 54, max_polls);
                     if (!ok) break;
                     tc::fence_proxy_async();
                     tc::tc_fence_after();
@@ -469,6 +488,8 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                         tc::commit2(&bars.pv_done[pb]);
                     }
                     __syncwarp();
+                    if (++s == NV) { s = 0; phase ^= 1; }
+                    if (++pb == NG) { pb = 0; p_phase ^= 1; }
                 }
             }
         }
@@ -608,10 +629,12 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
             float l_a = 0.0f, l_b = 0.0f, m_a = -INFINITY, m_b = -INFINITY;   // sums, and the references they are at
             const int i1 = i0 + (w.t1 - w.t0);
             bool ok = true;
+            int i = i0 + (th + 2 * NG - i0 % NG) % NG;
+            int n = i / NG, sv = i % NV, usev = i / NV;    // the group's tiles before; slot and use of the token words
 #pragma unroll 1
-            for (int i = i0 + (th + 2 * NG - i0 % NG) % NG; i < i1; i += NG) {
-                const int sv = i % NV, j0 = (w.t0 + i - i0) * TM_TILE, sb = i & 1;
-                ok = wait_for(&bars.tok_full[sv], (i / NV) & 1, abort_flag, 61, max_polls) && wait_for(&bars.s_full[th], (i / NG) & 1, abort_flag, 62, max_polls);
+            for (; i < i1; i += NG, ++n, usev += sv >= NV - NG, sv += sv >= NV - NG ? NG - NV : NG) {
+                const int j0 = (w.t0 + i - i0) * TM_TILE, sb = i & 1;
+                ok = wait_for(&bars.tok_full[sv], usev & 1, abort_flag, 61, max_polls) && wait_for(&bars.s_full[th], n & 1, abort_flag, 62, max_polls);
                 if (!ok) { give_up(); break; }
                 tc::tc_fence_after();
                 // x: scores in log2 units; [k][row][token tq + e] of each run k of eight tokens
@@ -640,7 +663,7 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                     x[2 * k] = mul2(x[2 * k], mul2(pack(a_a, a_a), c));
                     x[2 * k + 1] = mul2(x[2 * k + 1], mul2(pack(a_b, a_b), c));
                 }
-                if (j0 + TM_TILE > w.s.n || (see.x & see.y) != ~0u || (see.z | see.w)) {
+                if (__builtin_expect(j0 + TM_TILE > w.s.n || (see.x & see.y) != ~0u || (see.z | see.w), 0)) {
                     // rows of the tree, rows that are not there, scales that are no numbers: what a node does not see scores -inf
                     const uint64_t there = (uint64_t)see.y << 32 | see.x, wild = ((uint64_t)see.w << 32 | see.z) >> tq;
                     const uint64_t va = (tree_visible(mask_a, w.s.T, w.s.n, j0) & there) >> tq, vb = (tree_visible(mask_b, w.s.T, w.s.n, j0) & there) >> tq;
@@ -700,7 +723,7 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                     // the references as the tile before left them (another group's)
                     const int gb = th ? th - 1 : NG - 1;
                     if (i > i0) {
-                        ok = wait_for(&bars.dec[gb], ((i - 1) / NG) & 1, abort_flag, 65, max_polls);
+                        ok = wait_for(&bars.dec[gb], (n & 1) ^ (th == 0), abort_flag, 65, max_polls);
                         const float na = s_mref[ra], nb = s_mref[rb];
                         if (na != m_a) { l_a *= exp2f(m_a - na); m_a = na; }
                         if (nb != m_b) { l_b *= exp2f(m_b - nb); m_b = nb; }
@@ -709,13 +732,13 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                     bool grown = i == i0 || __any_sync(0xffffffffu, m_a != was_a || m_b != was_b);
                     if (!grown) {
                         const float2 t2 = __half22float2(top);
-                        grown = fmaxf(t2.x, t2.y) > 256.0f;
-                        if (m_a == -INFINITY || m_b == -INFINITY) {
+                        grown = fmaxf(t2.x, t2.y) > TM_MOST;
+                        if (__builtin_expect(m_a == -INFINITY || m_b == -INFINITY, 0)) {
 #pragma unroll
                             for (int k = 0; k < 16; ++k) { const float2 y = unpack(x[k]); grown |= ((k & 1) ? m_b : m_a) == -INFINITY && fmaxf(y.x, y.y) > -INFINITY; }
                         }
                     }
-                    if (tc::barrier_any(6 + th, TM_GROUP, grown || !ok)) {
+                    if (__builtin_expect(tc::barrier_any(6 + th, TM_GROUP, grown || !ok), 0)) {
                         // the largest x + log2(scale) of a row is what P' goes by
                         float ta = -INFINITY, tb2 = -INFINITY;
 #pragma unroll
@@ -726,11 +749,11 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                         }
 #pragma unroll
                         for (int o = 1; o < 4; o <<= 1) { ta = fmaxf(ta, __shfl_xor_sync(0xffffffffu, ta, o)); tb2 = fmaxf(tb2, __shfl_xor_sync(0xffffffffu, tb2, o)); }
-                        // a reference that stands keeps its lag; any that does not takes all of the growth
+                        // all references take all of their growth (taken by those alone that had to, the next tile's row would have to)
                         auto move = [](float& m, float top_now) -> float {
                             float f = 1.0f;
                             if (m == -INFINITY) { if (top_now > -INFINITY) m = top_now; }
-                            else if (top_now > m + TM_LAG) { f = exp2f(m - top_now); m = top_now; }
+                            else if (top_now > m) { f = exp2f(m - top_now); m = top_now; }
                             return f;
                         };
                         const float fa = move(m_a, ta), fb = move(m_b, tb2);
@@ -783,7 +806,7 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
             }
 
             // ---- epilogue of the segment ----
-            // l per row: its twelve threads (four neighbouring lanes in a warp of each group) meet at the last reference
+            // l per row: its eight threads (four neighbouring lanes in a warp of each group) meet at the last reference
             const int own = i1 - 1 - (i1 - 1 - th + NG) % NG;  // this group's last tile
             if (ok && own >= i0) ok = pv_done(own);
             if (ok) ok = pv_done(i1 - 1);
@@ -803,7 +826,7 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
             const int slot = 2 * pair + (w.t0 == 0 ? 1 : 0);
             if (th == 0 && lane < 16) {
                 // (l and O carry 2^5; NaN stays NaN)
-                const float l = s_wmax[hd] + s_wmax[64 + hd] + s_wmax[128 + hd];
+                const float l = s_wmax[hd] + s_wmax[64 + hd];
                 if (!whole) reinterpret_cast<float2*>(scratch + SC_ML)[slot * TM_BLOCK + rank * TM_ROWS + hd] = make_float2(m_last, l);
                 else if (hd < valid && A.out_lse) A.out_lse[flat + hd] = l == 0.0f ? -INFINITY : (m_last - TM_POFF) * 0.6931471805599453f + logf(l);
                 s_fac[hd] = l == 0.0f ? 0.0f : 1.0f / l;
