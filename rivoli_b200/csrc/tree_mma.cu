@@ -132,6 +132,15 @@ __device__ __forceinline__ f2 pack(float lo, float hi) { f2 r; asm("mov.b64 %0, 
 __device__ __forceinline__ float2 unpack(f2 v) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v)); return r; }
 __device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ f2 mul2(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+// Tensor copies: K's four chunks of 32 rows, V's two of 64 (y: pool row, z: the first chunk's parity).
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, int y, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(0), "r"(y), "r"(0), "r"(tc::smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(0), "r"(y), "r"(0), "r"(z), "r"(tc::smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -169,8 +178,8 @@ __device__ __forceinline__ void walk_on(const TreeArgs& A, Walk& w) {
 __device__ __forceinline__ long long run_begin(long long total, int g, int n) { return total * g / n; }
 
 __global__ void __launch_bounds__(TM_THREADS, 1)
-tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const __grid_constant__ CUtensorMap ropes, int box_rows, int* err, uint8_t* scratch,
-                int max_polls) {
+tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap r_map, const __grid_constant__ CUtensorMap v_map, int tma, int* err,
+                uint8_t* scratch, int max_polls) {
     extern __shared__ __align__(1024) uint8_t smem[];
     Bars& bars = *reinterpret_cast<Bars*>(smem + SM_BARS);
     float* s_tok = reinterpret_cast<float*>(smem + SM_TOK);
@@ -255,7 +264,7 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
         // A lane resolves two tokens of a tile, 32 apart: entry -> page -> pool row -> scale, each level asked for a tile or more before it
         // is used (the loads come back through queues that the copies have filled).
         const bool is_k = warp < TM_VW;
-        const int shift = rv_log2(A.page_tokens);
+        const int shift = rv_log2(A.page_tokens), inside = A.page_tokens - 1;
         constexpr uint32_t NONE = 0xffffffffu;
         bool ok = true;
         const int g = warp - (is_k ? TM_KW : TM_VW), depth = is_k ? NK : NV;
@@ -269,42 +278,21 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
 #pragma unroll 1
                 for (int o = ((warp - TM_KW) * 32 + lane) * 128; o < bytes; o += 2 * GW * 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + o));
             }
-            const int tj = box_rows && !w.s.listed ? max(w.t0, min(w.t1, w.s.n / TM_TILE)) : w.t0;   // tiles from here on are gathered
+            const int tj = tma && !w.s.listed ? max(w.t0, min(w.t1, w.s.n / TM_TILE)) : w.t0;   // tiles from here on are gathered
             const int32_t* table = A.block_table + (size_t)w.b * A.max_pages;
-            auto entry = [&](int t, int u) -> uint32_t {
-                const int j = t * TM_TILE + u * 32 + lane;
-                return t < w.t1 && j < total ? tree_token(A, w.s, w.b, j) : NONE;
-            };
-            auto page = [&](uint32_t tok) -> int { return tok != NONE && (tok >> shift) < (uint32_t)A.max_pages ? table[tok >> shift] : -1; };
-            auto pool_row = [&](uint32_t tok, int pg) -> uint32_t {
-                return pg >= 0 && pg < A.n_pool_pages ? (uint32_t)pg * (uint32_t)A.page_tokens + (tok & (uint32_t)(A.page_tokens - 1)) : NONE;
-            };
-            auto scale = [&](uint32_t r) -> float { return is_k && r != NONE ? A.pscale[r] : 0.0f; };
-            uint32_t row[2], row1[2], tok2[2];     // pool rows of this warp's tile t and its next; entries of the one after
             int t = w.t0 + turn;
-            float scl[2];                          // scales of tile t
-#pragma unroll
-            for (int u = 0; u < 2; ++u) { row[u] = entry(t, u); row1[u] = entry(t + GW, u); tok2[u] = entry(t + 2 * GW, u); }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) { row[u] = pool_row(row[u], page(row[u])); row1[u] = pool_row(row1[u], page(row1[u])); }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) scl[u] = scale(row[u]);
-            float scl1[2];
-            int pg2[2];
-            uint32_t tok3[2];
-            // A stage of one's own ring (K: and of the token words') is free; the loads that later tiles need are on their way before it is.
-            auto begin = [&](int t) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u) { scl1[u] = scale(row1[u]); pg2[u] = page(tok2[u]); tok3[u] = entry(t + 3 * GW, u); }
+            // A stage of one's own ring (K: and of the token words') is free.
+            auto stage_free = [&]() {
                 if (usev > 0) ok = wait_for(&bars.v_empty[sv], (usev & 1) ^ 1, abort_flag, 41, max_polls);
                 if (ok && is_k && use > 0) ok = wait_for(&bars.k_empty[s], (use & 1) ^ 1, abort_flag, 42, max_polls);
             };
-            auto end = [&]() {
+            // scales of the lane's two tokens and which are there, to the softmax warps; the next stage
+            auto stage_done = [&](const float* scl, bool mapped0, bool mapped1) {
                 if (is_k) {
                     uint32_t there[2], wild[2];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const bool odd = !(scl[u] < INFINITY), live = row[u] != NONE && !(scl[u] <= 0.0f);   // odd: NaN, or infinite
+                        const bool odd = !(scl[u] < INFINITY), live = (u ? mapped1 : mapped0) && !(scl[u] <= 0.0f);   // odd: NaN, or infinite
                         s_tok[sv * TM_TILE + u * 32 + lane] = !live ? 0.0f : odd ? 1.0f : scl[u];
                         there[u] = __ballot_sync(0xffffffffu, live);
                         wild[u] = __ballot_sync(0xffffffffu, live && odd);
@@ -315,99 +303,120 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                 }
                 if ((s += GW) >= depth) { s -= depth; ++use; }
                 if ((sv += GW) >= NV) { sv -= NV; ++usev; }
-#pragma unroll
-                for (int u = 0; u < 2; ++u) { row[u] = row1[u]; scl[u] = scl1[u]; row1[u] = pool_row(tok2[u], pg2[u]); tok2[u] = tok3[u]; }
             };
-            // Tensor copies: box k holds tokens k * box_rows on, of the CTA's 32 (K) or of all (V).
-            const int boxes = tj > w.t0 ? (is_k ? TM_OWN : TM_TILE) / box_rows : 0, slot = (is_k ? rank * TM_OWN : 0) + lane * box_rows;
+            if (t < tj) {
+                // Pages of 64 tokens and more, a tile inside one: K is two tensor copies, V is one. The page is asked for two of the warp's
+                // tiles ahead, the scales one.
+                auto page_of = [&](int x) -> int {
+                    const int lp = x * TM_TILE >> shift, pg = x < tj && lp < A.max_pages ? table[lp] : -1;
+                    return pg < A.n_pool_pages ? pg : -1;
+                };
+                auto row_of = [&](int x, int pg) -> uint32_t { return pg >= 0 ? (uint32_t)pg * (uint32_t)A.page_tokens + (uint32_t)(x * TM_TILE & inside) : NONE; };
+                uint32_t y = row_of(t, page_of(t));
+                int pg1 = page_of(t + GW);
+                float scl[2] = {0.0f, 0.0f};
+                if (is_k && y != NONE) { scl[0] = A.pscale[y + lane]; scl[1] = A.pscale[y + 32 + lane]; }
 #pragma unroll 1
-            for (; t < tj; t += GW) {
-                begin(t);
-                if (!ok) break;
-                uint64_t* full = (is_k ? bars.k_full : bars.v_full) + s;
-                const uint32_t at = tc::smem_u32(smem) + (is_k ? SM_K + s * KSTAGE : SM_V + s * VSTAGE);
-                const uint32_t y0 = __shfl_sync(0xffffffffu, row[0], slot & 31), y1 = __shfl_sync(0xffffffffu, row[1], slot & 31);
-                const uint32_t y = (slot & 32) ? y1 : y0;
-                const bool mine = lane < boxes && y != NONE;
-                const uint32_t mapped = __ballot_sync(0xffffffffu, mine);
-                if (lane == 0) tc::mbar_arrive_expect_tx(full, __popc(mapped) * box_rows * (is_k ? TM_W : 256));
-                __syncwarp();
-                if (mine) {
-                    if (is_k) {
-                        const uint32_t to = at + lane * box_rows * 128;
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) tc::tma_load_2d(to + c * KCHUNK, &latents, c * 128, (int)y, full);
-                        tc::tma_load_2d(at + 4 * KCHUNK + lane * box_rows * 64, &ropes, TM_KVL, (int)y, full);
-                    } else {
-                        const uint32_t to = at + lane * box_rows * 128;
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) tc::tma_load_2d(to + c * VCHUNK, &latents, (2 * c + rank) * 128, (int)y, full);
-                    }
-                }
-                if (__builtin_expect(__popc(mapped) != boxes, 0)) {        // pages that are not there: zeros
-                    uint8_t* buf = smem + (is_k ? SM_K + s * KSTAGE : SM_V + s * VSTAGE);
-                    const int chunks = is_k ? 36 : 16, rows = is_k ? TM_OWN : TM_TILE;
+                for (; t < tj; t += GW) {
+                    const uint32_t y1 = row_of(t + GW, pg1);
+                    pg1 = page_of(t + 2 * GW);
+                    float scl1[2] = {0.0f, 0.0f};
+                    if (is_k && y1 != NONE) { scl1[0] = A.pscale[y1 + lane]; scl1[1] = A.pscale[y1 + 32 + lane]; }
+                    stage_free();
+                    if (!ok) break;
+                    uint64_t* full = (is_k ? bars.k_full : bars.v_full) + s;
+                    const uint32_t at = tc::smem_u32(smem) + (is_k ? SM_K + s * KSTAGE : SM_V + s * VSTAGE);
+                    if (__builtin_expect(y == NONE, 0)) {          // a page that is not there: zeros
 #pragma unroll 1
-                    for (int x = lane; x < rows * chunks; x += 32) {
-                        const int r = x / chunks, c = x - r * chunks;
-                        if ((mapped >> (r / box_rows)) & 1) continue;
-                        *reinterpret_cast<uint4*>(buf + (!is_k ? (c >> 3) * VCHUNK + tc::sw128_chunk(r, c & 7) : c < 32 ? (c >> 3) * KCHUNK + tc::sw128_chunk(r, c & 7)
-                                                                                                                          : 4 * KCHUNK + sw64_chunk(r, c - 32))) = make_uint4(0u, 0u, 0u, 0u);
+                        for (int o = lane * 16; o < (is_k ? KSTAGE : VSTAGE); o += 512)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + o), "r"(0) : "memory");
+                        tc::fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_n(full, FULL);
+                    } else if (tc::elect_one()) {
+                        tc::mbar_arrive_expect_tx(full, is_k ? KSTAGE : VSTAGE);
+                        if (is_k) {
+                            tma_load_3d(at, &k_map, (int)y + rank * TM_OWN, full);
+                            tc::tma_load_2d(at + 4 * KCHUNK, &r_map, TM_KVL, (int)y + rank * TM_OWN, full);
+                        } else {
+                            tma_load_4d(at, &v_map, (int)y, rank, full);
+                        }
+                        mbar_arrive_n(full, FULL - 1);
                     }
-                    tc::fence_proxy_async();
                     __syncwarp();
+                    stage_done(scl, y != NONE, y != NONE);
+                    y = y1; scl[0] = scl1[0]; scl[1] = scl1[1];
                 }
-                if (lane == 0) mbar_arrive_n(full, FULL - 1);
-                end();
             }
-#pragma unroll 1
-            for (; t < w.t1 && ok; t += GW) {
-                begin(t);
-                if (!ok) break;
-                uint64_t* full = (is_k ? bars.k_full : bars.v_full) + s;
-                uint8_t* buf = smem + (is_k ? SM_K + s * KSTAGE : SM_V + s * VSTAGE);
-                const uint32_t at = tc::smem_u32(buf);
-                if (is_k) {
-                    const uint32_t own = rank ? row[1] : row[0];
-#pragma unroll 8
-                    for (int it = 0; it < TM_OWN; ++it) {
-                        const uint32_t r = __shfl_sync(0xffffffffu, own, it);
-                        tc::cp_async16_zfill(at + (lane >> 3) * KCHUNK + tc::sw128_chunk(it, lane & 7),
-                                             A.pool + (r != NONE ? (size_t)r * TM_W + lane * 16 : 0), r != NONE ? 16u : 0u);
-                    }
+            if (ok && t < w.t1) {
+                // A lane resolves two tokens of a tile, 32 apart: entry -> page -> pool row -> scale, each level asked for one of the warp's
+                // tiles or more before it is used (the loads come back through queues that the copies have filled).
+                auto entry = [&](int x, int u) -> uint32_t {
+                    const int j = x * TM_TILE + u * 32 + lane;
+                    return x < w.t1 && j < total ? tree_token(A, w.s, w.b, j) : NONE;
+                };
+                auto page = [&](uint32_t tok) -> int { return tok != NONE && (tok >> shift) < (uint32_t)A.max_pages ? table[tok >> shift] : -1; };
+                auto pool_row = [&](uint32_t tok, int pg) -> uint32_t {
+                    return pg >= 0 && pg < A.n_pool_pages ? (uint32_t)pg * (uint32_t)A.page_tokens + (tok & (uint32_t)inside) : NONE;
+                };
+                auto scale = [&](uint32_t r) -> float { return is_k && r != NONE ? A.pscale[r] : 0.0f; };
+                uint32_t row[2], row1[2], tok2[2];     // pool rows of this warp's tile t and its next; entries of the one after
+                float scl[2];
 #pragma unroll
-                    for (int it = 0; it < 4; ++it) {
-                        const int rl = it * 8 + (lane >> 2);
-                        const uint32_t r = __shfl_sync(0xffffffffu, own, rl);
-                        tc::cp_async16_zfill(at + 4 * KCHUNK + sw64_chunk(rl, lane & 3),
-                                             A.pool + (r != NONE ? (size_t)r * TM_W + TM_KVL + (lane & 3) * 16 : 0), r != NONE ? 16u : 0u);
+                for (int u = 0; u < 2; ++u) { row[u] = entry(t, u); row1[u] = entry(t + GW, u); tok2[u] = entry(t + 2 * GW, u); }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) { row[u] = pool_row(row[u], page(row[u])); row1[u] = pool_row(row1[u], page(row1[u])); }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) scl[u] = scale(row[u]);
+                const int c = lane & 15;               // V: two rows an instruction, 16 chunks each
+                const uint8_t* from = A.pool + (is_k ? lane * 16 : (2 * (c >> 3) + rank) * 128 + (c & 7) * 16);
+                const uint32_t to = is_k ? (lane >> 3) * KCHUNK : (c >> 3) * VCHUNK + (lane >> 4) * 128;
+#pragma unroll 1
+                for (; t < w.t1; t += GW) {
+                    float scl1[2];
+                    int pg2[2];
+                    uint32_t tok3[2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) { scl1[u] = scale(row1[u]); pg2[u] = page(tok2[u]); tok3[u] = entry(t + 3 * GW, u); }
+                    stage_free();
+                    if (!ok) break;
+                    uint64_t* full = (is_k ? bars.k_full : bars.v_full) + s;
+                    const uint32_t at = tc::smem_u32(smem) + (is_k ? SM_K + s * KSTAGE : SM_V + s * VSTAGE);
+                    const uint32_t first = is_k && rank ? row[1] : row[0];
+#pragma unroll 4
+                    for (int it = 0; it < 32; ++it) {
+                        const int rl = is_k ? it : 2 * it + (lane >> 4);
+                        const uint32_t r = __shfl_sync(0xffffffffu, is_k || it < 16 ? first : row[1], rl & 31);
+                        tc::cp_async16_zfill(at + to + (is_k ? it * 128 : it * 256) + (((lane ^ rl) & 7) << 4), r != NONE ? from + (size_t)r * TM_W : A.pool, r != NONE ? 16u : 0u);
                     }
-                } else {
-                    const int c = lane & 15;
-                    const uint8_t* from = A.pool + (2 * (c >> 3) + rank) * 128 + (c & 7) * 16;
-#pragma unroll 8
-                    for (int it = 0; it < 32; ++it) {                  // two rows an instruction, 16 chunks each
-                        const int rl = 2 * it + (lane >> 4);
-                        const uint32_t r = __shfl_sync(0xffffffffu, it < 16 ? row[0] : row[1], rl & 31);
-                        tc::cp_async16_zfill(at + (c >> 3) * VCHUNK + tc::sw128_chunk(rl, c & 7), r != NONE ? from + (size_t)r * TM_W : A.pool, r != NONE ? 16u : 0u);
-                    }
-                    if ((t + 1) * TM_TILE > w.s.n) {
+                    if (is_k) {
+#pragma unroll 1
+                        for (int it = 0; it < 4; ++it) {
+                            const int rl = it * 8 + (lane >> 2);
+                            const uint32_t r = __shfl_sync(0xffffffffu, first, rl);
+                            tc::cp_async16_zfill(at + 4 * KCHUNK + sw64_chunk(rl, lane & 3),
+                                                 A.pool + (r != NONE ? (size_t)r * TM_W + TM_KVL + (lane & 3) * 16 : 0), r != NONE ? 16u : 0u);
+                        }
+                    } else if ((t + 1) * TM_TILE > w.s.n) {
                         // rows of the tree: each lane looks through what it copied itself, once it is there
                         tc::cp_async_commit();
                         tc::cp_async_wait<0>();
-#pragma unroll 4
+                        uint8_t* buf = smem + SM_V + s * VSTAGE + (c >> 3) * VCHUNK;
+#pragma unroll 2
                         for (int it = 0; it < 32; ++it) {
                             const int rl = 2 * it + (lane >> 4);
-                            uint4* v = reinterpret_cast<uint4*>(buf + (c >> 3) * VCHUNK + tc::sw128_chunk(rl, c & 7));
+                            uint4* v = reinterpret_cast<uint4*>(buf + tc::sw128_chunk(rl, c & 7));
                             if (t * TM_TILE + rl >= w.s.n) { const uint4 x = *v; *v = make_uint4(no_nan(x.x), no_nan(x.y), no_nan(x.z), no_nan(x.w)); }
                         }
                     }
+                    tc::cp_async_mbar_arrive_noinc(full);
+                    tc::fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(full);
+                    stage_done(scl, row[0] != NONE, row[1] != NONE);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) { row[u] = row1[u]; scl[u] = scl1[u]; row1[u] = pool_row(tok2[u], pg2[u]); tok2[u] = tok3[u]; }
                 }
-                tc::cp_async_mbar_arrive_noinc(full);
-                tc::fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(full);
-                end();
             }
             turn = t - w.t1;
         }
@@ -514,8 +523,6 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
         for (; !failed && walk_segment(A, w); i0 += w.t1 - w.t0, walk_on(A, w)) {
             const int rows_all = w.s.T * A.H, r0 = w.rb * TM_BLOCK + rank * TM_ROWS, valid = max(0, min(TM_ROWS, rows_all - r0));
             const size_t flat = (size_t)w.s.node0 * A.H + r0;      // first row of the CTA in q, out and out_lse
-            const uint64_t mask_a = ra < valid ? A.node_mask[w.s.node0 + (r0 + ra) / A.H] : 0ull;
-            const uint64_t mask_b = rb < valid ? A.node_mask[w.s.node0 + (r0 + rb) / A.H] : 0ull;
             // ---- q -> two e4m3 terms per row: hi = e4m3(q / s), s = absmax / 448, lo = e4m3(q / s - hi) ----
             // A warp of the first two groups takes sixteen rows and half th of their columns. They arrive as whole 128-byte lines (lanes 8 k .. 8 k + 7 on one row),
             // are split there and go through shared memory, 64 columns at a time, to the lanes whose tensor-memory row they are. (A
@@ -665,6 +672,7 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                 }
                 if (__builtin_expect(j0 + TM_TILE > w.s.n || (see.x & see.y) != ~0u || (see.z | see.w), 0)) {
                     // rows of the tree, rows that are not there, scales that are no numbers: what a node does not see scores -inf
+                    const uint64_t mask_a = ra < valid ? A.node_mask[w.s.node0 + (r0 + ra) / A.H] : 0ull, mask_b = rb < valid ? A.node_mask[w.s.node0 + (r0 + rb) / A.H] : 0ull;
                     const uint64_t there = (uint64_t)see.y << 32 | see.x, wild = ((uint64_t)see.w << 32 | see.z) >> tq;
                     const uint64_t va = (tree_visible(mask_a, w.s.T, w.s.n, j0) & there) >> tq, vb = (tree_visible(mask_b, w.s.T, w.s.n, j0) & there) >> tq;
 #pragma unroll
@@ -728,16 +736,12 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap latents, const _
                         if (na != m_a) { l_a *= exp2f(m_a - na); m_a = na; }
                         if (nb != m_b) { l_b *= exp2f(m_b - nb); m_b = nb; }
                     }
-                    // They stand as long as no P' exceeds 2^(5 + 3) by them (one barrier with an OR), and a row that has none sees nothing.
-                    bool grown = i == i0 || __any_sync(0xffffffffu, m_a != was_a || m_b != was_b);
-                    if (!grown) {
-                        const float2 t2 = __half22float2(top);
-                        grown = fmaxf(t2.x, t2.y) > TM_MOST;
-                        if (__builtin_expect(m_a == -INFINITY || m_b == -INFINITY, 0)) {
-#pragma unroll
-                            for (int k = 0; k < 16; ++k) { const float2 y = unpack(x[k]); grown |= ((k & 1) ? m_b : m_a) == -INFINITY && fmaxf(y.x, y.y) > -INFINITY; }
-                        }
-                    }
+                    // They stand as long as no P' exceeds 2^(5 + 3) by them (one barrier with an OR). One that has moved meanwhile brings the
+                    // P' of before down with it; rows that have none yet are looked at.
+                    const float2 t2 = __half22float2(top);
+                    float most = fmaxf(t2.x, t2.y);
+                    if (m_a != was_a || m_b != was_b) most *= fmaxf(exp2f(was_a - m_a), exp2f(was_b - m_b));
+                    const bool grown = most > TM_MOST || was_a == -INFINITY || was_b == -INFINITY;
                     if (__builtin_expect(tc::barrier_any(6 + th, TM_GROUP, grown || !ok), 0)) {
                         // the largest x + log2(scale) of a row is what P' goes by
                         float ta = -INFINITY, tb2 = -INFINITY;
@@ -958,13 +962,14 @@ int rv_tree_mma(const TreeArgs& a, void* scratch, cudaStream_t st) {
     const int pairs = tree_pairs();
     rv_drain_error();
     uint8_t* s = reinterpret_cast<uint8_t*>(scratch);
-    // tensor copies of a page's rows, 16 or 32 of them; smaller pages are gathered row by row
-    const int box = a.page_tokens < 16 ? 0 : (a.page_tokens < TM_OWN ? a.page_tokens : TM_OWN);
-    CUtensorMap latents{}, ropes{};
-    if (box) {
-        const uint64_t rows = (uint64_t)a.n_pool_pages * a.page_tokens;
-        if (int e = rivoli::make_tmap_columns(&latents, a.pool, rows, TM_W, 128, box)) return e;
-        if (int e = rivoli::make_tmap_columns(&ropes, a.pool, rows, TM_W, TM_ROPE, box)) return e;
+    // a tile inside a page is a few tensor copies; smaller pages are gathered row by row
+    const int tma = a.page_tokens >= TM_TILE;
+    CUtensorMap k_map{}, r_map{}, v_map{};
+    if (tma) {
+        const cuuint64_t rows = (cuuint64_t)a.n_pool_pages * a.page_tokens;
+        if (int e = rivoli::make_tmap_bytes(&k_map, a.pool, 3, {128, rows, 4}, {TM_W, 128}, {128, TM_OWN, 4}, true)) return e;
+        if (int e = rivoli::make_tmap_bytes(&r_map, a.pool, 2, {TM_W, rows}, {TM_W}, {TM_ROPE, TM_OWN}, false)) return e;
+        if (int e = rivoli::make_tmap_bytes(&v_map, a.pool, 4, {128, rows, 2, 2}, {TM_W, 256, 128}, {128, TM_TILE, 2, 1}, true)) return e;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(2 * pairs)); cfg.blockDim = dim3(TM_THREADS); cfg.dynamicSmemBytes = (size_t)SM_TOTAL; cfg.stream = st;
@@ -974,7 +979,7 @@ int rv_tree_mma(const TreeArgs& a, void* scratch, cudaStream_t st) {
     at[1].id = cudaLaunchAttributeClusterDimension;
     at[1].val.clusterDim.x = 2; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = 2;
-    (void)cudaLaunchKernelEx(&cfg, tree_mma_kernel, a, latents, ropes, box, reinterpret_cast<int*>(s), s, (int)tc::kMaxPolls);
+    (void)cudaLaunchKernelEx(&cfg, tree_mma_kernel, a, k_map, r_map, v_map, tma, reinterpret_cast<int*>(s), s, (int)tc::kMaxPolls);
     if (int e = rv_launch_status()) return e;
     rv_launch_dependent(tree_join_kernel, dim3(pairs, TM_BLOCK / 8), dim3(256), 0, st, (const uint8_t*)s, a.out, a.out_lse);
     return rv_launch_status();
