@@ -38,7 +38,11 @@ constexpr int NK = 5, NG = 2, GW = 4;                // stages; softmax groups, 
 constexpr int TM_SW = 4 * NG, TM_QKW = TM_SW, TM_PVW = TM_SW + 1, TM_GW0 = TM_SW + 2;
 constexpr int TM_THREADS = (TM_GW0 + GW) * 32, TM_SOFTMAX = TM_SW * 32, TM_GROUP = 128;
 constexpr float TM_POFF = 5.0f, TM_MOST = 256.0f;    // P' = 2^(s - ref + 5) <= 2^8: references lag by 2^3 at most, see attend_mma.cu
-constexpr int TM_MIN_UNITS = 4;                      // tiles a CTA takes at least, while there are few
+constexpr int TM_MIN_TILES = 4;                      // tiles a CTA takes at least, while there are few
+// What a row block costs beside its tiles, in tiles: its queries, its output and the pipeline's ramp take 26,000 cycles, a tile 1,650. It
+// is counted where CTAs take several blocks each (32 trees over 512 to 8,192 rows: 383 us with runs of as many tiles, 280 with runs of
+// equal cost); with fewer blocks than CTAs every run pays it once.
+constexpr int TM_BLOCK_COST = 16;
 
 // tensor memory columns
 constexpr int TMC_S = 0, TMC_Q = 2 * TM_TILE, TMC_O = TMC_Q + TM_KVL / 4;
@@ -116,9 +120,10 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, int y
 // Bytes of a word whose low seven bits are all up (NaN codes), as their top bits.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t v) { return ((v & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-// A walk over a run of (row block, tile) pairs. Units are numbered tile by tile, block by block, sequence by sequence.
+// A walk over a run of (row block, tile) pairs. Units are numbered block by block, sequence by sequence: the block's own cost, then its tiles.
 struct Walk {
     int b, rb, t0, t1;             // sequence, row block, tiles [t0, t1) of the current segment
+    int cost;                      // of a block beside its tiles
     long long left;                // units of the run from t0 on
     int nt, nrb;                   // tiles and row blocks of the sequence
     TreeSeq s;
@@ -138,7 +143,7 @@ __device__ __forceinline__ bool walk_segment(const TreeArgs& A, Walk& w) {
     return true;
 }
 __device__ __forceinline__ void walk_on(const TreeArgs& A, Walk& w) {
-    w.left -= w.t1 - w.t0;
+    w.left -= w.t1 - w.t0 + w.cost;
     w.t0 = 0;
     if (++w.rb == w.nrb) { w.rb = 0; w.nrb = 0; }
 }
@@ -157,8 +162,8 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
     float* s_mref = reinterpret_cast<float*>(smem + SM_MREF);
     uint32_t* tmem_base_s = reinterpret_cast<uint32_t*>(smem + SM_MISC);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + SM_MISC + 4);
-    int* s_run = reinterpret_cast<int*>(smem + SM_MISC + 8);               // b, rb, t0 of the run's beginning, number of runs
-    long long* s_units = reinterpret_cast<long long*>(smem + SM_MISC + 24);   // its units, all units
+    int* s_run = reinterpret_cast<int*>(smem + SM_MISC + 8);               // b, rb, t0 of the run's beginning, number of runs, a block's own cost
+    long long* s_units = reinterpret_cast<long long*>(smem + SM_MISC + 32);   // its units, all units
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
@@ -185,36 +190,41 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
 
     // ------------------------------ the CTA's run ------------------------------------------------
     if (warp == 0) {
-        auto scan = [&](int b, long long& inc) {   // units of sequence b, and of all of its 32 up to it
-            int nt = 0, nrb = 0;
-            if (b < A.B) { const TreeSeq s = tree_seq(A, b); units_of(A, s, nt, nrb); }
-            const long long mine = (long long)nt * nrb;
-            inc = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) { const long long v = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += v; }
-            return mine;
+        int nt = 0, nrb = 0;                       // of sequence b0 + lane
+        auto sizes = [&](int b) {
+            nt = nrb = 0;
+            if (b < A.B) units_of(A, tree_seq(A, b), nt, nrb);
         };
-        long long total = 0, inc = 0, mine = 0;
-        for (int b0 = 0; b0 < A.B; b0 += 32) { mine = scan(b0 + lane, inc); total += __shfl_sync(0xffffffffu, inc, 31); }
-        const int n = (int)max(1LL, min((long long)gridDim.x, total / TM_MIN_UNITS)), g = blockIdx.x;
+        long long tiles = 0, blocks = 0;
+        for (int b0 = 0; b0 < A.B; b0 += 32) { sizes(b0 + lane); tiles += (long long)nt * nrb; blocks += nrb; }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) { tiles += __shfl_xor_sync(0xffffffffu, tiles, o); blocks += __shfl_xor_sync(0xffffffffu, blocks, o); }
+        const int cost = blocks > gridDim.x ? TM_BLOCK_COST : 0, g = blockIdx.x;
+        const long long total = tiles + cost * blocks;
+        const int n = (int)max(1LL, min((long long)gridDim.x, tiles / TM_MIN_TILES));
         const long long u0 = g < n ? run_begin(total, g, n) : total, u1 = g < n ? run_begin(total, g + 1, n) : total;
-        if (lane == 0) { s_units[0] = u1 - u0; s_units[1] = total; s_run[0] = A.B; s_run[1] = s_run[2] = 0; s_run[3] = n; }
+        if (lane == 0) { s_units[0] = 0; s_units[1] = total; s_run[0] = A.B; s_run[1] = s_run[2] = 0; s_run[3] = n; s_run[4] = cost; }
         __syncwarp();
         long long before = 0;
         for (int b0 = 0; b0 < A.B && u1 > u0; b0 += 32) {
-            if (A.B > 32) mine = scan(b0 + lane, inc);     // (a batch of 32 is scanned already)
-            if (u0 >= before + inc - mine && u0 < before + inc) {
-                int nt, nrb;
-                units_of(A, tree_seq(A, b0 + lane), nt, nrb);
-                const long long in = u0 - (before + inc - mine);
-                s_run[0] = b0 + lane; s_run[1] = (int)(in / nt); s_run[2] = (int)(in % nt);
+            if (A.B > 32) sizes(b0 + lane);        // (a batch of 32 is read already)
+            const long long mine = (long long)(nt + cost) * nrb;
+            long long inc = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const long long v = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += v; }
+            const long long from = before + inc - mine;
+            if (u0 >= from && u0 < from + mine) {
+                // a run that begins in a block's own cost has that block's first tile, if it reaches it
+                const int rb = (int)((u0 - from) / (nt + cost)), in = (int)((u0 - from) % (nt + cost));
+                s_run[0] = b0 + lane; s_run[1] = rb; s_run[2] = max(0, in - cost);
+                s_units[0] = u1 - u0 - max(0, cost - in);
             }
             before += __shfl_sync(0xffffffffu, inc, 31);
         }
     }
     __syncthreads();
     Walk w;
-    w.b = s_run[0]; w.rb = s_run[1]; w.t0 = s_run[2]; w.left = w.b < A.B ? s_units[0] : 0;
+    w.b = s_run[0]; w.rb = s_run[1]; w.t0 = s_run[2]; w.cost = s_run[4]; w.left = w.b < A.B ? s_units[0] : 0;
     w.nt = w.nrb = 0;
     if (w.left > 0) { w.s = tree_seq(A, w.b); units_of(A, w.s, w.nt, w.nrb); }
 
@@ -463,7 +473,7 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
         // in the barrier it has seen, and then for another's within the NG behind it.
         auto pv_done = [&](int i) { return wait_for(&bars.pv_done[i % NG], (i / NG) & 1, abort_flag, 63, max_polls); };
         int i0 = 0;                                        // tiles of the CTA before this segment
-        bool failed = false;
+        bool failed = false, told = false;
         for (; !failed && walk_segment(A, w); i0 += w.t1 - w.t0, walk_on(A, w)) {
             const int rows_all = w.s.T * A.H, r0 = w.rb * TM_ROWS, valid = min(TM_ROWS, rows_all - r0);
             const size_t flat = (size_t)w.s.node0 * A.H + r0;      // first row of the block in q, out and out_lse
@@ -827,14 +837,14 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
                     while (run_begin(total, last + 1, s_run[3]) <= end) ++last;
                     Head h{(int32_t)flat, valid, last - (int)blockIdx.x + 1, 0};
                     reinterpret_cast<Head*>(scratch + SC_HEAD)[blockIdx.x] = h;
-                    w.left = -1;                           // (told; the walk ends here in any case)
+                    told = true;
                 }
             }
             tc::tc_fence_before();
         }
         if (sq == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         // no block begins in this run and ends in another: nothing for the joining kernel
-        if (tid == 0 && w.left >= 0) {
+        if (tid == 0 && !told) {
             Head h{0, 0, 0, 0};
             reinterpret_cast<Head*>(scratch + SC_HEAD)[blockIdx.x] = h;
         }

@@ -146,14 +146,14 @@ def run_tree(be, cache, H, prefix, trees, masks, rows=None, n_rows=None, tree_po
     tree_pos = prefix if tree_pos is None else tree_pos
     out = torch.full((N + 1, H, kvl), 7.0, dtype=BF, device=DEV)
     lse = torch.full((N + 1, H), 7.0, device=DEV)
-    sc = torch.zeros(be.mla_tree_attend_scratch_bytes(g, B, N), dtype=torch.uint8, device=DEV) if scratch else None
+    sc = scratch if torch.is_tensor(scratch) else torch.zeros(be.mla_tree_attend_scratch_bytes(g, B, N), dtype=torch.uint8, device=DEV) if scratch else None
     r = None if rows is None else i32([[v - (1 << 32) if v >> 31 else v for v in row] for row in rows])
     counts = None if n_rows is None else i32(n_rows)
     args = [g, q.to(DEV), codes, scale, table, r, 0 if r is None else r.shape[1], counts, i32(tree_pos), i32(start), signed(masks), B, N, out, lse, sc, stream]
     torch.cuda.synchronize()
     be.launch_mla_tree_attend_paged_bf16(*args)
     torch.cuda.synchronize()
-    if scratch:
+    if sc is not None:
         be.mla_tree_attend_status(g, sc)
     assert (out[N] == 7).all() and (lse[N] == 7).all()
     got, got_lse = out[:N].double().cpu().numpy(), lse[:N].double().cpu().numpy()
@@ -300,6 +300,18 @@ def test_long_cache(be):
     trees, prefix = [2, 5, 1], [20011, 40, 1500]
     masks = [m for t in trees for m in masks_of(host, t, "tree")]
     run_tree(be, Cache(16, [p + t for p, t in zip(prefix, trees)], 64), 64, prefix, trees, masks)
+
+
+def test_one_scratch_for_calls_of_every_shape(be):
+    """What one call leaves in the scratch is nothing to the next: long after short, one block after many, and back."""
+    host = random.Random(22)
+    shared = torch.zeros(64 << 20, dtype=torch.uint8, device=DEV)
+    g = be.DsaGeom.make(max_pages_per_seq=4, n_pool_pages=8)
+    assert be.mla_tree_attend_scratch_bytes(g, 1, 1) <= shared.numel()
+    for trees, prefix, H in (([2], [9000], 64), ([1] * 200, [70 + i for i in range(200)], 64), ([3, 1], [10, 300], 16), ([64] * 5, [600] * 5, 64),
+                             ([1], [5], 64), ([33], [5000], 64), ([2] * 40, [1000 - 20 * i for i in range(40)], 64)):
+        masks = [m for t in trees for m in masks_of(host, t, "tree")]
+        run_tree(be, Cache(len(trees), [p + t for p, t in zip(prefix, trees)], 64), H, prefix, trees, masks, scratch=shared)
 
 
 def test_many_sequences(be):
