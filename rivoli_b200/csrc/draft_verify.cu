@@ -10,18 +10,21 @@
 // from; -1 if that is empty too.
 //
 // Every r in that chain is max(a p - b q, 0) with two numbers a and b: a rejection needs one pass over the rows (for Z), which also
-// leaves the sums by chunk that the draw needs, and nothing is written but the answer. Sums, products and comparisons are in 64 bits:
-// a draw next to a border has to come out the same whatever the order of summation.
+// leaves the sums by chunk that the draw needs, and nothing is written but the answer. Of tokens that were chosen, one pass a node serves all
+// rejections: Z goes down by the token's own probability, and before the draw the few chunks that hold such tokens are summed again
+// without them (as they are when Z has come below a thousandth of the whole and would lose its last bits). Sums, products and
+// comparisons are in 64 bits: a draw next to a border has to come out the same whatever the order of summation.
 //
-// A cluster of blocks per sequence, each a contiguous part of the vocabulary; every block walks the tree itself (the few
-// probabilities that decide are gathered at once for all nodes), and only sums are exchanged, through distributed shared memory. Bound by memory: one
-// row of the target and one of the draft per sequence, a chunk of 2 KiB of each per warp and step.
+// A cluster of up to eight blocks per sequence, each a contiguous part of the vocabulary; every block walks the tree itself (the few
+// probabilities that decide are gathered at once for all nodes), and only sums are exchanged, through distributed shared memory. Bound by
+// memory where the batch is large: one row of the target and one of the draft per pass, a chunk of 2 KiB of each per warp and step; for few
+// sequences by the chain launch, node words, probabilities, pass, exchange, chunk, place.
 #include "codec.cuh"
 #include "common.cuh"
 
 namespace {
 
-constexpr int DV_THREADS = 512, DV_WARPS = DV_THREADS / 32;
+constexpr int DV_THREADS = 256, DV_WARPS = DV_THREADS / 32;
 constexpr int DV_NODES = 64, DV_MAX_VOCAB = 1 << 20, DV_MAX_CLUSTER = 8;
 
 struct VerifyArgs {
@@ -54,6 +57,12 @@ __device__ __forceinline__ double warp_sum(double v) {
 template <class T> struct Row;           // 16 bytes of probabilities
 template <> struct Row<float> {
     static constexpr int PER = 4;
+    __device__ static uint4 some(const float* p, int v, int end) {             // values from v on, zeros from `end` on
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = v + i < end ? __float_as_uint(p[v + i]) : 0u;
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
     __device__ static float one(const float* p, long long i) { return clean(p[i]); }
     __device__ static void unpack(const uint4 w, float* x) {
         x[0] = clean(__uint_as_float(w.x)); x[1] = clean(__uint_as_float(w.y)); x[2] = clean(__uint_as_float(w.z)); x[3] = clean(__uint_as_float(w.w));
@@ -61,6 +70,12 @@ template <> struct Row<float> {
 };
 template <> struct Row<uint16_t> {
     static constexpr int PER = 8;
+    __device__ static uint4 some(const uint16_t* p, int v, int end) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (v + 2 * i < end ? (uint32_t)p[v + 2 * i] : 0u) | (v + 2 * i + 1 < end ? (uint32_t)p[v + 2 * i + 1] << 16 : 0u);
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
     __device__ static float one(const uint16_t* p, long long i) { return clean(rv_bf16_to_f32(p[i])); }
     __device__ static void unpack(const uint4 w, float* x) {
         const uint32_t v[4] = {w.x, w.y, w.z, w.w};
@@ -72,11 +87,11 @@ constexpr int DV_STEPS = 4;              // 16-byte loads of a lane per chunk an
 template <class T> __host__ __device__ constexpr int chunk_of() { return 32 * DV_STEPS * Row<T>::PER; }
 
 template <class T, bool DRAFT, bool VEC>
-__global__ void __launch_bounds__(DV_THREADS)
+__global__ void __launch_bounds__(DV_THREADS, 4)
 draft_verify_kernel(VerifyArgs A) {
     constexpr int PER = Row<T>::PER, CHUNK = chunk_of<T>();
     extern __shared__ double sums[];                           // [chunks] of this block's part, from the last pass
-    __shared__ int s_parent[DV_NODES], s_token[DV_NODES];
+    __shared__ int s_token[DV_NODES];
     __shared__ float s_u[DV_NODES], s_p[DV_NODES], s_q[DV_NODES];
     __shared__ unsigned long long s_kids[DV_NODES];
     __shared__ int s_out[DV_NODES];                            // tokens left out of r (given drafts)
@@ -109,52 +124,52 @@ draft_verify_kernel(VerifyArgs A) {
     const int lo = (int)rank * A.chunks * CHUNK, hi = min(A.vocab, lo + A.chunks * CHUNK);   // (at most 2^20 + 8 chunks)
     const int n_chunks = hi > lo ? (hi - lo + CHUNK - 1) / CHUNK : 0;
     int parity = 0;
-    // r at an index of the current node's rows
+    // r at an index of the current node's rows, up to a factor
     auto value = [&](double a, double bq, float p, float q) -> double { return DRAFT ? fmax(a * (double)p - bq * (double)q, 0.0) : (double)p; };
     auto left_out = [&](int v, int n_out) -> bool {
         bool hit = false;
         for (int i = 0; i < n_out; ++i) hit |= s_out[i] == v;
         return hit;
     };
-    // one pass over the rows of node `cur`: chunk sums of r, and its sum over the vocabulary (the same in every thread)
-    auto pass = [&](int cur, double a, double bq, int n_out) -> double {
-        const T* p = target + (long long)(start + cur) * A.target_stride;
-        const T* q = DRAFT ? draft + (long long)(start + cur) * A.draft_stride : nullptr;
-        const bool with_q = DRAFT && bq != 0.0;
-        for (int c = warp; c < n_chunks; c += DV_WARPS) {
-            const int at = lo + c * CHUNK;
-            double s = 0.0;
-            if (VEC && at + CHUNK <= hi) {
-                uint4 wp[DV_STEPS], wq[DV_STEPS];
+    // sum of r over chunk c of the rows of node `cur`, without the tokens that are left out (all lanes)
+    auto chunk_sum = [&](const T* p, const T* q, int c, double a, double bq, int n_out) -> double {
+        const int at = lo + c * CHUNK;
+        double s = 0.0;
+        if (VEC && at + CHUNK <= hi) {
+            uint4 wp[DV_STEPS], wq[DV_STEPS];
 #pragma unroll
-                for (int i = 0; i < DV_STEPS; ++i) wp[i] = __ldg(reinterpret_cast<const uint4*>(p + at) + i * 32 + lane);
-                if (with_q)
+            for (int i = 0; i < DV_STEPS; ++i) wp[i] = __ldg(reinterpret_cast<const uint4*>(p + at) + i * 32 + lane);
+            if (DRAFT) {
 #pragma unroll
-                    for (int i = 0; i < DV_STEPS; ++i) wq[i] = __ldg(reinterpret_cast<const uint4*>(q + at) + i * 32 + lane);
-                else
-#pragma unroll
-                    for (int i = 0; i < DV_STEPS; ++i) wq[i] = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-                for (int i = 0; i < DV_STEPS; ++i) {
-                    float xp[PER], xq[PER];
-                    Row<T>::unpack(wp[i], xp);
-                    if (DRAFT) Row<T>::unpack(wq[i], xq);
-                    if (!DRAFT && n_out > 0)
-                        for (int k = 0; k < n_out; ++k) {
-                            const int d = s_out[k] - (at + (i * 32 + lane) * PER);
-#pragma unroll
-                            for (int e = 0; e < PER; ++e) xp[e] = d == e ? 0.0f : xp[e];
-                        }
-#pragma unroll
-                    for (int e = 0; e < PER; ++e) s += value(a, bq, xp[e], DRAFT ? xq[e] : 0.0f);
-                }
-            } else {
-                for (int v = at + lane; v < min(at + CHUNK, hi); v += 32)
-                    if (DRAFT || !left_out(v, n_out)) s += value(a, bq, Row<T>::one(p, v), with_q ? Row<T>::one(q, v) : 0.0f);
+                for (int i = 0; i < DV_STEPS; ++i) wq[i] = q ? __ldg(reinterpret_cast<const uint4*>(q + at) + i * 32 + lane) : make_uint4(0u, 0u, 0u, 0u);
             }
-            s = warp_sum(s);
-            if (lane == 0) sums[c] = s;
+            double s2 = 0.0;
+#pragma unroll
+            for (int i = 0; i < DV_STEPS; ++i) {
+                float xp[PER], xq[PER];
+                Row<T>::unpack(wp[i], xp);
+                if (DRAFT) Row<T>::unpack(wq[i], xq);
+                if (!DRAFT)
+                    for (int k = 0; k < n_out; ++k) {
+                        const int d = s_out[k] - (at + (i * 32 + lane) * PER);
+#pragma unroll
+                        for (int e = 0; e < PER; ++e) xp[e] = d == e ? 0.0f : xp[e];
+                    }
+#pragma unroll
+                for (int e = 0; e < PER; e += 2) {
+                    s += value(a, bq, xp[e], DRAFT ? xq[e] : 0.0f);
+                    s2 += value(a, bq, xp[e + 1], DRAFT ? xq[e + 1] : 0.0f);
+                }
+            }
+            s += s2;
+        } else {
+            for (int v = at + lane; v < min(at + CHUNK, hi); v += 32)
+                if (DRAFT || !left_out(v, n_out)) s += value(a, bq, Row<T>::one(p, v), DRAFT && q ? Row<T>::one(q, v) : 0.0f);
         }
+        return warp_sum(s);
+    };
+    // the chunk sums' sum over the vocabulary, the same in every thread of the cluster
+    auto all_sums = [&]() -> double {
         __syncthreads();
         if (warp == 0) {
             double s = 0.0;
@@ -165,46 +180,77 @@ draft_verify_kernel(VerifyArgs A) {
         cluster_sync();
         double z = 0.0;
         for (uint32_t i = 0; i < n_rank; ++i) z += s_part[parity][i];
-        parity ^= 1;                     // (the next pass writes the other set: a block may still be reading this one)
+        parity ^= 1;                     // (the next sum goes to the other set: a block may still be reading this one)
         return z;
+    };
+    // one pass over the rows of node `cur`
+    auto pass = [&](int cur, double a, double bq) -> double {
+        const T* p = target + (long long)(start + cur) * A.target_stride;
+        const T* q = DRAFT && bq != 0.0 ? draft + (long long)(start + cur) * A.draft_stride : nullptr;
+        for (int c = warp; c < n_chunks; c += DV_WARPS) {
+            const double s = chunk_sum(p, q, c, a, bq, 0);
+            if (lane == 0) sums[c] = s;
+        }
+        return all_sums();
+    };
+    // the sums of the chunks that hold a token that is left out, again and without it (two tokens of a chunk: twice the same)
+    auto without = [&](int cur, int n_out) -> double {
+        const T* p = target + (long long)(start + cur) * A.target_stride;
+        for (int k = warp; k < n_out; k += DV_WARPS) {
+            const int v = s_out[k];
+            if (v < lo || v >= hi) continue;
+            const int c = (v - lo) / CHUNK;
+            const double s = chunk_sum(p, nullptr, c, 1.0, 0.0, n_out);
+            if (lane == 0) sums[c] = s;
+        }
+        return all_sums();
     };
 
     int cur = 0, n = 1, n_out = 0;
     double a = 1.0, bq = 0.0, total = 0.0;
     double da = 1.0, db = 0.0;           // the two numbers of the last pass: the chunk sums' scale, and the draw's
-    bool have = false, dead = false;     // have: the chunk sums are those of r; dead: nothing is left of r
+    double whole = 0.0;                  // (chosen tokens) the sum of the node's row
+    bool have = false, dead = false;     // have: the chunk sums are those of the node; dead: nothing is left of r
+    bool apart = false;                  // (chosen tokens) the chunk sums are without the tokens left out
     unsigned long long kids = s_kids[0];
     if (rank == 0 && tid == 0) path[0] = 0;
     while (kids && n < A.max_path) {
         const int j = __ffsll((long long)kids) - 1;
         kids &= kids - 1;
         const double p = s_p[j], q = s_q[j];
-        double r;
-        if (DRAFT) r = fmax(a * p - bq * q, 0.0);
-        else r = left_out(s_token[j], n_out) ? 0.0 : a * p;
+        const bool out = !DRAFT && left_out(s_token[j], n_out);
+        const double r = DRAFT ? fmax(a * p - bq * q, 0.0) : out ? 0.0 : a * p;
         if (!dead && (double)s_u[j] * q < r) {
             if (rank == 0 && tid == 0) path[n] = j;
             cur = j; ++n; kids = s_kids[j];
-            a = 1.0; bq = 0.0; n_out = 0; have = dead = false;
+            a = 1.0; bq = 0.0; n_out = 0; have = dead = apart = false;
             continue;
         }
         if (dead) continue;
-        if (DRAFT) bq += 1.0;
-        else {
+        if (DRAFT) {
+            bq += 1.0;
+            da = a; db = bq;
+            total = pass(cur, da, db);
+            have = true;
+            if (total > 0.0) { a /= total; bq /= total; }      // r / Z (the draw needs no division)
+            else { dead = true; have = false; }
+            continue;
+        }
+        if (!have) { whole = total = pass(cur, 1.0, 0.0); have = true; }
+        if (!out && s_token[j] >= 0) {
             __syncthreads();             // (everyone has looked at the list)
             if (tid == 0) s_out[n_out] = s_token[j];
             ++n_out;
             __syncthreads();
+            total -= p;
+            apart = false;
+            if (total < whole * 0.0009765625) { total = without(cur, n_out); apart = true; }
         }
-        da = a; db = bq;
-        total = pass(cur, da, db, n_out);
-        have = true;
-        if (!(total > 0.0)) { dead = true; have = false; continue; }
-        // r / Z (the draw needs no division)
-        if (DRAFT) { a /= total; bq /= total; }
-        else a = 1.0 / total;
+        if (total > 0.0) a = 1.0 / total;
+        else { dead = true; have = false; }
     }
-    if (!have) { da = 1.0; db = 0.0; n_out = 0; total = pass(cur, da, db, 0); }
+    if (!have) { da = 1.0; db = 0.0; n_out = 0; total = pass(cur, da, db); }
+    else if (!DRAFT && n_out && !apart) total = without(cur, n_out);
     if (rank == 0 && tid == 0) A.n_path[b] = n;
 
     // The block whose part holds the draw finds the chunk and the place in it, with one warp.
@@ -222,9 +268,8 @@ draft_verify_kernel(VerifyArgs A) {
     if (none) { owner = last; before = 0.0; }
     if (last < 0) { if (rank == 0 && tid == 0) A.next[b] = -1; }
     else if (owner == (int)rank && warp == 0) {
-        // chunk: lanes take runs of chunks in order
-        const int each = (n_chunks + 31) >> 5;
-        auto find = [&](double mine, double from, bool& hit, double& base) -> int {   // the first lane whose running sum passes `want`
+        // the first lane whose running sum passes `want`, or the last that has any: its index, and what came before it
+        auto find = [&](double mine, double from, bool& hit, double& base) -> int {
             double inc = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) { const double t = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += t; }
@@ -236,6 +281,8 @@ draft_verify_kernel(VerifyArgs A) {
             base = __shfl_sync(0xffffffffu, exc, who);
             return who;
         };
+        // chunk: lanes take runs of chunks in order
+        const int each = (n_chunks + 31) >> 5;
         double mine = 0.0;
         for (int i = 0; i < each; ++i) { const int c = lane * each + i; if (c < n_chunks) mine += sums[c]; }
         bool hit;
@@ -253,30 +300,70 @@ draft_verify_kernel(VerifyArgs A) {
             }
             run2 += s;
         }
-        // place: lanes take runs of the chunk's values in order
+        // place: the chunk's runs of 32 x PER values, all asked for at once, then the run's lanes, then a lane's values
         const T* p = target + (long long)(start + cur) * A.target_stride;
-        const T* q = DRAFT ? draft + (long long)(start + cur) * A.draft_stride : nullptr;
-        const int at = lo + chunk * CHUNK, end = min(at + CHUNK, hi), run_len = CHUNK / 32;
-        auto at_value = [&](int v) -> double {
-            if (!DRAFT && left_out(v, n_out)) return 0.0;
-            return value(da, db, Row<T>::one(p, v), DRAFT && db != 0.0 ? Row<T>::one(q, v) : 0.0f);
-        };
-        mine = 0.0;
-        for (int i = 0; i < run_len; ++i) { const int v = at + lane * run_len + i; if (v < end) mine += at_value(v); }
-        const int who2 = find(mine, base, hit, run2);
-        if (lane == who2) {
-            int found = -1;
-            for (int i = 0; i < run_len; ++i) {
-                const int v = at + lane * run_len + i;
-                if (v >= end) break;
-                const double x = at_value(v);
-                if (x > 0.0) {
-                    found = v;
-                    if (hit && run2 + x > want) break;
-                }
-                run2 += x;
+        const T* q = DRAFT && db != 0.0 ? draft + (long long)(start + cur) * A.draft_stride : nullptr;
+        const int at = lo + chunk * CHUNK, end = min(at + CHUNK, hi);
+        uint4 wp[DV_STEPS], wq[DV_STEPS];
+#pragma unroll
+        for (int i = 0; i < DV_STEPS; ++i) {
+            const int v = at + (i * 32 + lane) * PER;
+            wp[i] = wq[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (VEC && v + PER <= end) {
+                wp[i] = __ldg(reinterpret_cast<const uint4*>(p + v));
+                if (DRAFT && q) wq[i] = __ldg(reinterpret_cast<const uint4*>(q + v));
+            } else {
+                wp[i] = Row<T>::some(p, v, end);
+                if (DRAFT && q) wq[i] = Row<T>::some(q, v, end);
             }
-            A.next[b] = found;
+        }
+        double x[PER];
+        auto values = [&](const uint4 a4, const uint4 b4, int v) -> double {
+            float xp[PER], xq[PER];
+            Row<T>::unpack(a4, xp);
+            Row<T>::unpack(b4, xq);
+            if (!DRAFT)
+                for (int k = 0; k < n_out; ++k) {
+                    const int d = s_out[k] - v;
+#pragma unroll
+                    for (int e = 0; e < PER; ++e) xp[e] = d == e ? 0.0f : xp[e];
+                }
+            double sum = 0.0;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) { x[e] = value(da, db, xp[e], xq[e]); sum += x[e]; }
+            return sum;
+        };
+        int pick = -1;                   // the run whose sum passes `want`, or the last that has any
+        double start_of = base;
+#pragma unroll
+        for (int i = 0; i < DV_STEPS; ++i) {
+            const double s = warp_sum(values(wp[i], wq[i], at + (i * 32 + lane) * PER));
+            const bool passed = pick >= 0 && hit && !none && start_of > want;   // (a run before has it)
+            if (s > 0.0 && !passed) { pick = i; base = run2 = start_of; }
+            if (!passed) start_of += s;
+            if (s > 0.0 && hit && start_of > want) start_of = INFINITY;         // found: nothing behind it is looked at
+        }
+        if (pick >= 0) {
+            uint4 a4 = wp[0], b4 = wq[0];
+#pragma unroll
+            for (int i = 1; i < DV_STEPS; ++i)
+                if (pick == i) { a4 = wp[i]; b4 = wq[i]; }
+            const int v = at + (pick * 32 + lane) * PER;
+            const double mine2 = values(a4, b4, v);
+            const int who2 = find(mine2, base, hit, run2);
+            if (lane == who2) {
+                int found = -1;
+                bool done = false;
+#pragma unroll
+                for (int e = 0; e < PER; ++e) {
+                    if (x[e] > 0.0 && !done) {
+                        found = v + e;
+                        done = hit && run2 + x[e] > want;
+                    }
+                    run2 += x[e];
+                }
+                A.next[b] = found;
+            }
         }
     }
     cluster_sync();                      // no block leaves while another may still write into it
@@ -299,10 +386,10 @@ int launch(const VerifyArgs& a, int n, int B, cudaStream_t st) {
 }
 template <class T>
 int dispatch(VerifyArgs& a, int B, cudaStream_t st) {
-    // blocks a sequence: until there are two to an SM, a part being at least two chunks a warp
+    // blocks a sequence: until there are two to an SM, while a part has four chunks
     const int sms = rv_sm_count(), all = (a.vocab + chunk_of<T>() - 1) / chunk_of<T>();
     int n = 1;
-    while (n < DV_MAX_CLUSTER && (long long)B * n < 2 * sms && all / (2 * n) >= 2 * DV_WARPS) n *= 2;
+    while (n < DV_MAX_CLUSTER && (long long)B * n < 2 * sms && all / (2 * n) >= 4) n *= 2;
     a.chunks = (all + n - 1) / n;
     const bool vec = (((uintptr_t)a.target | (uintptr_t)a.draft) & 15) == 0 && a.target_stride * (long long)sizeof(T) % 16 == 0 &&
                      (!a.draft || a.draft_stride * (long long)sizeof(T) % 16 == 0);
