@@ -21,6 +21,7 @@
 // sequences by the chain launch, node words, probabilities, pass, exchange, chunk, place.
 #include "codec.cuh"
 #include "common.cuh"
+#include "tc_common.cuh"
 
 namespace {
 
@@ -48,6 +49,11 @@ __device__ __forceinline__ void put_remote(double* mine, uint32_t rank, double v
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
     asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(v) : "memory");
 }
+__device__ __forceinline__ uint4 load16(uint32_t at) {
+    uint4 w;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at) : "memory");
+    return w;
+}
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -65,7 +71,14 @@ template <> struct Row<float> {
     }
     __device__ static float one(const float* p, long long i) { return clean(p[i]); }
     __device__ static void unpack(const uint4 w, float* x) {
-        x[0] = clean(__uint_as_float(w.x)); x[1] = clean(__uint_as_float(w.y)); x[2] = clean(__uint_as_float(w.z)); x[3] = clean(__uint_as_float(w.w));
+        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+        uint32_t bad = 0u;               // a sign, or an exponent of ones that reaches the sign with one more
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { x[i] = __uint_as_float(v[i]); bad |= v[i] | (v[i] + 0x00800000u); }
+        if (__builtin_expect((bad & 0x80000000u) != 0u, 0)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = clean(x[i]);
+        }
     }
 };
 template <> struct Row<uint16_t> {
@@ -79,18 +92,31 @@ template <> struct Row<uint16_t> {
     __device__ static float one(const uint16_t* p, long long i) { return clean(rv_bf16_to_f32(p[i])); }
     __device__ static void unpack(const uint4 w, float* x) {
         const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+        uint32_t bad = 0u;               // (a half that carries into its neighbour had the sign itself)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { x[2 * i] = clean(__uint_as_float(v[i] << 16)); x[2 * i + 1] = clean(__uint_as_float(v[i] & 0xffff0000u)); }
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(v[i] << 16); x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+            bad |= v[i] | (v[i] + 0x00800080u);
+        }
+        if (__builtin_expect((bad & 0x80008000u) != 0u, 0)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = clean(x[i]);
+        }
     }
 };
 constexpr int DV_STEPS = 4;              // 16-byte loads of a lane per chunk and row
+// with the draft's rows: three blocks an SM and one chunk ahead; without: four and two
+__host__ __device__ constexpr int per_sm(bool draft) { return draft ? 3 : 4; }
+__host__ __device__ constexpr int ring_of(bool draft) { return draft ? 2 : 3; }
+constexpr int ring_bytes(bool draft) { return DV_WARPS * ring_of(draft) * (draft ? 2 : 1) * DV_STEPS * 512; }
+__host__ __device__ constexpr int ring_at(int chunks) { return (chunks + 1) & ~1; }   // (behind the sums, 16-byte aligned)
 template <class T> __host__ __device__ constexpr int chunk_of() { return 32 * DV_STEPS * Row<T>::PER; }
 
 template <class T, bool DRAFT, bool VEC>
-__global__ void __launch_bounds__(DV_THREADS, 4)
+__global__ void __launch_bounds__(DV_THREADS, per_sm(DRAFT))
 draft_verify_kernel(VerifyArgs A) {
-    constexpr int PER = Row<T>::PER, CHUNK = chunk_of<T>();
-    extern __shared__ double sums[];                           // [chunks] of this block's part, from the last pass
+    constexpr int PER = Row<T>::PER, CHUNK = chunk_of<T>(), RING = ring_of(DRAFT), ROWS = DRAFT ? 2 : 1;
+    extern __shared__ __align__(16) double sums[];             // [chunks] of this block's part, from the last pass; the ring
     __shared__ int s_token[DV_NODES];
     __shared__ float s_u[DV_NODES], s_p[DV_NODES], s_q[DV_NODES];
     __shared__ unsigned long long s_kids[DV_NODES];
@@ -131,6 +157,28 @@ draft_verify_kernel(VerifyArgs A) {
         for (int i = 0; i < n_out; ++i) hit |= s_out[i] == v;
         return hit;
     };
+    // a lane's share of the sum of r over a full chunk
+    auto share = [&](const uint4 (&wp)[DV_STEPS], const uint4 (&wq)[DV_STEPS], int at, double a, double bq, int n_out) -> double {
+        double s = 0.0, s2 = 0.0;
+#pragma unroll
+        for (int i = 0; i < DV_STEPS; ++i) {
+            float xp[PER], xq[PER];
+            Row<T>::unpack(wp[i], xp);
+            if (DRAFT) Row<T>::unpack(wq[i], xq);
+            if (!DRAFT)
+                for (int k = 0; k < n_out; ++k) {
+                    const int d = s_out[k] - (at + (i * 32 + lane) * PER);
+#pragma unroll
+                    for (int e = 0; e < PER; ++e) xp[e] = d == e ? 0.0f : xp[e];
+                }
+#pragma unroll
+            for (int e = 0; e < PER; e += 2) {
+                s += value(a, bq, xp[e], DRAFT ? xq[e] : 0.0f);
+                s2 += value(a, bq, xp[e + 1], DRAFT ? xq[e + 1] : 0.0f);
+            }
+        }
+        return s + s2;
+    };
     // sum of r over chunk c of the rows of node `cur`, without the tokens that are left out (all lanes)
     auto chunk_sum = [&](const T* p, const T* q, int c, double a, double bq, int n_out) -> double {
         const int at = lo + c * CHUNK;
@@ -143,25 +191,7 @@ draft_verify_kernel(VerifyArgs A) {
 #pragma unroll
                 for (int i = 0; i < DV_STEPS; ++i) wq[i] = q ? __ldg(reinterpret_cast<const uint4*>(q + at) + i * 32 + lane) : make_uint4(0u, 0u, 0u, 0u);
             }
-            double s2 = 0.0;
-#pragma unroll
-            for (int i = 0; i < DV_STEPS; ++i) {
-                float xp[PER], xq[PER];
-                Row<T>::unpack(wp[i], xp);
-                if (DRAFT) Row<T>::unpack(wq[i], xq);
-                if (!DRAFT)
-                    for (int k = 0; k < n_out; ++k) {
-                        const int d = s_out[k] - (at + (i * 32 + lane) * PER);
-#pragma unroll
-                        for (int e = 0; e < PER; ++e) xp[e] = d == e ? 0.0f : xp[e];
-                    }
-#pragma unroll
-                for (int e = 0; e < PER; e += 2) {
-                    s += value(a, bq, xp[e], DRAFT ? xq[e] : 0.0f);
-                    s2 += value(a, bq, xp[e + 1], DRAFT ? xq[e + 1] : 0.0f);
-                }
-            }
-            s += s2;
+            s = share(wp, wq, at, a, bq, n_out);
         } else {
             for (int v = at + lane; v < min(at + CHUNK, hi); v += 32)
                 if (DRAFT || !left_out(v, n_out)) s += value(a, bq, Row<T>::one(p, v), DRAFT && q ? Row<T>::one(q, v) : 0.0f);
@@ -187,7 +217,43 @@ draft_verify_kernel(VerifyArgs A) {
     auto pass = [&](int cur, double a, double bq) -> double {
         const T* p = target + (long long)(start + cur) * A.target_stride;
         const T* q = DRAFT && bq != 0.0 ? draft + (long long)(start + cur) * A.draft_stride : nullptr;
-        for (int c = warp; c < n_chunks; c += DV_WARPS) {
+        const int n_full = VEC && hi > lo ? (hi - lo) / CHUNK : 0;
+        // a warp's chunks come through its own ring, each lane reading what it copied itself
+        const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sums + ring_at(A.chunks)) + (warp * RING * ROWS * DV_STEPS * 32 + lane) * 16;
+        auto fetch = [&](int c, int slot) {
+            if (c < n_full) {
+                const uint32_t to = ring + slot * (ROWS * DV_STEPS * 512);
+                const T* from = p + lo + c * CHUNK + lane * PER;
+#pragma unroll
+                for (int i = 0; i < DV_STEPS; ++i) tc::cp_async16(to + i * 512, from + i * 32 * PER);
+                if (DRAFT && q) {
+                    const T* qf = q + lo + c * CHUNK + lane * PER;
+#pragma unroll
+                    for (int i = 0; i < DV_STEPS; ++i) tc::cp_async16(to + (DV_STEPS + i) * 512, qf + i * 32 * PER);
+                }
+            }
+            tc::cp_async_commit();
+        };
+        int slot = 0;
+#pragma unroll
+        for (int i = 0; i < RING - 1; ++i) fetch(warp + i * DV_WARPS, i);
+#pragma unroll 1
+        for (int c = warp; c < n_full; c += DV_WARPS) {
+            const int over = slot == 0 ? RING - 1 : slot - 1;
+            fetch(c + (RING - 1) * DV_WARPS, over);
+            tc::cp_async_wait<RING - 1>();
+            const uint32_t at = ring + slot * (ROWS * DV_STEPS * 512);
+            uint4 wp[DV_STEPS], wq[DV_STEPS];
+#pragma unroll
+            for (int i = 0; i < DV_STEPS; ++i) {
+                wp[i] = load16(at + i * 512);
+                if (DRAFT) wq[i] = q ? load16(at + (DV_STEPS + i) * 512) : make_uint4(0u, 0u, 0u, 0u);
+            }
+            const double s = warp_sum(share(wp, wq, 0, a, bq, 0));
+            if (lane == 0) sums[c] = s;
+            slot = slot == RING - 1 ? 0 : slot + 1;
+        }
+        for (int c = n_full + warp; c < n_chunks; c += DV_WARPS) {         // (the last one, or all where nothing is aligned)
             const double s = chunk_sum(p, q, c, a, bq, 0);
             if (lane == 0) sums[c] = s;
         }
@@ -333,11 +399,18 @@ draft_verify_kernel(VerifyArgs A) {
             for (int e = 0; e < PER; ++e) { x[e] = value(da, db, xp[e], xq[e]); sum += x[e]; }
             return sum;
         };
+        double s4[DV_STEPS];
+#pragma unroll
+        for (int i = 0; i < DV_STEPS; ++i) s4[i] = values(wp[i], wq[i], at + (i * 32 + lane) * PER);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < DV_STEPS; ++i) s4[i] += __shfl_xor_sync(0xffffffffu, s4[i], o);
         int pick = -1;                   // the run whose sum passes `want`, or the last that has any
         double start_of = base;
 #pragma unroll
         for (int i = 0; i < DV_STEPS; ++i) {
-            const double s = warp_sum(values(wp[i], wq[i], at + (i * 32 + lane) * PER));
+            const double s = s4[i];
             const bool passed = pick >= 0 && hit && !none && start_of > want;   // (a run before has it)
             if (s > 0.0 && !passed) { pick = i; base = run2 = start_of; }
             if (!passed) start_of += s;
@@ -372,9 +445,11 @@ draft_verify_kernel(VerifyArgs A) {
 template <class T, bool DRAFT, bool VEC>
 int launch(const VerifyArgs& a, int n, int B, cudaStream_t st) {
     rv_drain_error();
+    const size_t smem = (size_t)ring_at(a.chunks) * sizeof(double) + (VEC ? ring_bytes(DRAFT) : 0);
+    rv_allow_smem<draft_verify_kernel<T, DRAFT, VEC>>(ring_at(DV_MAX_VOCAB / chunk_of<T>()) * 8 + ring_bytes(DRAFT));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)n, (unsigned)B); cfg.blockDim = dim3(DV_THREADS);
-    cfg.dynamicSmemBytes = (size_t)a.chunks * sizeof(double); cfg.stream = st;
+    cfg.dynamicSmemBytes = smem; cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -386,10 +461,10 @@ int launch(const VerifyArgs& a, int n, int B, cudaStream_t st) {
 }
 template <class T>
 int dispatch(VerifyArgs& a, int B, cudaStream_t st) {
-    // blocks a sequence: until there are two to an SM, while a part has four chunks
+    // blocks a sequence: as many as run at once, while a part has four chunks
     const int sms = rv_sm_count(), all = (a.vocab + chunk_of<T>() - 1) / chunk_of<T>();
     int n = 1;
-    while (n < DV_MAX_CLUSTER && (long long)B * n < 2 * sms && all / (2 * n) >= 4) n *= 2;
+    while (n < DV_MAX_CLUSTER && (long long)B * 2 * n <= per_sm(a.draft != nullptr) * sms && all / (2 * n) >= 4) n *= 2;
     a.chunks = (all + n - 1) / n;
     const bool vec = (((uintptr_t)a.target | (uintptr_t)a.draft) & 15) == 0 && a.target_stride * (long long)sizeof(T) % 16 == 0 &&
                      (!a.draft || a.draft_stride * (long long)sizeof(T) % 16 == 0);
