@@ -38,10 +38,10 @@ constexpr int NK = 5, NG = 2, GW = 4;                // stages; softmax groups, 
 constexpr int TM_SW = 4 * NG, TM_QKW = TM_SW, TM_PVW = TM_SW + 1, TM_GW0 = TM_SW + 2;
 constexpr int TM_THREADS = (TM_GW0 + GW) * 32, TM_SOFTMAX = TM_SW * 32, TM_GROUP = 128;
 constexpr float TM_POFF = 5.0f, TM_MOST = 256.0f;    // P' = 2^(s - ref + 5) <= 2^8: references lag by 2^3 at most, see attend_mma.cu
-constexpr int TM_MIN_TILES = 4;                      // tiles a CTA takes at least, while there are few
-// What a row block costs beside its tiles, in tiles: its queries, its output and the pipeline's ramp take 26,000 cycles, a tile 1,650. It
-// is counted where CTAs take several blocks each (32 trees over 512 to 8,192 rows: 383 us with runs of as many tiles, 280 with runs of
-// equal cost); with fewer blocks than CTAs every run pays it once.
+constexpr int TM_MIN_TILES = 4;                      // tiles a CTA takes at least, while there are few: a CTA per block, or as many as that leaves
+// What a row block costs beside its tiles, in tiles: its queries, its output and the pipeline's ramp take 26,000 cycles, a tile 1,650. A
+// run pays it for each block that it touches; the first is the same for all runs, so that the blocks that begin inside a run count
+// (32 trees over 512 to 8,192 rows: 383 us with runs of as many tiles, 280 with runs of equal cost; 31 nodes over 32,771 rows: 161 and 157).
 constexpr int TM_BLOCK_COST = 16;
 
 // tensor memory columns
@@ -199,9 +199,9 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
         for (int b0 = 0; b0 < A.B; b0 += 32) { sizes(b0 + lane); tiles += (long long)nt * nrb; blocks += nrb; }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) { tiles += __shfl_xor_sync(0xffffffffu, tiles, o); blocks += __shfl_xor_sync(0xffffffffu, blocks, o); }
-        const int cost = blocks > gridDim.x ? TM_BLOCK_COST : 0, g = blockIdx.x;
+        const int cost = blocks > 1 ? TM_BLOCK_COST : 0, g = blockIdx.x;
         const long long total = tiles + cost * blocks;
-        const int n = (int)max(1LL, min((long long)gridDim.x, tiles / TM_MIN_TILES));
+        const int n = (int)max(1LL, min((long long)gridDim.x, max(blocks, tiles / TM_MIN_TILES)));
         const long long u0 = g < n ? run_begin(total, g, n) : total, u1 = g < n ? run_begin(total, g + 1, n) : total;
         if (lane == 0) { s_units[0] = 0; s_units[1] = total; s_run[0] = A.B; s_run[1] = s_run[2] = 0; s_run[3] = n; s_run[4] = cost; }
         __syncwarp();
@@ -681,7 +681,7 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
                     if (again) break;
                     const float was_a = m_a, was_b = m_b;
                     // the references as the tile before left them (another group's)
-                                        if (i > i0) {
+                    if (i > i0) {
                         ok = wait_for(&bars.dec[th ^ 1], ((i - 1) >> 1) & 1, abort_flag, 65, max_polls);
                         const float na = s_mref[ra], nb = s_mref[rb];
                         if (na != m_a) { l_a *= exp2f(m_a - na); m_a = na; }
