@@ -20,6 +20,12 @@ from . import backend as be
 MAX_NODES = 64
 
 
+def _fits(name: str, t: torch.Tensor, rows: int, shape: tuple, dtype) -> None:
+    """At least ``rows`` rows of ``shape``, one behind the other."""
+    if t.dim() != len(shape) + 1 or t.shape[0] < rows or tuple(t.shape[1:]) != shape or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(f"{name}: {tuple(t.shape)} of {t.dtype}; contiguous {dtype} of {(rows, *shape)} or more rows")
+
+
 class DraftTree:
     """The trees of a batch. ``parents[b][j]`` is the node that node ``j`` of sequence ``b`` hangs below, an earlier one; node 0 has
     none (-1). A sequence without nodes sits the step out."""
@@ -85,6 +91,8 @@ class DraftStep:
 
     def rotate(self, q: torch.Tensor, k: "torch.Tensor | None" = None, stream=None) -> None:
         """Rotary positions of the step's rows, in place: ``q`` [n_nodes, heads, seg], ``k`` [n_nodes, seg], views of wider rows."""
+        if self.inv_freq is None or q.shape[0] < self.tree.n_nodes or (k is not None and k.shape[0] < self.tree.n_nodes) or q.shape[-1] != 2 * len(self.inv_freq):
+            raise ValueError("rotate: rows of the step and the segment of its frequencies")
         be.launch_rope_rows_bf16(be.rope_vecs(q), None if k is None else be.rope_vecs(k), self.tree.n_nodes, self.pos, self.inv_freq,
                                  q.shape[-1], self.layout, self.rope_scale, stream)
 
@@ -94,9 +102,18 @@ class DraftStep:
         [n_nodes, index_dim] or None, ``q`` [n_nodes, heads, kv_lora + rope]. Every node sees the whole prefix, or, with ``selection`` (rows u32
         [B, k], counts i32 [B]), those rows of it. Returns [n_nodes, heads, kv_lora]."""
         L, t, n = self.stack.layers[i], self.tree, self.tree.n_nodes
+        g, bf16 = L.g, torch.bfloat16
+        _fits("latent", latent, n, (g.kv_lora + g.rope_dim,), bf16)
+        _fits("q", q, n, (g.n_heads, g.kv_lora + g.rope_dim), bf16)
+        if index_key is not None:
+            _fits("index_key", index_key, n, (g.index_dim,), bf16)
         be.launch_kv_append_paged(L.g, latent, L._no_key(n) if index_key is None else index_key, t.seq, self.row_pos, n, L.block_table,
                                   L.latent_pool, L.latent_scale, L.index_pool, L.index_scale, self.status, stream)
         rows, counts = (None, None) if selection is None else selection
+        if rows is not None:
+            if rows.dim() != 2 or rows.shape[0] < t.B or rows.element_size() != 4 or not rows.is_contiguous():
+                raise ValueError(f"selection: {tuple(rows.shape)} of {rows.dtype}; contiguous u32 of {t.B} sequences")
+            _fits("selection's counts", counts, t.B, (), torch.int32)
         be.launch_mla_tree_attend_paged_bf16(L.g, q, L.latent_pool, L.latent_scale, L.block_table, rows,
                                              0 if rows is None else rows.shape[1], counts, self.tree_pos, t.node_start, t.mask, t.B, n,
                                              self.out, self.lse, self.scratch, stream)
@@ -111,6 +128,11 @@ class DraftStep:
         if target.dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"probabilities in {target.dtype}")
         t = self.tree
+        if target.dim() != 2 or target.shape[0] < t.n_nodes:
+            raise ValueError(f"probabilities of {tuple(target.shape)} for {t.n_nodes} nodes")
+        _fits("token", token, t.n_nodes, (), torch.int32)
+        _fits("u", u, t.n_nodes, (), torch.float32)
+        _fits("u_next", u_next, t.B, (), torch.float32)
         be.launch_draft_verify(t.node_start, t.parent, token, target, target.stride(0), draft, 0 if draft is None else draft.stride(0),
                                target.element_size() * 8, target.shape[1], u, u_next, t.B, self.path, MAX_NODES, self.n_path,
                                self.next_token, stream)
@@ -119,6 +141,7 @@ class DraftStep:
     def commit(self, seq_len: torch.Tensor, stream=None) -> None:
         """The accepted rows of all layers to their places; ``seq_len`` i32 [B] becomes the tokens in the cache."""
         L = self.stack.layers[0]
+        _fits("seq_len", seq_len, self.tree.B, (), torch.int32)
         be.launch_kv_commit_paged(L.g, self.pools, len(self.stack.layers), L.block_table, self.tree_pos, self.path, MAX_NODES,
                                   self.n_path, self.tree.B, seq_len, self.status, stream)
 

@@ -475,6 +475,35 @@ def test_verify_leaves_the_targets_distribution(be, given):
     assert (n_path > 1).double().mean() > 0.3
 
 
+@pytest.mark.parametrize("dtype, V, given", [(torch.float32, 32003, False), (BF, 151552, True), (BF, 5000, False), (torch.float32, 4099, True)])
+def test_verify_draws_every_place(be, dtype, V, given):
+    """A draw lands where it has to at the borders of loads, runs, chunks and blocks' parts: three neighbours hold all of a row, in
+    quarters whose sums are exact, and the random number is a border itself or lies between two."""
+    at = sorted({p for c in (4, 8, 32, 128, 256, 512, 1024, 2048, 4096, 8192, 18944, 32768) for k in (1, 2, 3, 5, 7) for p in (c * k - 1, c * k, c * k + 1)
+                 if 1 <= p < V - 1} | {1, 2, V - 2, V - 3})
+    B = 4 * len(at)
+    mid = torch.tensor(at, device=DEV).repeat(4)
+    row = torch.arange(B, device=DEV)
+    target = torch.zeros((B, V), dtype=dtype, device=DEV)
+    for d, w in ((-1, 0.25), (0, 0.5), (1, 0.25)):
+        target[row, mid + d] = w
+    u_next = torch.tensor([0.0, 0.25, 0.625, 0.75], device=DEV).repeat_interleave(len(at))
+    move = torch.tensor([-1, 0, 0, 1], device=DEV).repeat_interleave(len(at))
+    path, n_path, nxt = torch.zeros((B, 1), dtype=torch.int32, device=DEV), i32([0] * B), i32([-9] * B)
+    be.launch_draft_verify(i32(range(B + 1)), i32([-1] * B), i32([0] * B), target, V, None if given else target, V, dtype.itemsize * 8, V,
+                           torch.zeros(B, device=DEV), u_next, B, path, 1, n_path, nxt)
+    assert torch.equal(nxt.long(), mid + move)
+    assert (n_path == 1).all() and (path == 0).all()
+
+
+@pytest.mark.parametrize("B", [1, 37, 80, 400])
+def test_verify_few_and_many_sequences(be, B):
+    """From eight blocks a sequence to one, with rows of a whole number of chunks and with one value more."""
+    for V in (16384, 16385):
+        case = drafted(B + V, B, 3, V, BF, B % 2 == 0, "tree", 16384 + 8 - V)
+        run_verify(be, *case, most=3, vocab=V)
+
+
 # --- commit -----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("page, kvl, rope, hd, layers, B", [(64, 512, 64, 128, 3, 5), (16, 512, 64, 64, 40, 40), (1, 128, 16, 16, 1, 2), (128, 512, 128, 512, 2, 3)])
 def test_commit_against_the_definition(be, page, kvl, rope, hd, layers, B):
@@ -680,3 +709,35 @@ def test_step_refuses(be):
     for bad in (dict(target=p.half()), dict(target=p.t()), dict(target=p, draft=p.to(BF)), dict(target=p, draft=p[:, :4])):
         with pytest.raises(ValueError):
             step.verify(i32([0, 0]), bad["target"], u, u, bad.get("draft"))
+
+
+def test_step_refuses_what_does_not_fit(be):
+    """Sizes, types and strides that a kernel would read past."""
+    from rivoli_b200.draft import DraftStep, DraftTree
+    stack = make_stack(be, 2, 64, (True, True))
+    step = DraftStep(stack, 4)
+    step.begin(DraftTree([[-1, 0], [-1]]), i32([0, 0]))
+    g = stack.layers[0].g
+    p, u, tok = torch.full((3, 8), 0.125, device=DEV), torch.zeros(3, device=DEV), i32([0, 0, 0])
+    good = dict(token=tok, target=p, u=u, u_next=u[:2])
+    for name, bad in (("token", i32([0, 0])), ("token", tok.long()), ("token", i32([0] * 6)[::2]), ("target", p[:2]), ("u", u[:2]), ("u", u.double()),
+                      ("u_next", u[:1]), ("u_next", u.to(BF))):
+        with pytest.raises(ValueError):
+            step.verify(**{**good, name: bad})
+    w = g.kv_lora + g.rope_dim
+    lat, key, q = (torch.zeros(x, dtype=BF, device=DEV) for x in ((3, w), (3, g.index_dim), (3, g.n_heads, w)))
+    good = dict(latent=lat, index_key=key, q=q)
+    for name, bad in (("latent", lat[:2]), ("latent", lat.float()), ("latent", torch.zeros((3, 2 * w), dtype=BF, device=DEV)[:, :w]), ("index_key", key[:, :8]),
+                      ("q", q[:2]), ("q", q[:, :1]), ("q", q.transpose(0, 1))):
+        with pytest.raises(ValueError):
+            step.layer(0, **{**good, name: bad})
+    rows, n = torch.zeros((2, 4), dtype=torch.int32, device=DEV), i32([0, 0])
+    for bad in ((rows[:1], n), (rows, n[:1]), (rows.t(), n), (rows, n.long())):
+        with pytest.raises(ValueError):
+            step.layer(0, **good, selection=bad)
+    with pytest.raises(ValueError):
+        step.rotate(q[:2, :, g.kv_lora:])
+    with pytest.raises(ValueError):
+        step.commit(n[:1])
+    with pytest.raises(ValueError):
+        step.commit(n.long())
