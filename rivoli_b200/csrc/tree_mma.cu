@@ -2,13 +2,14 @@
 //
 //     out[r] = sum_j softmax_j((q_r . [L_j | R_j]) * scale) * L_j,    r = (node, head) of one sequence, j = its prefix, then its tree
 //
-// The arithmetic is that of the decode step's attention (attend_mma.cu): cache rows are consumed as the e4m3 codes they are, q and the
-// softmax weights are two e4m3 terms each (2^-8 relative), a row's scale rides in its weight (P' = weight * scale * 2^5), references
+// The arithmetic is that of the decode step's attention (attend_mma.cu): cache rows are consumed as the e4m3 codes they are, q is two e4m3
+// terms (here to a power of two, which loses none of its bits: the scores are those of the bf16 queries), the softmax weights are two
+// each (2^-8 relative), a row's scale rides in its weight (P' = weight * scale * 2^5), references
 // lag behind the running maximum by at most 2^3, sums are f32. What differs is the shape of the work. The nodes of a tree share their
 // prefix, so that the rows of a sequence are nodes x heads, 64 to a block, and one tile of 64 cache rows serves them all: 240 products and
 // more per byte from a single node on and sixteen times that at sixteen nodes. The kernel is bound by the tensor cores and what feeds
 // them, the cache's tiles come from L2, and what has to be even is the number of (row block, tile) pairs per SM:
-//   * one persistent CTA per SM; the pairs of all sequences, in order, are cut into equal runs, one per CTA. A run that begins or ends
+//   * one persistent CTA per SM; the pairs of all sequences, in order, are cut into runs of equal cost, one per CTA. A run that begins or ends
 //     inside a row block leaves that block's (maximum, sum, O) in scratch and a second, small kernel joins the parts; all others are
 //     written directly. No sequence is too long and no batch too ragged for this.
 //   * barriers and their phases run on over the row blocks of a CTA: the next block's tiles are fetched while this one's output is
@@ -477,7 +478,10 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
         for (; !failed && walk_segment(A, w); i0 += w.t1 - w.t0, walk_on(A, w)) {
             const int rows_all = w.s.T * A.H, r0 = w.rb * TM_ROWS, valid = min(TM_ROWS, rows_all - r0);
             const size_t flat = (size_t)w.s.node0 * A.H + r0;      // first row of the block in q, out and out_lse
-            // ---- q -> two e4m3 terms per row: hi = e4m3(q / s), s = absmax / 448, lo = e4m3(q / s - hi) ----
+            // ---- q -> two e4m3 terms per row: hi = e4m3(q / s), s the power of two at or above absmax / 448, lo = e4m3(q / s - hi) ----
+            // With a power of two the terms are q itself: a bf16 has eight bits, hi takes four of them, and what is left is at most eight of
+            // the last one's units. Only values below 2^-10 of the row's largest lose bits, to the last subnormal of lo: half of 2^-9 s,
+            // 2^-18 of the largest at most. (With s = absmax / 448 each value was 2^-8 off and the sums of the softmax 1e-4.)
             // A warp takes sixteen rows and half th of their columns. They arrive as whole 128-byte lines (lanes 8 k .. 8 k + 7 on one row),
             // are split there and go through shared memory, 64 columns at a time, to the lanes whose tensor-memory row they are. (A
             // lane reading its own row, a line per load, waited 10,500 cycles for them.)
@@ -521,7 +525,10 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
                     if (lane < 16) s_wmax[th * 64 + hd] = __uint_as_float(rv_max_bf16x2(a, x) << 16);
                 }
                 tc::named_barrier(3, TM_SOFTMAX);          // (also: all groups are through with the block before)
-                auto scale_of = [&](int r) { const float amax = fmaxf(s_wmax[r], s_wmax[64 + r]); return amax > 0.0f ? amax / 448.0f : 1.0f; };
+                auto scale_of = [&](int r) -> float {          // the power of two at or above absmax / 448
+                    const float amax = fmaxf(s_wmax[r], s_wmax[64 + r]);
+                    return amax > 0.0f ? fmaxf(__uint_as_float((__float_as_uint(amax / 448.0f) + 0x007fffffu) & 0xff800000u), 1.17549435e-38f) : 1.0f;
+                };
                 if (th == 0 && tb == 0) { s_ahi[hd] = scale_of(hd) * A.softmax_scale * 1.4426950408889634f; s_mref[hd] = -INFINITY; }
                 auto codes8 = [&](const uint4 x, float inv, uint2& hi, uint2& lo) {
                     const uint32_t ww[4] = {x.x, x.y, x.z, x.w};

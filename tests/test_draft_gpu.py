@@ -294,6 +294,28 @@ def test_flat_and_peaked_scores(be, q_scale):
     run_tree(be, Cache(15, [700], 64, spread=0.3), 64, [690], [4], masks_of(host, 4, "tree"), q_scale=q_scale)
 
 
+@pytest.mark.parametrize("H, q_scale, spread", [(64, 1.0, 1.0), (16, 1.0, 0.3), (64, 7.3, 0.3), (64, 1e-30, 1.0)])
+def test_scores_keep_the_querys_bits(be, H, q_scale, spread):
+    """A bf16 is two e4m3 terms in full if it is within 2^-10 of its row's largest, and off by at most 2^-18 of that if not: the sums of
+    the softmax, which nothing else rounds to fewer than 32 bits, show it. Sums in the tensor cores: 18 steps of 32 products for each
+    of two terms and their own sum, each rounded or cut to 24 bits, 2^-23; 2^-18 for the exponentials and the sum over 1,106 rows."""
+    cache = Cache(21, [1106], 64, spread=spread)
+    out, lse, args, _ = run_tree(be, cache, H, [1100], [6], masks_of(random.Random(21), 6, "chain"), q_scale=q_scale, seed=3)
+    at = orc.tree_rows(cache.table[0], cache.page, cache.n_pages, 1100, None, 1100, 6)
+    k = torch.from_numpy(cache.codes).view(torch.float8_e4m3fn).double().numpy()[at] * cache.scale[at].astype(np.float64)[:, None]
+    q = args[1].double().cpu().numpy()
+    scale = float(np.float32(args[0].softmax_scale))
+    for t in range(6):
+        seen = slice(0, 1100 + t + 1)
+        s = q[t] @ k[seen].T * scale
+        top = s.max(1, keepdims=True)
+        want = top[:, 0] + np.log(np.exp(s - top).sum(1))
+        off = (2.0 ** -18 * np.abs(q[t]).max(1, keepdims=True) * np.abs(k[seen]).sum(1) + 37 * 2.0 ** -23 * (np.abs(q[t]) @ np.abs(k[seen]).T)) * scale
+        # what a row's score is off by moves the sum by its share of it
+        tol = (np.exp(s - top) / np.exp(s - top).sum(1, keepdims=True) * off).sum(1) + 2.0 ** -18 + 2.0 ** -22 * np.abs(want)
+        assert (np.abs(lse[t].double().cpu().numpy() - want) <= tol).all(), (np.abs(lse[t].double().cpu().numpy() - want) / tol).max()
+
+
 def test_long_cache(be):
     """One sequence split over the whole chip, and short ones beside it."""
     host = random.Random(16)
