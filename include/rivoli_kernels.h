@@ -601,7 +601,7 @@ int rivoli_rope_rows_bf16(const RopeVecs* q, const RopeVecs* k, int n_rows, cons
  * the whole tree (its root's selection, say), or with rows NULL the first n_rows[b] tokens, n_rows NULL meaning tree_pos[b] of them;
  * a list that begins with the dense marker 0xFFFFFFFF stands for the first n_rows[b] tokens - and node i of its own tree, whose row is
  * token tree_pos[b] + i, where bit i of node_mask (u64 [n_nodes]) is up: for a tree its ancestors and itself. A node that sees nothing
- * gets zeros and -inf. Rows on unmapped pages are seen by nobody. Outputs of nodes from node_start[B] on, and of a sequence's nodes
+ * gets zeros and -inf. Rows on unmapped pages, and rows of a scale of zero or below, are seen by nobody. Outputs of nodes from node_start[B] on, and of a sequence's nodes
  * behind its 64th, are left as they were. scratch = rivoli_mla_tree_attend_scratch_bytes(), zeroed once (it begins with a sticky error
  * word); calls that may run at the same time need one each. kv_lora 512 with rope_dim 64 runs on the tensor cores for any number of
  * heads (given scratch), other geometries on CUDA cores. Which rows share a block goes by the whole call, so that the last bits of a

@@ -5,7 +5,7 @@
 //
 // over the n prefix rows of the node's sequence (a row list, or its first n tokens) and those rows of the tree itself whose bit is up
 // in the node's mask; node j's row is the sequence's token tree_pos + j. A node that sees nothing gets zeros and a log-sum-exp of
-// minus infinity. Rows on pages that the block table leaves unmapped are seen by nobody.
+// minus infinity. Rows on pages that the block table leaves unmapped, and rows whose scale is not above zero, are seen by nobody.
 //
 // CUDA cores: a block takes 16 (node, head) rows of one sequence, two a warp, and 16 cache rows at a time, dequantised into shared
 // memory once for all of them; scores, running maximum and sum, and the output are 32-bit. It is bound by its shuffles and
@@ -56,7 +56,10 @@ tree_simt_kernel(TreeArgs A, int kvl, int rope) {
     const int total = s.n + s.T;
     for (int j0 = 0; j0 < total; j0 += TS_TILE) {
         __syncthreads();
-        if (tid < TS_TILE) s_row[tid] = j0 + tid < total ? tree_pool_row(A, b, tree_token(A, s, b, j0 + tid)) : 0xffffffffu;
+        if (tid < TS_TILE) {
+            const uint32_t r = j0 + tid < total ? tree_pool_row(A, b, tree_token(A, s, b, j0 + tid)) : 0xffffffffu;
+            s_row[tid] = r != 0xffffffffu && A.pscale[r] <= 0.0f ? 0xffffffffu : r;
+        }
         __syncthreads();
         for (int i = tid; i < TS_TILE * (W / 2); i += TS_THREADS) {
             const int t = i / (W / 2), c = 2 * (i - t * (W / 2));
@@ -82,7 +85,7 @@ tree_simt_kernel(TreeArgs A, int kvl, int rope) {
                 if (lane == t && ((sees >> t) & 1) && s_row[t] != 0xffffffffu) mine = d;
             }
             const float top = fmaxf(m[u], rv_warp_max(mine));
-            if (top == -INFINITY) continue;                    // nothing seen so far (the same for all lanes)
+            if (top == -INFINITY && !__any_sync(0xffffffffu, mine != mine)) continue;   // nothing seen so far (NaN is something)
             const float fac = expf(m[u] - top), p = expf(mine - top);
             l[u] = l[u] * fac + rv_warp_sum(p);
             m[u] = top;
@@ -100,11 +103,11 @@ tree_simt_kernel(TreeArgs A, int kvl, int rope) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         if (!live[u]) continue;
-        const float inv = l[u] > 0.0f ? 1.0f / l[u] : 0.0f;
+        const float inv = l[u] == 0.0f ? 0.0f : 1.0f / l[u];   // (NaN stays NaN)
 #pragma unroll
         for (int k = 0; k < TS_KVL / 32; ++k)
             if (lane + 32 * k < kvl) A.out[at[u] * kvl + lane + 32 * k] = rv_f32_to_bf16(acc[u][k] * inv);
-        if (A.out_lse && lane == 0) A.out_lse[at[u]] = l[u] > 0.0f ? m[u] + logf(l[u]) : -INFINITY;
+        if (A.out_lse && lane == 0) A.out_lse[at[u]] = l[u] == 0.0f ? -INFINITY : m[u] + logf(l[u]);
     }
 }
 

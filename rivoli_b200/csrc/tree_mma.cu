@@ -701,12 +701,13 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
                     if (m_a != was_a || m_b != was_b) most *= fmaxf(exp2f(was_a - m_a), exp2f(was_b - m_b));
                     const bool grown = most > TM_MOST || was_a == -INFINITY || was_b == -INFINITY;
                     if (__builtin_expect(tc::barrier_any(6 + th, TM_GROUP, grown || !ok), 0)) {
-                        // the largest x + log2(scale) of a row is what P' goes by
+                        // the largest x + log2(scale) of a row is what P' goes by (scales below 2^-100 as that: their weights would
+                        // pass 2^127)
                         float ta = -INFINITY, tb2 = -INFINITY;
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
                             const float2 s2 = unpack(sc[4 * k]), ya = unpack(x[2 * k]), yb = unpack(x[2 * k + 1]);
-                            const float g0 = __log2f(s2.x), g1 = __log2f(s2.y);
+                            const float g0 = fmaxf(__log2f(s2.x), -100.0f), g1 = fmaxf(__log2f(s2.y), -100.0f);
                             ta = fmaxf(ta, fmaxf(ya.x + g0, ya.y + g1)); tb2 = fmaxf(tb2, fmaxf(yb.x + g0, yb.y + g1));
                         }
 #pragma unroll

@@ -259,6 +259,26 @@ def test_a_node_that_is_nan_reaches_its_descendants_alone(be, kvl):
         assert lse2[node].isnan().all() or (lse2[node] == math.inf).all() or again[node].isnan().any(), node
 
 
+@pytest.mark.parametrize("kvl", [512, 256])
+@pytest.mark.parametrize("where", ["code", "scale", "query"])
+def test_a_node_that_sees_nan_alone(be, kvl, where):
+    """Nothing but NaN is not nothing: the node's output and log-sum-exp are NaN, and the next sequence's are what they are."""
+    cache = Cache(22, [1, 9], 64, kvl)
+    out, lse, args, _ = run_tree(be, cache, 8, [0, 8], [1, 1], [1, 1], kvl=kvl)
+    at = orc.tree_rows(cache.table[0], 64, cache.n_pages, 0, None, 0, 1)
+    q, codes, scale = args[1].clone(), args[2].clone(), args[3].clone()
+    if where == "code":
+        codes[at[0]] = 0x7f
+    elif where == "scale":
+        scale[at[0]] = math.nan
+    else:
+        q[0] = math.nan
+    again, lse2 = torch.zeros_like(out), torch.zeros_like(lse)
+    be.launch_mla_tree_attend_paged_bf16(args[0], q, codes, scale, *args[4:13], again, lse2, *args[15:])
+    assert again[0].isnan().all() and lse2[0].isnan().all()
+    assert torch.equal(again[1], out[1]) and torch.equal(lse2[1], lse[1])
+
+
 def test_rows_that_no_node_may_see_do_not_matter(be):
     """NaN codes and infinite scales in rows that only masks hide, and behind the last one."""
     cache = Cache(12, [200, 64], 64)
@@ -316,12 +336,69 @@ def test_scores_keep_the_querys_bits(be, H, q_scale, spread):
         assert (np.abs(lse[t].double().cpu().numpy() - want) <= tol).all(), (np.abs(lse[t].double().cpu().numpy() - want) / tol).max()
 
 
+@pytest.mark.parametrize("kvl, rope", [(512, 64), (256, 64)])
+def test_scales_from_tiny_to_huge(be, kvl, rope):
+    """Row scales of 2^-90 and 2^60 (the query the other way round there, so that scores stay small); below 2^-100 the outputs may vanish
+    but nothing overflows; rows of scale zero are not there."""
+    host = random.Random(24)
+    masks = masks_of(host, 5, "tree")
+    for e in (-90, 60):
+        cache = Cache(24, [205], 64, kvl, rope, spread=0.3)
+        cache.scale = np.ldexp(cache.scale, e).astype(np.float32)
+        run_tree(be, cache, 24, [200], [5], masks, kvl=kvl, rope=rope, q_scale=2.0 ** min(0, -e))
+    cache = Cache(25, [205], 64, kvl, rope, spread=0.3)
+    keep = cache.scale.copy()
+    cache.scale = np.ldexp(keep, -118).astype(np.float32)
+    at = orc.tree_rows(cache.table[0], 64, cache.n_pages, 200, None, 200, 5)
+    cache.scale[at[:50]] = 0.0
+    g = be.DsaGeom.make(n_heads=24, kv_lora=kvl, rope_dim=rope, max_pages_per_seq=4, n_pool_pages=cache.n_pages)
+    q = torch.randn((5, 24, kvl + rope), generator=torch.Generator().manual_seed(1)).to(BF).to(DEV)
+    out, lse = torch.zeros((5, 24, kvl), dtype=BF, device=DEV), torch.zeros((5, 24), device=DEV)
+    sc = torch.zeros(be.mla_tree_attend_scratch_bytes(g, 1, 5), dtype=torch.uint8, device=DEV)
+    be.launch_mla_tree_attend_paged_bf16(g, q, *cache.dev(), None, 0, None, i32([200]), i32([0, 5]), signed(masks), 1, 5, out, lse, sc)
+    torch.cuda.synchronize()
+    seen = torch.tensor([150 + bin(m).count("1") for m in masks], device=DEV, dtype=torch.float64)
+    # scores below 2^-100: the log-sum-exp is the logarithm of the rows' number; 32 bits of an exponent of about 110 and of the sum
+    assert ((lse.double() - seen.log()[:, None]).abs() <= 2.0 ** -15).all()
+    assert (out.float().abs() <= float(cache.scale.max()) * 448).all()
+
+
 def test_long_cache(be):
     """One sequence split over the whole chip, and short ones beside it."""
     host = random.Random(16)
     trees, prefix = [2, 5, 1], [20011, 40, 1500]
     masks = [m for t in trees for m in masks_of(host, t, "tree")]
     run_tree(be, Cache(16, [p + t for p, t in zip(prefix, trees)], 64), 64, prefix, trees, masks)
+
+
+@pytest.mark.parametrize("page, listed", [(64, False), (16, False), (64, True)])
+def test_rows_past_four_gigabytes(be, page, listed):
+    """The same pages at the end of a pool of 4.4 GB and in a small one: the same bits, and the rows move there too."""
+    host = random.Random(23)
+    prefix, trees, H = [700, 90], [5, 9], 16
+    cache = Cache(23, [p + t for p, t in zip(prefix, trees)], page)
+    masks = [m for t in trees for m in masks_of(host, t, "tree")]
+    rows = [sorted(host.sample(range(p), 80)) for p in prefix] if listed else None
+    out, lse, args, _ = run_tree(be, cache, H, prefix, trees, masks, rows=rows, n_rows=[80, 80] if listed else None)
+    g, codes, scale, table = args[0], args[2], args[3], args[4]
+    big_pages = 7_700_000 // page
+    shift = big_pages - cache.n_pages
+    big = be.DsaGeom.make(n_heads=H, page_tokens=page, max_pages_per_seq=table.shape[1], n_pool_pages=big_pages)
+    far = torch.empty((big_pages * page, cache.W), dtype=torch.uint8, device=DEV)
+    far_scale = torch.empty(big_pages * page, device=DEV)
+    far[shift * page:], far_scale[shift * page:] = codes, scale
+    far_table = torch.where(table >= 0, table + shift, table)
+    again, lse2 = torch.zeros_like(out), torch.zeros_like(lse)
+    be.launch_mla_tree_attend_paged_bf16(big, args[1], far, far_scale, far_table, *args[5:13], again, lse2, args[15])
+    torch.cuda.synchronize()
+    be.mla_tree_attend_status(big, args[15])
+    assert torch.equal(again[:14], out[:14]) and torch.equal(lse2[:14], lse[:14])
+    path = torch.tensor([[0, 2, 4], [0, 5, 8]], dtype=torch.int32, device=DEV)
+    for G, pool, sc, tab in ((g, codes, scale, table), (big, far, far_scale, far_table)):
+        be.launch_kv_commit_paged(G, be.commit_layers([(pool, sc, None, None)]), 1, tab, args[8], path, 3, i32([3, 3]), 2, None, None)
+    torch.cuda.synchronize()
+    assert torch.equal(far[shift * page:], codes) and torch.equal(far_scale[shift * page:], scale)
+    assert not torch.equal(codes.cpu(), torch.from_numpy(cache.codes))
 
 
 def test_one_scratch_for_calls_of_every_shape(be):
