@@ -74,10 +74,10 @@ struct Bars {
 static_assert(sizeof(Bars) <= 256, "barrier block");
 constexpr int FULL = GW * 33;                               // arrivals that fill a stage: the copies of 128 lanes, and each gathering warp
 
-// scratch: error word (256 bytes) | per CTA the block it has the beginning of, for the joining kernel | (reference, sum) of parts | O of parts
-constexpr int SLOTS = 2 * RV_SMS;                           // a CTA leaves at most the end of one block and the beginning of another
-struct Head { int32_t row0, valid, parts, pad; };
-constexpr size_t SC_HEAD = 256, SC_ML = SC_HEAD + RV_SMS * sizeof(Head), SC_O = (SC_ML + (size_t)SLOTS * TM_ROWS * 8 + 255) / 256 * 256;
+// scratch: error word (256 bytes) | whose part a CTA has left, for the joining kernel | (reference, sum) of parts | O of parts
+constexpr int SLOTS = 2 * RV_SMS;                           // a CTA leaves at most a later part of one block and the beginning of another
+struct Head { int32_t row0, valid, parts, part; };          // of a slot: the block's first row, its rows (0: nothing left here), parts, which one
+constexpr size_t SC_HEAD = 256, SC_ML = SC_HEAD + SLOTS * sizeof(Head), SC_O = (SC_ML + (size_t)SLOTS * TM_ROWS * 8 + 255) / 256 * 256;
 constexpr size_t SC_TOTAL = SC_O + (size_t)SLOTS * TM_ROWS * TM_KVL * 4;
 
 __device__ __forceinline__ uint32_t sw64_chunk(uint32_t row, uint32_t chunk) { return row * 64u + ((chunk ^ ((row >> 1) & 3u)) << 4); }
@@ -427,10 +427,28 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
         }
     } else if (warp == TM_PVW) {
         // ------------------------------ PV issuer: O^T += V(i)^T . P'(i) --------------------------
+        // Beside it, while it waits for a segment's first weights: whose parts this CTA will have left, for the joining kernel.
         const uint32_t id_pv = tc::idesc_e4m3(128, TM_ROWS, 1, 0);
+        Head* heads = reinterpret_cast<Head*>(scratch + SC_HEAD) + 2 * blockIdx.x;
         bool ok = true;
-        int i = 0, s = 0;
+        int i = 0, s = 0, told = 0;                        // told: which of the two slots have a part
         for (; ok && walk_segment(A, w); walk_on(A, w)) {
+            if (lane == 0 && (w.t0 > 0 || w.t1 < w.nt)) {
+                const long long total = s_units[1];
+                const int n = s_run[3], r0 = w.rb * TM_ROWS;
+                auto run_of = [&](long long unit) -> int {
+                    int g = (int)(unit * n / total);
+                    while (run_begin(total, g + 1, n) <= unit) ++g;
+                    return g;
+                };
+                // (a segment that goes on in the next run ends with this one; one that does not, and is no beginning, begins with it)
+                const bool on = w.t1 < w.nt;
+                const long long at = on ? run_begin(total, blockIdx.x + 1, n) - w.t1 : run_begin(total, blockIdx.x, n) - w.t0;   // the unit of tile 0
+                const int first = w.t0 == 0 ? (int)blockIdx.x : run_of(at), last = on ? run_of(at + w.nt - 1) : (int)blockIdx.x;
+                heads[w.t0 == 0] = Head{w.s.node0 * A.H + r0, min(TM_ROWS, w.s.T * A.H - r0), last - first + 1, (int)blockIdx.x - first};
+                told |= 1 << (w.t0 == 0);
+            }
+            __syncwarp();
 #pragma unroll 1
             for (int t = w.t0; t < w.t1 && ok; ++t, ++i) {
                 const int pb = i & 1;
@@ -458,6 +476,9 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
                 if (++s == NK) s = 0;
             }
         }
+        if (lane == 0)
+            for (int u = 0; u < 2; ++u)
+                if (!(told >> u & 1)) heads[u] = Head{0, 0, 0, 0};
     } else {
         // ------------------------------ queries, softmax, epilogue -------------------------------
         // S: lanes 0-15 of a warp's quarter hold the hi terms of 16 rows, lanes 16-31 their lo terms. Read 16 lanes at a time in the
@@ -474,7 +495,7 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
         // in the barrier it has seen, and then for another's within the NG behind it.
         auto pv_done = [&](int i) { return wait_for(&bars.pv_done[i % NG], (i / NG) & 1, abort_flag, 63, max_polls); };
         int i0 = 0;                                        // tiles of the CTA before this segment
-        bool failed = false, told = false;
+        bool failed = false;
         for (; !failed && walk_segment(A, w); i0 += w.t1 - w.t0, walk_on(A, w)) {
             const int rows_all = w.s.T * A.H, r0 = w.rb * TM_ROWS, valid = min(TM_ROWS, rows_all - r0);
             const size_t flat = (size_t)w.s.node0 * A.H + r0;      // first row of the block in q, out and out_lse
@@ -838,24 +859,10 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
 #pragma unroll
                     for (int h = 0; h < 32; ++h) po[(size_t)(th * 32 + h) * TM_KVL + c * 128] = __uint_as_float(r[h]);
                 }
-                if (w.t0 == 0 && tid == 0) {
-                    // this CTA has the block's beginning: which runs hold the rest
-                    const long long total = s_units[1], end = run_begin(total, blockIdx.x + 1, s_run[3]) + (w.nt - w.t1) - 1;   // the block's last unit
-                    int last = (int)(end * s_run[3] / total);
-                    while (run_begin(total, last + 1, s_run[3]) <= end) ++last;
-                    Head h{(int32_t)flat, valid, last - (int)blockIdx.x + 1, 0};
-                    reinterpret_cast<Head*>(scratch + SC_HEAD)[blockIdx.x] = h;
-                    told = true;
-                }
             }
             tc::tc_fence_before();
         }
         if (sq == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        // no block begins in this run and ends in another: nothing for the joining kernel
-        if (tid == 0 && !told) {
-            Head h{0, 0, 0, 0};
-            reinterpret_cast<Head*>(scratch + SC_HEAD)[blockIdx.x] = h;
-        }
     }
 
     tc::tc_fence_before();
@@ -867,44 +874,109 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
     if (tid == 0 && *abort_flag) atomicCAS(err, 0, *abort_flag);
 }
 
-// Joins the parts of the row block whose beginning CTA blockIdx.x of the kernel before left, eight of its rows per block: a warp per row.
-__global__ void __launch_bounds__(256)
+// Joins the parts of row blocks, eight rows per blockIdx.y. Up to eight parts: by the CTA of the first, a warp per row. More: the CTAs of
+// all parts share the rows, part k takes rows k, k + parts, ... of the eight, all its warps on one row at a time, so that a hundred parts
+// have their loads on their way at once (one sequence over 131,072 rows, both kernels: 117 us with a warp per row, 59 so; blocks of two
+// parts the other way round: 16 trees of 8 over 2,048 rows 72 us when shared, 64 alone).
+constexpr int TJ_WARPS = 8, TJ_ALONE = 8;
+// dims 4 d .. 4 d + 3 of a row
+__device__ __forceinline__ void join_put(uint16_t* out, int d, float4 x, float inv) {
+    uint2 v;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v.x) : "f"(x.y * inv), "f"(x.x * inv));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v.y) : "f"(x.w * inv), "f"(x.z * inv));
+    reinterpret_cast<uint2*>(out)[d] = v;
+}
+__device__ __forceinline__ void join_add(float4& acc, float4 x, float f) {
+    acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+}
+__device__ __forceinline__ float join_lse(float m, float l) { return l == 0.0f ? -INFINITY : (m - TM_POFF) * 0.6931471805599453f + logf(l); }
+__device__ __forceinline__ bool saw_nothing(float2 part) { return part.x == -INFINITY && part.y == 0.0f; }
+
+__global__ void __launch_bounds__(TJ_WARPS * 32, 4)
 tree_join_kernel(const uint8_t* scratch, uint16_t* out, float* out_lse) {
+    __shared__ float4 s_o[TJ_WARPS][TM_KVL / 4];
     rv_grid_dep_wait();
     rv_grid_dep_trigger();
-    const int g = blockIdx.x, row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const Head h = reinterpret_cast<const Head*>(scratch + SC_HEAD)[g];
-    if (row >= h.valid) return;
-    auto slot = [&](int p) { return p == 0 ? 2 * g + 1 : 2 * (g + p); };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float2* ml = reinterpret_cast<const float2*>(scratch + SC_ML);
-    float m = -INFINITY, l = 0.0f;
-    for (int p = 0; p < h.parts; ++p) m = fmaxf(m, ml[slot(p) * TM_ROWS + row].x);
-    float4 acc[4];
+    const float4* o4 = reinterpret_cast<const float4*>(scratch + SC_O) + lane;
+    const Head* heads = reinterpret_cast<const Head*>(scratch + SC_HEAD) + 2 * blockIdx.x;
+    const Head first = heads[1], later = heads[0];
+    auto at = [](int g, int p, int row) -> size_t { return (size_t)(p == 0 ? 2 * g + 1 : 2 * (g + p)) * TM_ROWS + row; };   // of part p of the block that begins in CTA g
+    const int own = blockIdx.y * 8 + warp;
+    if (first.parts <= TJ_ALONE && own < first.valid) {
+        const int g = blockIdx.x;
+        float m = -INFINITY, l = 0.0f;
+        for (int p = 0; p < first.parts; ++p) m = fmaxf(m, ml[at(g, p, own)].x);
+        float4 acc[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) acc[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int p = 0; p < h.parts; ++p) {
-        const float2 part = ml[slot(p) * TM_ROWS + row];
-        if (part.x == -INFINITY && part.y == 0.0f) continue;       // the part saw nothing
-        const float f = exp2f(part.x - m);
-        l += part.y * f;
-        const float4* o = reinterpret_cast<const float4*>(scratch + SC_O) + ((size_t)slot(p) * TM_ROWS + row) * (TM_KVL / 4);
+        for (int c = 0; c < 4; ++c) acc[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int p = 0; p < first.parts; ++p) {
+            const float2 part = ml[at(g, p, own)];
+            if (saw_nothing(part)) continue;
+            const float f = exp2f(part.x - m);
+            l += part.y * f;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const float4 x = o[c * 32 + lane];
-            acc[c].x = fmaf(x.x, f, acc[c].x); acc[c].y = fmaf(x.y, f, acc[c].y);
-            acc[c].z = fmaf(x.z, f, acc[c].z); acc[c].w = fmaf(x.w, f, acc[c].w);
+            for (int c = 0; c < 4; ++c) join_add(acc[c], o4[at(g, p, own) * (TM_KVL / 4) + c * 32], f);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) join_put(out + ((size_t)first.row0 + own) * TM_KVL, c * 32 + lane, acc[c], l == 0.0f ? 0.0f : 1.0f / l);
+        if (out_lse && lane == 0) out_lse[first.row0 + own] = join_lse(m, l);
+    }
+#pragma unroll 1
+    for (int u = 0; u < 2; ++u) {
+        const Head h = u ? first : later;
+        if (h.parts <= TJ_ALONE) continue;                     // (the same for the whole block)
+        const int g = blockIdx.x - h.part;
+#pragma unroll 1
+        for (int row = blockIdx.y * 8 + h.part; row < min(h.valid, (int)blockIdx.y * 8 + 8); row += h.parts) {
+            float m = -INFINITY, l = 0.0f;
+            for (int p = lane; p < h.parts; p += 32) m = fmaxf(m, ml[at(g, p, row)].x);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            for (int p = lane; p < h.parts; p += 32) {
+                const float2 part = ml[at(g, p, row)];
+                if (!saw_nothing(part)) l += part.y * exp2f(part.x - m);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            float4 acc[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+            for (int p0 = warp; p0 < h.parts; p0 += 2 * TJ_WARPS) {            // two parts on their way at once
+                float4 x[2][4];
+                float2 part[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int p = p0 + e * TJ_WARPS;
+                    part[e] = make_float2(-INFINITY, 0.0f);
+                    if (p >= h.parts) continue;
+                    part[e] = ml[at(g, p, row)];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) x[e][c] = o4[at(g, p, row) * (TM_KVL / 4) + c * 32];
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if (saw_nothing(part[e])) continue;
+                    const float f = exp2f(part[e].x - m);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) join_add(acc[c], x[e][c], f);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s_o[warp][c * 32 + lane] = acc[c];
+            __syncthreads();
+            if (threadIdx.x < TM_KVL / 4) {
+                float4 x = s_o[0][threadIdx.x];
+#pragma unroll
+                for (int k = 1; k < TJ_WARPS; ++k) join_add(x, s_o[k][threadIdx.x], 1.0f);
+                join_put(out + ((size_t)h.row0 + row) * TM_KVL, threadIdx.x, x, l == 0.0f ? 0.0f : 1.0f / l);
+            }
+            if (out_lse && threadIdx.x == 0) out_lse[h.row0 + row] = join_lse(m, l);
+            __syncthreads();
         }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint2* to = reinterpret_cast<uint2*>(out + ((size_t)h.row0 + row) * TM_KVL);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        uint2 v;
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v.x) : "f"(acc[c].y * inv), "f"(acc[c].x * inv));
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v.y) : "f"(acc[c].w * inv), "f"(acc[c].z * inv));
-        to[c * 32 + lane] = v;
-    }
-    if (out_lse && lane == 0) out_lse[h.row0 + row] = l == 0.0f ? -INFINITY : (m - TM_POFF) * 0.6931471805599453f + logf(l);
 }
 
 }  // namespace
@@ -927,6 +999,6 @@ int rv_tree_mma(const TreeArgs& a, void* scratch, cudaStream_t st) {
     }
     rv_launch_dependent(tree_mma_kernel, dim3(grid), dim3(TM_THREADS), (size_t)SM_TOTAL, st, a, k_map, r_map, tma, reinterpret_cast<int*>(s), s, (int)tc::kMaxPolls);
     if (int e = rv_launch_status()) return e;
-    rv_launch_dependent(tree_join_kernel, dim3(grid, TM_ROWS / 8), dim3(256), 0, st, (const uint8_t*)s, a.out, a.out_lse);
+    rv_launch_dependent(tree_join_kernel, dim3(grid, TM_ROWS / 8), dim3(TJ_WARPS * 32), 0, st, (const uint8_t*)s, a.out, a.out_lse);
     return rv_launch_status();
 }
