@@ -15,10 +15,12 @@
 // without them (as they are when Z has come below a thousandth of the whole and would lose its last bits). Sums, products and
 // comparisons are in 64 bits: a draw next to a border has to come out the same whatever the order of summation.
 //
-// A cluster of up to eight blocks per sequence, each a contiguous part of the vocabulary; every block walks the tree itself (the few
-// probabilities that decide are gathered at once for all nodes), and only sums are exchanged, through distributed shared memory. Bound by
-// memory where the batch is large: one row of the target and one of the draft per pass, a chunk of 2 KiB of each per warp and step; for few
-// sequences by the chain launch, node words, probabilities, pass, exchange, chunk, place.
+// A cluster of up to eight blocks per sequence, each a contiguous part of the vocabulary, as many blocks as run at once; every block walks
+// the tree itself (the few probabilities that decide are gathered at once for all nodes), and only sums are exchanged, through distributed
+// shared memory. A warp's chunks of 2 KiB a row come through a ring of its own (with one chunk in registers at a time a pass of five chunks
+// waited 15,000 cycles, so 9,000). 128 sequences of 12 chosen tokens over 151,552 bf16: 26 us, the first pass of all sequences at
+// 3.9 TB/s (conversions to 64 bits: 16 a clock and SM), then the few that take two more; 48 of 8 drawn over 131,072 f32: 30 us. For
+// few sequences bound by the chain launch, node words, probabilities, pass, exchange, chunk, place: 7.5 us for one of 6 over 32,003.
 #include "codec.cuh"
 #include "common.cuh"
 #include "tc_common.cuh"
