@@ -737,8 +737,8 @@ def rope_frequencies(seg: int, theta: float = 10000.0, scaling: str = "none", fa
     than ``beta_slow`` times over the original context, keeps those that turn more than ``beta_fast`` times, blends between, and
     scales by 0.1 ln(factor) + 1."""
     import numpy as np
-    if seg <= 0 or seg % 2 or theta <= 1 or factor < 1:
-        raise ValueError(f"rope_frequencies: seg {seg}, theta {theta}, factor {factor}")
+    if seg <= 0 or seg % 2 or theta <= 1 or factor < 1 or original < 1:
+        raise ValueError(f"rope_frequencies: seg {seg}, theta {theta}, factor {factor}, original {original}")
     if scaling == "ntk":
         if seg < 4:
             raise ValueError("rope_frequencies: ntk needs two pairs")

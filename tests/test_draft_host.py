@@ -191,3 +191,9 @@ def test_oracle_commit():
     for path in ([1, 1], [0, 3, 2], [0, 64]):
         assert not orc.commit([a], np.array([1, 0]), 16, 2, 0, path)
     assert not orc.commit([a], np.array([1, -1]), 16, 2, 14, [0, 2])
+
+
+def test_frequencies_need_an_original_context(be):
+    for scaling in ("none", "yarn"):
+        with pytest.raises(ValueError):
+            be.rope_frequencies(64, 10000.0, scaling, 4.0, 0)
