@@ -42,10 +42,9 @@ struct VerifyArgs {
 __device__ __forceinline__ float clean(float x) { return x > 0.0f && x < INFINITY ? x : 0.0f; }
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync() { cluster_arrive(); cluster_wait(); }
 __device__ __forceinline__ void put_remote(double* mine, uint32_t rank, double v) {
     uint32_t at;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
@@ -126,6 +125,9 @@ draft_verify_kernel(VerifyArgs A) {
     __shared__ double s_part[2][DV_MAX_CLUSTER];               // the blocks' sums of a pass, by the pass's parity
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.y;
     const uint32_t rank = cluster_rank(), n_rank = cluster_size();
+    // Another block's shared memory may be written once that block runs: blocks of a cluster are placed together, but do not start
+    // together. The nodes' words are read meanwhile.
+    cluster_arrive();
     rv_grid_dep_wait();
     rv_grid_dep_trigger();
     const int start = A.node_start[b], T_all = A.node_start[b + 1] - start, T_n = min(T_all, DV_NODES);
@@ -144,6 +146,7 @@ draft_verify_kernel(VerifyArgs A) {
     }
     __syncthreads();
     int32_t* path = A.path + (size_t)b * A.max_path;
+    cluster_wait();                                            // all blocks have started
     if (T_n <= 0) {                                            // (the same for all blocks of the cluster)
         if (rank == 0 && tid == 0) { A.n_path[b] = 0; A.next[b] = -1; }
         return;
