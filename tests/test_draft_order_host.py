@@ -21,3 +21,12 @@ def test_the_verification_stores_into_blocks_that_have_started():
     wait = k.find("cluster_wait();")
     assert 0 <= k.find("cluster_arrive();") < k.index("rv_grid_dep_wait()") < wait
     assert "return" not in k[:wait] and wait < k.index("put_remote") and wait < k.index("cluster_sync();")
+
+
+def test_the_verifications_warps_come_to_a_barrier_whole():
+    """An aligned barrier is undefined for a warp whose lanes come to it apart, and the compiler need not bring them together behind a
+    branch: here the lanes that store a sum, and the one that writes the next token."""
+    s = source("draft_verify.cu")
+    assert len(re.findall(r"barrier\.cluster\.(?:arrive|wait)", s)) == 2
+    for m in re.finditer(r"barrier\.cluster\.[\w.]*\.aligned", s):
+        assert re.search(r"__syncwarp\(\);\s*asm volatile\(\"$", s[:m.start()])
