@@ -91,8 +91,12 @@ class DraftStep:
 
     def rotate(self, q: torch.Tensor, k: "torch.Tensor | None" = None, stream=None) -> None:
         """Rotary positions of the step's rows, in place: ``q`` [n_nodes, heads, seg], ``k`` [n_nodes, seg], views of wider rows."""
-        if self.inv_freq is None or q.shape[0] < self.tree.n_nodes or (k is not None and k.shape[0] < self.tree.n_nodes) or q.shape[-1] != 2 * len(self.inv_freq):
-            raise ValueError("rotate: rows of the step and the segment of its frequencies")
+        if self.inv_freq is None:
+            raise ValueError("rotate: a step without frequencies")
+        seg, n = 2 * len(self.inv_freq), self.tree.n_nodes
+        for name, t in (("q", q), ("k", k)):
+            if t is not None and (t.dim() not in (2, 3) or t.shape[0] < n or t.shape[-1] != seg):
+                raise ValueError(f"rotate: {name} of {tuple(t.shape)}; {n} or more rows, segments of {seg}")
         be.launch_rope_rows_bf16(be.rope_vecs(q), None if k is None else be.rope_vecs(k), self.tree.n_nodes, self.pos, self.inv_freq,
                                  q.shape[-1], self.layout, self.rope_scale, stream)
 

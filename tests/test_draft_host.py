@@ -197,3 +197,42 @@ def test_frequencies_need_an_original_context(be):
     for scaling in ("none", "yarn"):
         with pytest.raises(ValueError):
             be.rope_frequencies(64, 10000.0, scaling, 4.0, 0)
+
+
+# --- what a step refuses before anything is launched ----------------------------------------------------------------
+class Stack:
+    """As much of a stack as a step asks for, on the CPU."""
+
+    class pool_layer:
+        def __init__(self, be, B):
+            self.g, self.dev, self.B = be.DsaGeom.make(n_heads=2, max_pages_per_seq=4, n_pool_pages=8), "cpu", B
+            self.latent_pool, self.latent_scale = torch.zeros((512, 576), dtype=torch.uint8), torch.zeros(512)
+            self.index_pool, self.index_scale = torch.zeros((512, 128), dtype=torch.uint8), torch.zeros(512)
+            self.block_table = torch.zeros((B, 4), dtype=torch.int32)
+
+    def __init__(self, be, B=2, layers=1):
+        self.layers = [self.pool_layer(be, B) for _ in range(layers)]
+
+
+@pytest.fixture()
+def step(be, monkeypatch):
+    """A step of three nodes in two sequences whose launches are written down instead of made."""
+    from rivoli_b200.draft import DraftStep, DraftTree
+    s = DraftStep(Stack(be), 4, be.rope_frequencies(64))
+    s.tree, s.launched = DraftTree([[-1, 0], [-1]], device="cpu"), []
+    for name in ("launch_rope_rows_bf16", "launch_kv_append_paged", "launch_mla_tree_attend_paged_bf16", "launch_draft_verify", "launch_kv_commit_paged"):
+        monkeypatch.setattr(be, name, lambda *a, name=name: s.launched.append((name, a)))
+    return s
+
+
+def test_a_step_rotates_keys_of_its_segment_alone(step):
+    """A key narrower than the segment would be read and written past its end, a wider one rotated in part."""
+    bf = torch.bfloat16
+    q, k = torch.zeros((3, 2, 64), dtype=bf), torch.zeros((3, 64), dtype=bf)
+    step.rotate(q, k)
+    step.rotate(q[:, 0], None)
+    assert len(step.launched) == 2
+    for bad in (dict(q=q, k=k[:, :32]), dict(q=q, k=torch.zeros((3, 128), dtype=bf)), dict(q=q, k=k[:2]), dict(q=q, k=k[0]), dict(q=q[..., :32], k=k), dict(q=q[:2], k=k)):
+        with pytest.raises(ValueError):
+            step.rotate(**bad)
+    assert len(step.launched) == 2
