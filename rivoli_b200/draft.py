@@ -72,6 +72,7 @@ class DraftStep:
         self.path = torch.full((B, MAX_NODES), -1, dtype=torch.int32, device=d)
         self.n_path, self.next_token = (torch.zeros(B, dtype=torch.int32, device=d) for _ in range(2))
         self.pools = be.commit_layers([(K.latent_pool, K.latent_scale, K.index_pool, K.index_scale) for K in stack.layers])
+        self.no_key = torch.zeros((max_nodes, g.index_dim), dtype=torch.bfloat16, device=d)   # for layers without an indexer
         self.status = torch.zeros(1, dtype=torch.int32, device=d)
         self.layout = be.ROPE_LAYOUTS[layout]
         self.inv_freq = None if rope is None else torch.from_numpy(rope[0]).to(d)
@@ -111,7 +112,7 @@ class DraftStep:
         _fits("q", q, n, (g.n_heads, g.kv_lora + g.rope_dim), bf16)
         if index_key is not None:
             _fits("index_key", index_key, n, (g.index_dim,), bf16)
-        be.launch_kv_append_paged(L.g, latent, L._no_key(n) if index_key is None else index_key, t.seq, self.row_pos, n, L.block_table,
+        be.launch_kv_append_paged(L.g, latent, self.no_key if index_key is None else index_key, t.seq, self.row_pos, n, L.block_table,
                                   L.latent_pool, L.latent_scale, L.index_pool, L.index_scale, self.status, stream)
         rows, counts = (None, None) if selection is None else selection
         if rows is not None:

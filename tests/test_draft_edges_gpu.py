@@ -1,0 +1,50 @@
+"""The drafted step's operators on the GPU where they can go wrong: long flat tails, rows that are not there, buffers between steps."""
+import pytest
+import torch
+
+from tests.test_draft_gpu import BF, DEV, be, i32, make_stack  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def test_a_captured_step_of_layers_without_a_key(be):
+    """Steps of other sizes between two replays take nothing away that the graph reads."""
+    from rivoli_b200.draft import DraftStep, DraftTree
+    stack = make_stack(be, 2, 16, (True, False))
+    for i in range(2):
+        stack.pool.reserve(i, 100)
+    stack.upload_block_table()
+    step, gen = DraftStep(stack, 8), torch.Generator().manual_seed(2)
+    trees = [DraftTree(p, device=DEV) for p in ([[-1, 0, 0], [-1]], [[-1], [-1]], [[-1, 0, 1, 2], [-1, 0, 0]])]
+    latent, q = (torch.randn(s, generator=gen).to(BF).to(DEV) for s in ((8, 576), (8, 16, 576)))
+    pos = i32([30, 64])
+    L = stack.layers[1]
+
+    def go(tree, stream=None):
+        step.begin(tree, pos, stream)
+        step.layer(1, latent, None, q, None, stream)
+
+    def state():
+        torch.cuda.synchronize()
+        return [t.clone() for t in (step.out[:4], step.lse[:4], L.latent_pool, L.index_pool, L.index_scale)]
+
+    go(trees[0])
+    want = state()
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        go(trees[0], side)
+    for tree in trees[1:]:
+        go(tree)
+        torch.cuda.synchronize()
+        # what the step might have let go of is handed out again
+        held = [torch.full((n, 128), 3.0, dtype=BF, device=DEV) for n in (1, 2, 4, 7, 8) for _ in range(4)]
+        step.out.zero_(), step.lse.zero_(), L.index_pool.fill_(9), L.latent_pool.fill_(9)
+        go(trees[0])
+        again = state()
+        step.out.zero_(), step.lse.zero_(), L.index_pool.fill_(9), L.latent_pool.fill_(9)
+        graph.replay()
+        assert all(torch.equal(x, y) for x, y in zip(state(), again))
+        del held
+    assert all(torch.equal(x, y) for x, y in zip(again[:2], want[:2]))
+    step.check_status()

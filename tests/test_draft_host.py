@@ -236,3 +236,15 @@ def test_a_step_rotates_keys_of_its_segment_alone(step):
         with pytest.raises(ValueError):
             step.rotate(**bad)
     assert len(step.launched) == 2
+
+
+def test_a_step_keeps_the_key_of_layers_without_one(step):
+    """The zero key is one of the step's own buffers: steps of any size, on any stream and captured, read the same one."""
+    from rivoli_b200.draft import DraftTree
+    bf, keys = torch.bfloat16, []
+    for parents in ([[-1, 0], [-1]], [[-1], []], [[-1, 0, 1], [-1]]):
+        step.tree = DraftTree(parents, device="cpu")
+        step.layer(0, torch.zeros((4, 576), dtype=bf), None, torch.zeros((4, 2, 576), dtype=bf))
+        keys.append([a[2] for name, a in step.launched if name == "launch_kv_append_paged"][-1])
+    assert keys[0] is keys[1] is keys[2] and any(keys[0] is v for v in vars(step).values())
+    assert keys[0].shape == (4, 128) and keys[0].dtype == bf and not keys[0].any()
