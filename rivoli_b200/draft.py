@@ -150,9 +150,13 @@ class DraftStep:
         be.launch_kv_commit_paged(L.g, self.pools, len(self.stack.layers), L.block_table, self.tree_pos, self.path, MAX_NODES,
                                   self.n_path, self.tree.B, seq_len, self.status, stream)
 
-    def check_status(self) -> None:
-        """Raise if a kernel flagged an unmapped page, an unsound path or a wait that gave up since the last check (synchronises)."""
-        be.mla_tree_attend_status(self.stack.layers[0].g, self.scratch)
-        if int(self.status.item()):
-            self.status.zero_()
+    def check_status(self, stream=None) -> None:
+        """Raise if a kernel flagged an unmapped page, an unsound path or a wait that gave up since the last check, in the launches of
+        ``stream`` so far (synchronises it)."""
+        be.mla_tree_attend_status(self.stack.layers[0].g, self.scratch, stream)
+        with torch.cuda.stream(be.torch_stream(stream, self.status.device)):
+            flagged = int(self.status.item())
+            if flagged:
+                self.status.zero_()
+        if flagged:
             raise be.BackendError("draft_step(status)", 1005)

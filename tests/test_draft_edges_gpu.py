@@ -48,3 +48,23 @@ def test_a_captured_step_of_layers_without_a_key(be):
         del held
     assert all(torch.equal(x, y) for x, y in zip(again[:2], want[:2]))
     step.check_status()
+
+
+def test_the_status_of_another_stream(be):
+    """What a step on a stream of its own flags is seen by a check of that stream, however late the step runs, and is then gone."""
+    from rivoli_b200.draft import DraftStep, DraftTree
+    stack = make_stack(be, 2, 16, (True,))
+    stack.pool.reserve(0, 100)                    # the second sequence has no pages
+    stack.upload_block_table()
+    step, tree, pos = DraftStep(stack, 4), DraftTree([[-1, 0], [-1]], device=DEV), i32([10, 20])
+    latent, key, q = (torch.zeros(s, dtype=BF, device=DEV) for s in ((4, 576), (4, 128), (4, 16, 576)))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)            # some 50 ms
+    step.begin(tree, pos, side)
+    step.layer(0, latent, key, q, None, side)
+    with pytest.raises(be.BackendError):
+        step.check_status(side)
+    step.check_status(side)
+    step.check_status()
