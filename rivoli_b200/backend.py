@@ -719,11 +719,12 @@ ROPE_LAYOUTS = {"adjacent": 0, "half": 1, "split": 2}
 def rope_vecs(src, dst=None) -> tuple:
     """The fields of ``RopeVecs`` (include/rivoli_kernels.h) for tensors ``[rows, vectors, seg]`` or ``[rows, seg]`` whose last axis is
     contiguous: views of the rotated part of wider rows. ``dst`` None rotates in place."""
+    import torch
     dst = src if dst is None else dst
     if src.shape != dst.shape or src.dim() not in (2, 3):
         raise ValueError(f"rope_vecs: shapes {tuple(src.shape)} and {tuple(dst.shape)}")
-    if src.element_size() != 2 or dst.element_size() != 2 or src.stride(-1) != 1 or dst.stride(-1) != 1:
-        raise ValueError("rope_vecs: bf16 tensors with a contiguous last axis")
+    if src.dtype != torch.bfloat16 or dst.dtype != torch.bfloat16 or src.stride(-1) != 1 or dst.stride(-1) != 1:
+        raise ValueError(f"rope_vecs: {src.dtype}, {dst.dtype}; bf16 tensors with a contiguous last axis")
     if src.dim() == 2:
         return src, dst, src.stride(0), 0, dst.stride(0), 0, 1
     return src, dst, src.stride(0), src.stride(1), dst.stride(0), dst.stride(1), src.shape[1]
