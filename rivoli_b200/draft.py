@@ -112,13 +112,13 @@ class DraftStep:
         _fits("q", q, n, (g.n_heads, g.kv_lora + g.rope_dim), bf16)
         if index_key is not None:
             _fits("index_key", index_key, n, (g.index_dim,), bf16)
-        be.launch_kv_append_paged(L.g, latent, self.no_key if index_key is None else index_key, t.seq, self.row_pos, n, L.block_table,
-                                  L.latent_pool, L.latent_scale, L.index_pool, L.index_scale, self.status, stream)
         rows, counts = (None, None) if selection is None else selection
         if rows is not None:
-            if rows.dim() != 2 or rows.shape[0] < t.B or rows.element_size() != 4 or not rows.is_contiguous():
+            if rows.dim() != 2 or rows.shape[0] < t.B or rows.dtype not in (torch.int32, torch.uint32) or not rows.is_contiguous():
                 raise ValueError(f"selection: {tuple(rows.shape)} of {rows.dtype}; contiguous u32 of {t.B} sequences")
             _fits("selection's counts", counts, t.B, (), torch.int32)
+        be.launch_kv_append_paged(L.g, latent, self.no_key if index_key is None else index_key, t.seq, self.row_pos, n, L.block_table,
+                                  L.latent_pool, L.latent_scale, L.index_pool, L.index_scale, self.status, stream)
         be.launch_mla_tree_attend_paged_bf16(L.g, q, L.latent_pool, L.latent_scale, L.block_table, rows,
                                              0 if rows is None else rows.shape[1], counts, self.tree_pos, t.node_start, t.mask, t.B, n,
                                              self.out, self.lse, self.scratch, stream)

@@ -13,3 +13,18 @@ def test_rope_vecs_of_another_type(be):
         for bad in ((x.to(t),), (x, x.to(t)), (x.to(t), x)):
             with pytest.raises(ValueError):
                 be.rope_vecs(*bad)
+
+
+def test_a_selection_of_another_type(step):
+    """Rows are 32-bit integers, signed or not: f32 numbers would be read as row numbers by their bits. A step that is refused has not
+    written its rows either."""
+    bf = torch.bfloat16
+    args = torch.zeros((3, 576), dtype=bf), None, torch.zeros((3, 2, 576), dtype=bf)
+    rows, n = torch.zeros((2, 4), dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    for good in (rows, rows.view(torch.uint32)):
+        step.layer(0, *args, selection=(good, n))
+    launched = len(step.launched)
+    for bad in (rows.float(), rows.long(), rows.short()):
+        with pytest.raises(ValueError):
+            step.layer(0, *args, selection=(bad, n))
+    assert len(step.launched) == launched == 4
