@@ -633,11 +633,12 @@ int rivoli_draft_verify(const int32_t* node_start, const int32_t* parent, const 
 
 /* What was accepted becomes the sequence: the pool rows of positions tree_pos[b] + path[b][k], k < n_path[b] (at most path_stride), move
  * to positions tree_pos[b] + k, codes and scales of latents and indexer keys, in n_layers layers (a device array; index_pool NULL: a
- * layer without an indexer) that share block_table. seq_len (i32 [B], may be NULL, not tree_pos itself) receives tree_pos + n_path.
+ * layer without an indexer) that share block_table. seq_len (i32 [B], may be NULL; an array of its own, apart from those that are read)
+ * receives tree_pos + n_path.
  * The paths are what rivoli_draft_verify writes: strictly ascending, path[b][k] >= k. A sequence whose path is not, or whose rows lie
  * on unmapped pages, is left as it is, seq_len included, and raises bit 0 of *status (device i32, may be NULL). Rows behind the path
  * are left as they were. Sequences must not share the pages that their drafts lie on.
- * 1001 nulls or sizes; 1002 path_stride > 64; 1003-1004 geometry; 1005 alignment, seq_len == tree_pos. */
+ * 1001 nulls or sizes; 1002 path_stride > 64; 1003-1004 geometry; 1005 alignment, seq_len overlaps tree_pos, path, n_path or block_table. */
 typedef struct CommitLayer { uint8_t* latent_pool; float* latent_scale; uint8_t* index_pool; float* index_scale; } CommitLayer;
 int rivoli_kv_commit_paged(const DsaGeom* g, const CommitLayer* layers, int n_layers, const int32_t* block_table,
                            const int32_t* tree_pos, const int32_t* path, int path_stride, const int32_t* n_path, int B,

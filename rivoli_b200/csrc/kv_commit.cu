@@ -109,7 +109,12 @@ RIVOLI_API int rivoli_kv_commit_paged(const DsaGeom* g, const CommitLayer* layer
     if (int e = rv_check_geom(g)) return e;
     if (!layers || n_layers <= 0 || !block_table || !tree_pos || !path || path_stride <= 0 || !n_path || B <= 0) return 1001;
     if (path_stride > KC_MAX_PATH || B > 65535) return 1002;
-    if (((uintptr_t)layers & 7) || seq_len == tree_pos) return 1005;   // (blocks read tree_pos while one writes seq_len)
+    if ((uintptr_t)layers & 7) return 1005;
+    // blocks of all layers read these while one writes seq_len
+    auto shared = [&](const int32_t* p, size_t n) { return (uintptr_t)seq_len < (uintptr_t)(p + n) && (uintptr_t)p < (uintptr_t)(seq_len + B); };
+    if (seq_len && (shared(tree_pos, B) || shared(n_path, B) || shared(path, (size_t)B * path_stride) ||
+                    shared(block_table, (size_t)B * g->max_pages_per_seq)))
+        return 1005;
     CommitArgs a{*g, layers, n_layers, block_table, tree_pos, path, n_path, path_stride, seq_len, status};
     rv_drain_error();
     rv_launch_dependent(kv_commit_kernel, dim3((n_layers + KC_WARPS - 1) / KC_WARPS, B), dim3(KC_WARPS * 32), 0, (cudaStream_t)stream, a);

@@ -28,3 +28,17 @@ def test_a_selection_of_another_type(step):
         with pytest.raises(ValueError):
             step.layer(0, *args, selection=(bad, n))
     assert len(step.launched) == launched == 4
+
+
+def test_a_commit_whose_lengths_overlap_what_it_reads(be):
+    """The lengths are written while blocks of other layers still read positions, paths and pages."""
+    G, B, stride, far = be.DsaGeom.make(max_pages_per_seq=4, n_pool_pages=8), 3, 8, 1 << 30
+    sizes = dict(pos=4 * B, n=4 * B, path=4 * B * stride, table=4 * B * 4)
+
+    def code(seq_len, **at):
+        a = {name: far + i * 4096 for i, name in enumerate(sizes)} | at
+        return refused(be, be.launch_kv_commit_paged, G, P, 1, a["table"], a["pos"], a["path"], stride, a["n"], B, seq_len, None)
+
+    for name, size in sizes.items():
+        for off in (0, 4, size - 4, -4, -(4 * B - 4)):
+            assert code(P + off, **{name: P}) == 1005, (name, off)
