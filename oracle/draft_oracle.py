@@ -109,11 +109,10 @@ def commit(pools, table, page, n_pages, tree_pos, path):
     for k, j in enumerate(path):
         if j < k or j >= 64 or (k and j <= path[k - 1]):
             return False
-        if j != k:
-            src, dst = tree_rows(table, page, n_pages, 0, None, tree_pos + j, 1)[0], tree_rows(table, page, n_pages, 0, None, tree_pos + k, 1)[0]
-            if src < 0 or dst < 0:
-                return False
-            rows.append((src, dst))
+        src, dst = tree_rows(table, page, n_pages, 0, None, tree_pos + j, 1)[0], tree_rows(table, page, n_pages, 0, None, tree_pos + k, 1)[0]
+        if src < 0 or dst < 0:
+            return False
+        rows.append((src, dst))
     for a in pools:
         was = [a[s].copy() for s, _ in rows]
         for (_, d), w in zip(rows, was):

@@ -36,18 +36,15 @@ kv_commit_kernel(CommitArgs A) {
     if (tid < n) {
         const int node = A.path[(size_t)b * A.path_stride + tid];
         const int before = tid ? A.path[(size_t)b * A.path_stride + tid - 1] : -1;
-        long long src = -1, dst = -1;
-        if (node != tid || before != tid - 1) {
-            auto pool_row = [&](int t) -> long long {
-                const int lp = t / A.g.page_tokens;
-                const int pg = lp < A.g.max_pages_per_seq ? A.block_table[(size_t)b * A.g.max_pages_per_seq + lp] : -1;
-                return pg >= 0 && pg < A.g.n_pool_pages ? (long long)pg * A.g.page_tokens + t % A.g.page_tokens : -1;
-            };
-            const bool sound = node > before && node >= tid && node < KC_MAX_PATH && pos >= 0 && pos < 0x7fffffff - KC_MAX_PATH;
-            src = sound ? pool_row(pos + node) : -1;
-            dst = sound ? pool_row(pos + tid) : -1;
-            if (src < 0 || dst < 0) s_bad = 1;
-        }
+        auto pool_row = [&](int t) -> long long {
+            const int lp = t / A.g.page_tokens;
+            const int pg = lp < A.g.max_pages_per_seq ? A.block_table[(size_t)b * A.g.max_pages_per_seq + lp] : -1;
+            return pg >= 0 && pg < A.g.n_pool_pages ? (long long)pg * A.g.page_tokens + t % A.g.page_tokens : -1;
+        };
+        const bool sound = node > before && node >= tid && node < KC_MAX_PATH && pos >= 0 && pos < 0x7fffffff - KC_MAX_PATH;
+        long long src = sound ? pool_row(pos + node) : -1, dst = sound ? pool_row(pos + tid) : -1;
+        if (src < 0 || dst < 0) s_bad = 1;
+        if (node == tid) src = dst = -1;                      // it stays (and so do all before it)
         s_src[tid] = src; s_dst[tid] = dst;
     }
     __syncthreads();

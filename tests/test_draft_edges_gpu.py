@@ -1,7 +1,9 @@
 """The drafted step's operators on the GPU where they can go wrong: long flat tails, rows that are not there, buffers between steps."""
+import numpy as np
 import pytest
 import torch
 
+from oracle import draft_oracle as orc
 from tests.test_draft_gpu import BF, DEV, be, i32, make_stack  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -68,3 +70,28 @@ def test_the_status_of_another_stream(be):
         step.check_status(side)
     step.check_status(side)
     step.check_status()
+
+
+@pytest.mark.parametrize("page", [1, 4])
+def test_a_commit_whose_rows_are_not_mapped(be, page):
+    """Rows that stay where they are have to be there too: a sequence whose pages ran out, or whose position is none, keeps its length."""
+    pages = 24 // page
+    order = np.random.RandomState(page).permutation(8 * pages).astype(np.int32)
+    table = order[:6 * pages].reshape(6, pages).copy()
+    pos = [6, 6, 6, 6, -3, 6]
+    paths = [[0, 1, 2, 3], [0, 1, 2, 3], [0], [0, 5, 7], [0, 1], [0, 1]]
+    table[1, (6 + 3) // page] = -1                # the last of a chain
+    table[2, 6 // page] = 8 * pages               # a root alone, past the pool
+    table[3, 6 // page] = -1                      # a root that stays before rows that move between pages that are there
+    R = 8 * pages * page
+    pools = [np.random.RandomState(1).randint(0, 256, (R, 144)).astype(np.uint8), np.random.RandomState(2).rand(R).astype(np.float32)]
+    dev = [torch.from_numpy(a).to(DEV) for a in pools]
+    geom = be.DsaGeom.make(kv_lora=128, rope_dim=16, index_dim=16, page_tokens=page, max_pages_per_seq=pages, n_pool_pages=8 * pages)
+    status, seq_len = i32([0]), i32([-1] * 6)
+    arr = i32([p + [-5] * (8 - len(p)) for p in paths])
+    be.launch_kv_commit_paged(geom, be.commit_layers([(*dev, None, None)]), 1, torch.from_numpy(table).to(DEV), i32(pos), arr, 8,
+                              i32([len(p) for p in paths]), 6, seq_len, status)
+    sound = [orc.commit(pools, table[b], page, 8 * pages, pos[b], paths[b]) for b in range(6)]
+    assert sound == [True, False, False, False, False, True]
+    assert seq_len.tolist() == [10, -1, -1, -1, -1, 8] and status.item() == 1
+    assert all(np.array_equal(a, t.cpu().numpy()) for a, t in zip(pools, dev))
