@@ -83,6 +83,8 @@ class DraftStep:
         """``tree_pos`` i32 [B]: tokens of each sequence in the cache. The pages of ``tree_pos + nodes`` tokens have to be mapped."""
         if tree.B != self.tree_pos.shape[0] or tree.n_nodes > self.max_nodes:
             raise ValueError(f"{tree.B} trees of {tree.n_nodes} nodes; the step holds {self.tree_pos.shape[0]} of {self.max_nodes}")
+        if tree_pos.shape != self.tree_pos.shape or tree_pos.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"tree_pos: {tuple(tree_pos.shape)} of {tree_pos.dtype}; one integer per sequence")
         self.tree, n = tree, tree.n_nodes
         with torch.cuda.stream(be.torch_stream(stream, self.tree_pos.device)):
             self.tree_pos.copy_(tree_pos)

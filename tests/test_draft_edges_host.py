@@ -42,3 +42,12 @@ def test_a_commit_whose_lengths_overlap_what_it_reads(be):
     for name, size in sizes.items():
         for off in (0, 4, size - 4, -4, -(4 * B - 4)):
             assert code(P + off, **{name: P}) == 1005, (name, off)
+
+
+def test_a_step_begins_with_a_position_per_sequence(step):
+    """One position would be given to all sequences, and a fraction cut off."""
+    tree, was = step.tree, step.tree_pos.clone()
+    for bad in (torch.tensor([5], dtype=torch.int32), torch.tensor(5), torch.tensor([[5, 6]]), torch.tensor([5.5, 6.0]), torch.tensor([5, 6, 7])):
+        with pytest.raises(ValueError):
+            step.begin(tree, bad)
+    assert torch.equal(step.tree_pos, was) and step.tree is tree
