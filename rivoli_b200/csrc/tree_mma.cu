@@ -19,7 +19,8 @@
 // A pair of CTAs per block of 128 rows (cta_group::2, 1,105 cycles of products a tile against 1,400 here) was built and measured: 862 us
 // against 781 for 8 trees of up to 64 nodes x 16,384 rows alone, 982 against 900 back to back, where both are held by the power limit.
 // Rows of the tree are tested against each node's mask in the tiles that hold them, the last one or two of a sequence. A hidden row's
-// weight is 0, but 0 x NaN is NaN: NaN codes of tree rows are fetched as 0, and the row makes scores NaN where it is seen.
+// weight is 0, but 0 x NaN is NaN: NaN codes of tree rows are fetched as 0, and the row makes scores NaN where it is seen. Rows that
+// nobody sees, for want of a page or of a scale above zero, are fetched as zeros altogether.
 //
 // Shared memory: a ring of five tiles of 64 rows (36 KiB), the rope columns of q, P' twice, 16 KiB of staging. Tensor memory: S twice
 // (64 columns each), q (128: its latent columns are the A operand of the QK products), O^T (4 x 64). Warps: 0-7 softmax and epilogue in two
@@ -235,7 +236,8 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
         // Tiles of a row list, of smaller pages, and those that hold rows of the tree or end inside are gathered by all four warps
         // together, sixteen rows each: the copies go row by row with 32 lanes on 32 consecutive 16-byte chunks (one warp per tile took
         // 5,200 cycles to issue them, and a stage was held for that long more). No warp waits for its copies: they signal the stage
-        // themselves. Rows past the end and on unmapped pages are written as zeros.
+        // themselves. Rows past the end, on unmapped pages and without a scale above zero are written as zeros, in a tile of a tensor copy
+        // by that tile's warp alone.
         const int g = warp - TM_GW0, shift = rv_log2(A.page_tokens), inside = A.page_tokens - 1;
         constexpr uint32_t NONE = 0xffffffffu;
         bool ok = true;
@@ -269,31 +271,40 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
                     float scl1[2] = {0.0f, 0.0f};
                     if (y1 != NONE) { scl1[0] = A.pscale[y1 + lane]; scl1[1] = A.pscale[y1 + 32 + lane]; }
                     const int i = c0 + t - w.t0, s = i % NK, use = i / NK;
+                    uint32_t there[2], wild[2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const bool odd = !(scl[u] < INFINITY), live = y != NONE && !(scl[u] <= 0.0f);   // odd: NaN, or infinite
+                        there[u] = __ballot_sync(0xffffffffu, live);
+                        wild[u] = __ballot_sync(0xffffffffu, live && odd);
+                        scl[u] = !live ? 0.0f : odd ? 1.0f : scl[u];
+                    }
                     if (use > 0) ok = wait_for(&bars.k_empty[s], (use & 1) ^ 1, abort_flag, 41, max_polls);
                     if (!ok) break;
-                    const uint32_t at = tc::smem_u32(smem) + SM_K + s * KSTAGE;
-                    if (__builtin_expect(y == NONE, 0)) {          // a page that is not there: zeros
-#pragma unroll 1
-                        for (int o = lane * 16; o < KSTAGE; o += 512) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + o), "r"(0) : "memory");
-                        tc::fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_n(&bars.k_full[s], 1);
+                    uint8_t* kbuf = smem + SM_K + s * KSTAGE;
+                    const uint32_t at = tc::smem_u32(kbuf);
+                    uint32_t others = FULL - 1;
+                    if (__builtin_expect((there[0] & there[1]) != ~0u, 0)) {   // rows that are not there: row by row, those as zeros
+                        const uint8_t* row = A.pool + (y != NONE ? (size_t)y * TM_W : 0);
+                        auto live = [&](int r) -> bool { return ((r < 32 ? there[0] : there[1]) >> (r & 31)) & 1; };
+#pragma unroll 4
+                        for (int r = 0; r < TM_TILE; ++r)
+                            tc::cp_async16_zfill(at + (lane >> 3) * KCHUNK + tc::sw128_chunk(r, lane & 7), live(r) ? row + r * TM_W + lane * 16 : A.pool, live(r) ? 16u : 0u);
+#pragma unroll 2
+                        for (int r = lane >> 2; r < TM_TILE; r += 8)
+                            tc::cp_async16_zfill(at + 4 * KCHUNK + sw64_chunk(r, lane & 3), live(r) ? row + r * TM_W + TM_KVL + (lane & 3) * 16 : A.pool, live(r) ? 16u : 0u);
+                        tc::cp_async_mbar_arrive_noinc(&bars.k_full[s]);
+                        others = FULL - 32;
                     } else if (tc::elect_one()) {
                         tc::mbar_arrive_expect_tx(&bars.k_full[s], KSTAGE);
                         tma_load_3d(at, &k_map, (int)y, &bars.k_full[s]);
                         tc::tma_load_2d(at + 4 * KCHUNK, &r_map, TM_KVL, (int)y, &bars.k_full[s]);
                     }
-                    uint32_t there[2], wild[2];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const bool odd = !(scl[u] < INFINITY), live = y != NONE && !(scl[u] <= 0.0f);   // odd: NaN, or infinite
-                        s_tok[s * TM_TILE + u * 32 + lane] = !live ? 0.0f : odd ? 1.0f : scl[u];
-                        there[u] = __ballot_sync(0xffffffffu, live);
-                        wild[u] = __ballot_sync(0xffffffffu, live && odd);
-                    }
+                    for (int u = 0; u < 2; ++u) s_tok[s * TM_TILE + u * 32 + lane] = scl[u];
                     if (lane == 0) *reinterpret_cast<uint4*>(s_see + s * 8) = make_uint4(there[0], there[1], wild[0], wild[1]);
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_n(&bars.k_full[s], FULL - 1);
+                    if (lane == 0) mbar_arrive_n(&bars.k_full[s], others);
                     y = y1; scl[0] = scl1[0]; scl[1] = scl1[1];
                 }
             }
@@ -329,8 +340,8 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
                     if (!ok) break;
                     uint8_t* kbuf = smem + SM_K + s * KSTAGE;
                     uint8_t* rope = kbuf + 4 * KCHUNK;
-                    const uint32_t mine = k < 2 ? row[0] : row[1];
                     const float sc = k < 2 ? scl[0] : scl[1];
+                    const uint32_t mine = sc <= 0.0f ? NONE : k < 2 ? row[0] : row[1];   // (rows without a scale are nobody's)
 #pragma unroll 8
                     for (int it = 0; it < 16; ++it) {
                         const uint32_t r = __shfl_sync(0xffffffffu, mine, l0 + it);
@@ -371,7 +382,7 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
                     tc::cp_async_mbar_arrive_noinc(&bars.k_full[s]);
                     {
                         const bool here = (lane >> 4) == (k & 1);
-                        const bool odd = bad || !(sc < INFINITY), live = mine != NONE && !(sc <= 0.0f);        // odd: seen as NaN
+                        const bool odd = bad || !(sc < INFINITY), live = mine != NONE;                         // odd: seen as NaN
                         if (here) s_tok[s * TM_TILE + 16 * g + (lane & 15)] = !live ? 0.0f : odd ? 1.0f : sc;
                         const uint32_t there = __ballot_sync(0xffffffffu, live), wild = __ballot_sync(0xffffffffu, live && odd);
                         if (lane == 0) { s_see[s * 8 + g] = (uint16_t)(there >> l0); s_see[s * 8 + 4 + g] = (uint16_t)(wild >> l0); }

@@ -1,10 +1,12 @@
 """The drafted step's operators on the GPU where they can go wrong: long flat tails, rows that are not there, buffers between steps."""
+import random
+
 import numpy as np
 import pytest
 import torch
 
 from oracle import draft_oracle as orc
-from tests.test_draft_gpu import BF, DEV, be, i32, make_stack  # noqa: F401
+from tests.test_draft_gpu import BF, DEV, Cache, be, i32, make_stack, masks_of, signed  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -95,3 +97,47 @@ def test_a_commit_whose_rows_are_not_mapped(be, page):
     assert sound == [True, False, False, False, False, True]
     assert seq_len.tolist() == [10, -1, -1, -1, -1, 8] and status.item() == 1
     assert all(np.array_equal(a, t.cpu().numpy()) for a, t in zip(pools, dev))
+
+
+@pytest.mark.parametrize("listed", [False, True])
+@pytest.mark.parametrize("kvl, page", [(512, 64), (512, 128), (512, 16), (256, 64)])
+def test_what_a_row_without_a_scale_holds_does_not_matter(be, kvl, page, listed):
+    """NaN codes in rows whose scale is zero or below, anywhere in the prefix and in the tree: the bits that zeros in their place give,
+    and what the definition gives without the rows. Tiles of nothing else are among them."""
+    host, H, W, n, T = random.Random(page + kvl), 24, kvl + 64, [700, 200], [5, 2]
+    cache = Cache(51, [a + b for a, b in zip(n, T)], page, kvl, spread=0.3)
+    masks = [m for t in T for m in masks_of(host, t, "tree")]
+    lists = [sorted(host.sample(range(m), 150)) for m in n]
+    at = [orc.tree_rows(cache.table[b], page, cache.n_pages, 150 if listed else n[b], lists[b] if listed else None, n[b], T[b]) for b in range(2)]
+    codes = np.zeros_like(cache.codes)
+    for b in range(2):
+        dead = set(host.sample(range(len(at[b])), 40)) | ({len(at[b]) - 2} if b == 0 else set()) | (set(range(64, 128)) if b == 0 else set())
+        for j in dead:
+            cache.scale[at[b][j]] = host.choice((0.0, -1.0))
+            codes[at[b][j]] = host.choice((0x7f, 0xff))
+            at[b][j] = -1
+    nobody = cache.scale <= 0
+    cache.codes[nobody] = 0
+    g = be.DsaGeom.make(n_heads=H, kv_lora=kvl, page_tokens=page, max_pages_per_seq=cache.table.shape[1], n_pool_pages=cache.n_pages)
+    q = torch.randn((7, H, W), generator=torch.Generator().manual_seed(1)).to(BF)
+    pool, scale, table = cache.dev()
+    sc = torch.zeros(be.mla_tree_attend_scratch_bytes(g, 2, 7), dtype=torch.uint8, device=DEV)
+    got = []
+    for fill in (False, True):
+        if fill:
+            rows = torch.from_numpy(nobody).to(DEV)
+            pool[rows] = torch.from_numpy(codes).to(DEV)[rows]
+        out, lse = torch.zeros((7, H, kvl), dtype=BF, device=DEV), torch.zeros((7, H), device=DEV)
+        be.launch_mla_tree_attend_paged_bf16(g, q.to(DEV), pool, scale, table, i32(lists) if listed else None, 150 if listed else 0,
+                                             i32([150, 150]) if listed else None, i32(n), i32([0, 5, 7]), signed(masks), 2, 7, out, lse, sc)
+        got.append((out, lse))
+    be.mla_tree_attend_status(g, sc)
+    assert (pool == 0x7f).any() and (pool == 0xff).any()
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    for b, (a, z) in enumerate(((0, 5), (5, 7))):
+        want, want_lse = orc.tree_attend(q[a:z].double().numpy(), cache.codes, cache.scale, at[b], 150 if listed else n[b], masks[a:z],
+                                         float(np.float32(g.softmax_scale)), kvl)[:2]
+        off = got[1][0][a:z].double().cpu().numpy() - want
+        # the result's own rounding and the weights' are 2^-8 each at most
+        assert np.linalg.norm(off) <= 2.0 ** -7 * np.linalg.norm(want)
+        assert np.abs(got[1][1][a:z].double().cpu().numpy() - want_lse).max() <= 2.0 ** -12
