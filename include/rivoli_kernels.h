@@ -604,7 +604,9 @@ int rivoli_rope_rows_bf16(const RopeVecs* q, const RopeVecs* k, int n_rows, cons
  * gets zeros and -inf. Rows on unmapped pages, and rows of a scale of zero or below, are seen by nobody. Outputs of nodes from node_start[B] on, and of a sequence's nodes
  * behind its 64th, are left as they were. scratch = rivoli_mla_tree_attend_scratch_bytes(), zeroed once (it begins with a sticky error
  * word); calls that may run at the same time need one each. kv_lora 512 with rope_dim 64 runs on the tensor cores for any number of
- * heads (given scratch), other geometries on CUDA cores. Which rows share a block goes by the whole call, so that the last bits of a
+ * heads (given scratch), other geometries on CUDA cores. On the tensor cores a weight is off by
+ * 2^-9 of itself, or by 2^-15 of a larger one that it lies far below; a long prefix that lies there whole is kept, but for some 2^-11 of
+ * all of a node's weights. Which rows share a block goes by the whole call, so that the last bits of a
  * node's output may differ between batches; the same call gives the same bits.
  * 1001 nulls or sizes; 1002 n_nodes * n_heads or the pool too large; 1003-1004 geometry; 1005 alignment. */
 size_t rivoli_mla_tree_attend_scratch_bytes(const DsaGeom* g, int B, int n_nodes);

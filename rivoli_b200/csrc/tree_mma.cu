@@ -4,8 +4,9 @@
 //
 // The arithmetic is that of the decode step's attention (attend_mma.cu): cache rows are consumed as the e4m3 codes they are, q is two e4m3
 // terms (here to a power of two, which loses none of its bits: the scores are those of the bf16 queries), the softmax weights are two
-// each (2^-8 relative), a row's scale rides in its weight (P' = weight * scale * 2^5), references
-// lag behind the running maximum by at most 2^3, sums are f32. What differs is the shape of the work. The nodes of a tree share their
+// each (2^-9 relative down to 2^-7 of the reference, 2^-10 * 2^-5 of it below), a row's scale rides in its weight (P' = weight * scale *
+// 2^5), references lag behind the running maximum by at most 2^3, sums are f32. What differs, beside references that come down again where
+// a long prefix would vanish under them (TM_LOW), is the shape of the work. The nodes of a tree share their
 // prefix, so that the rows of a sequence are nodes x heads, 64 to a block, and one tile of 64 cache rows serves them all: 240 products and
 // more per byte from a single node on and sixteen times that at sixteen nodes. The kernel is bound by the tensor cores and what feeds
 // them, the cache's tiles come from L2, and what has to be even is the number of (row block, tile) pairs per SM:
@@ -40,6 +41,16 @@ constexpr int NK = 5, NG = 2, GW = 4;                // stages; softmax groups, 
 constexpr int TM_SW = 4 * NG, TM_QKW = TM_SW, TM_PVW = TM_SW + 1, TM_GW0 = TM_SW + 2;
 constexpr int TM_THREADS = (TM_GW0 + GW) * 32, TM_SOFTMAX = TM_SW * 32, TM_GROUP = 128;
 constexpr float TM_POFF = 5.0f, TM_MOST = 256.0f;    // P' = 2^(s - ref + 5) <= 2^8: references lag by 2^3 at most, see attend_mma.cu
+// P' below 2^-10 comes to nothing in both terms, and is off by up to 2^-10 above. Behind a row that has most of the weight the whole of a
+// long prefix would lie there, so references come down, too. What the terms leave of a tile's P' is added up, sign in it. Where that is
+// more than TM_FEW of a thread's largest P', in a tile that is all prefix, the row's own sum goes to its account, and the row's largest
+// against it; above TM_LOST of those the reference of a row whose P' here are below TM_LOW comes down until its largest is 2^(5 - TM_SPARE),
+// and the sums go up with it (f32: no further than TM_ROOM above the account, nor from below 2^TM_LOWEST, so that none overflows). So
+// rounding takes 2^-7 of a row's weights at most, whatever their levels and the length, beside 2^-15 of a larger one for each of the 63
+// that share its tile. With references that only rise, 65,536 equal rows behind one with half of the weight left 0.4 of the output's
+// norm missing. Keeping the account costs 5 % of the time (32 trees over 512 to 8,192 rows 256 us, 244 without), where scores deviate by
+// two and three nats, so that references often move, 14 and 47 %.
+constexpr float TM_FEW = 1.0f / 128, TM_LOST = 1.0f / 2048, TM_LOW = 2.0f, TM_LOW_AT = -6.0f, TM_SPARE = 2.0f, TM_ROOM = 35.0f, TM_LOWEST = -64.0f;
 constexpr int TM_MIN_TILES = 4;                      // tiles a CTA takes at least, while there are few: a CTA per block, or as many as that leaves
 // What a row block costs beside its tiles, in tiles: its queries, its output and the pipeline's ramp take 26,000 cycles, a tile 1,650. A
 // run pays it for each block that it touches; the first is the same for all runs, so that the blocks that begin inside a run count
@@ -63,7 +74,8 @@ constexpr int SM_AHI = SM_SEE + NK * 16;                    // f32 [64] query sc
 constexpr int SM_WMAX = SM_AHI + 256;                       // f32 [NG][64]
 constexpr int SM_FAC = SM_WMAX + NG * 256;                  // f32 [64]
 constexpr int SM_MREF = SM_FAC + 256;                       // f32 [64]
-constexpr int SM_BARS = SM_MREF + 256;
+constexpr int SM_ACCT = SM_MREF + 256;                      // float2 [64]: a row's account, see TM_LOW
+constexpr int SM_BARS = SM_ACCT + 512;
 constexpr int SM_MISC = SM_BARS + 256;
 constexpr int SM_TOTAL = SM_MISC + 64;
 static_assert(SM_TOTAL <= 232448, "shared memory budget");
@@ -162,6 +174,7 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
     float* s_wmax = reinterpret_cast<float*>(smem + SM_WMAX);
     float* s_fac = reinterpret_cast<float*>(smem + SM_FAC);
     float* s_mref = reinterpret_cast<float*>(smem + SM_MREF);
+    float2* s_acct = reinterpret_cast<float2*>(smem + SM_ACCT);
     uint32_t* tmem_base_s = reinterpret_cast<uint32_t*>(smem + SM_MISC);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + SM_MISC + 4);
     int* s_run = reinterpret_cast<int*>(smem + SM_MISC + 8);               // b, rb, t0 of the run's beginning, number of runs, a block's own cost
@@ -561,7 +574,7 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
                     const float amax = fmaxf(s_wmax[r], s_wmax[64 + r]);
                     return amax > 0.0f ? fmaxf(__uint_as_float((__float_as_uint(amax / 448.0f) + 0x007fffffu) & 0xff800000u), 1.17549435e-38f) : 1.0f;
                 };
-                if (th == 0 && tb == 0) { s_ahi[hd] = scale_of(hd) * A.softmax_scale * 1.4426950408889634f; s_mref[hd] = -INFINITY; }
+                if (th == 0 && tb == 0) { s_ahi[hd] = scale_of(hd) * A.softmax_scale * 1.4426950408889634f; s_mref[hd] = -INFINITY; s_acct[hd] = make_float2(0.0f, 0.0f); }
                 auto codes8 = [&](const uint4 x, float inv, uint2& hi, uint2& lo) {
                     const uint32_t ww[4] = {x.x, x.y, x.z, x.w};
                     uint16_t ch[4], cl[4];
@@ -686,7 +699,7 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
                     // P' = 2^(x - ref + 5) * scale as two e4m3 terms (through f16); the sums take 2^(x - ref + 5)
                     const float ka = m_a == -INFINITY ? 0.0f : TM_POFF - m_a, kb = m_b == -INFINITY ? 0.0f : TM_POFF - m_b;
                     f2 la = 0ull, lb = 0ull;
-                    __half2 top = __float2half2_rn(0.0f);
+                    __half2 top[2] = {__float2half2_rn(0.0f), __float2half2_rn(0.0f)}, gone[2] = {top[0], top[1]};   // of rows a and b: the largest P', and what the terms leave of them
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         const volatile f2* cv = sc;
@@ -702,7 +715,7 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
                             if (r) lb = add2(lb, ww); else la = add2(la, ww);
                             const float2 p = unpack(mul2(ww, c8));
                             const __half2 ph = __floats2half2_rn(p.x, p.y);
-                            top = __hmax2(top, ph);
+                            top[r] = __hmax2(top[r], ph);
                             const uint32_t phb = *reinterpret_cast<const uint32_t*>(&ph);
                             uint16_t c, d;
                             uint32_t back;
@@ -710,6 +723,8 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
                             asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(c));
                             const __half2 rest = __hsub2(ph, *reinterpret_cast<const __half2*>(&back));
                             asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(d) : "r"(*reinterpret_cast<const uint32_t*>(&rest)));
+                            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(d));
+                            gone[r] = __hadd2(gone[r], __hsub2(rest, *reinterpret_cast<const __half2*>(&back)));
                             ch[r] = c; cl[r] = d;
                         }
                         hi_w[k] = ch[0] | (ch[1] << 16);
@@ -727,11 +742,42 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
                         if (nb != m_b) { l_b *= exp2f(m_b - nb); m_b = nb; }
                     }
                     // They stand as long as no P' exceeds 2^(5 + 3) by them (one barrier with an OR). One that has moved meanwhile brings the
-                    // P' of before down with it; rows that have none yet are looked at.
-                    const float2 t2 = __half22float2(top);
-                    float most = fmaxf(t2.x, t2.y);
-                    if (m_a != was_a || m_b != was_b) most *= fmaxf(exp2f(was_a - m_a), exp2f(was_b - m_b));
-                    const bool grown = most > TM_MOST || was_a == -INFINITY || was_b == -INFINITY;
+                    // P' of before along. Rows that have none yet are looked at, too.
+                    __half2 t = __hmax2(__lows2half2(top[0], top[1]), __highs2half2(top[0], top[1]));
+                    __half2 g = __hadd2(__lows2half2(gone[0], gone[1]), __highs2half2(gone[0], gone[1]));
+                    if (m_a != was_a || m_b != was_b) {
+                        const float2 t2 = __half22float2(t), g2 = __half22float2(g);
+                        const float fa = exp2f(was_a - m_a), fb = exp2f(was_b - m_b);
+                        t = __floats2half2_rn(t2.x * fa, t2.y * fb);
+                        g = __floats2half2_rn(g2.x * fa, g2.y * fb);
+                    }
+                    const bool inside = j0 + TM_TILE <= w.s.n;
+                    bool down_a = false, down_b = false;
+                    if (__builtin_expect(__any_sync(0xffffffffu, inside && !__hble2(__habs2(g), __hmul2(t, __float2half2_rn(TM_FEW))) && i > i0), 0)) {
+                        // (where a group's first tile is all small, its reference comes down below)
+#pragma unroll
+                        for (int o = 1; o < 4; o <<= 1) {
+                            t = __hmax2(t, __shfl_xor_sync(0xffffffffu, t, o));
+                            g = __hadd2(g, __shfl_xor_sync(0xffffffffu, g, o));
+                        }
+                        auto look = [&](float most, float took, float was, int row) -> bool {
+                            float2 c = s_acct[row];
+                            bool down = false;
+                            if (most < TM_LOW && was > -INFINITY && fabsf(took) > TM_FEW * most && took - took == 0.0f) {
+                                c.y += took;
+                                down = fabsf(c.y) > TM_LOST * (c.x + most);
+                                if (down) c.y = 0.0f;
+                            }
+                            c.x += most;
+                            __syncwarp();
+                            if (tq == 0) s_acct[row] = c;
+                            return down;
+                        };
+                        const float2 most = __half22float2(t), took = __half22float2(g);
+                        down_a = look(most.x, took.x, was_a, ra);
+                        down_b = look(most.y, took.y, was_b, rb);
+                    }
+                    const bool grown = !__hble2(t, __float2half2_rn(TM_MOST)) || was_a == -INFINITY || was_b == -INFINITY || down_a || down_b;
                     if (__builtin_expect(tc::barrier_any(6 + th, TM_GROUP, grown || !ok), 0)) {
                         // the largest x + log2(scale) of a row is what P' goes by (scales below 2^-100 as that: their weights would
                         // pass 2^127)
@@ -744,17 +790,25 @@ tree_mma_kernel(TreeArgs A, const __grid_constant__ CUtensorMap k_map, const __g
                         }
 #pragma unroll
                         for (int o = 1; o < 4; o <<= 1) { ta = fmaxf(ta, __shfl_xor_sync(0xffffffffu, ta, o)); tb2 = fmaxf(tb2, __shfl_xor_sync(0xffffffffu, tb2, o)); }
-                        // all references take all of their growth (taken by those alone that had to, the next tile's row would have to)
-                        auto move = [](float& m, float top_now) -> float {
+                        // all references take all of their growth (taken by those alone that had to, the next tile's row would have to), and
+                        // come down where the account says so
+                        auto move = [&](float& m, float was, float t_now, bool down, int row) -> float {
+                            float2 c = s_acct[row];
+                            down |= was == -INFINITY && inside && t_now < m + TM_LOW_AT;
                             float f = 1.0f;
-                            if (m == -INFINITY) { if (top_now > -INFINITY) m = top_now; }
-                            else if (top_now > m) { f = exp2f(m - top_now); m = top_now; }
+                            if (t_now > -INFINITY) {
+                                const float to = fmaxf(t_now + (down ? TM_SPARE : 0.0f), m - (down && m > TM_LOWEST ? fmaxf(TM_ROOM - __log2f(c.x), 0.0f) : 0.0f));
+                                if (m > -INFINITY) f = exp2f(m - to);
+                                m = to;
+                                c.x = c.x * f + exp2f(t_now - m + TM_POFF);
+                            }
+                            __syncwarp();
+                            if (tq == 0) { s_fac[row] = f; s_mref[row] = m; s_acct[row] = make_float2(c.x, c.y * f); }
                             return f;
                         };
-                        const float fa = move(m_a, ta), fb = move(m_b, tb2);
-                        if (tq == 0) { s_fac[ra] = fa; s_mref[ra] = m_a; s_fac[rb] = fb; s_mref[rb] = m_b; }
+                        const float fa = move(m_a, was_a, ta, down_a, ra), fb = move(m_b, was_b, tb2, down_b, rb);
                         left = tc::barrier_any(9 + th, TM_GROUP, !ok);
-                        if (!left && i > i0) {                     // O^T to the new references
+                        if (!left && i > i0 && __any_sync(0xffffffffu, s_fac[lane] != 1.0f || s_fac[32 + lane] != 1.0f)) {   // O^T to the new references
                             if (i >= i0 + NG) ok = pv_done(i - NG);
                             if (ok) ok = pv_done(i - 1);
                             tc::tc_fence_after();
