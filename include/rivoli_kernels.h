@@ -599,7 +599,9 @@ int rivoli_rope_rows_bf16(const RopeVecs* q, const RopeVecs* k, int n_rows, cons
 /* Attention of all nodes of all trees: q bf16 [n_nodes][n_heads][kv_lora + rope_dim], out bf16 [n_nodes][n_heads][kv_lora], out_lse
  * f32 [n_nodes][n_heads] (may be NULL). A node of sequence b sees n_rows[b] rows of the prefix - rows u32 [B][row_stride], one list for
  * the whole tree (its root's selection, say), or with rows NULL the first n_rows[b] tokens, n_rows NULL meaning tree_pos[b] of them;
- * a list that begins with the dense marker 0xFFFFFFFF stands for the first n_rows[b] tokens - and node i of its own tree, whose row is
+ * a list that begins with the dense marker 0xFFFFFFFF stands for the first n_rows[b] tokens; what either names from tree_pos[b] on is of
+ * the tree and not of the prefix, and is left out, so that the selection of the root may be made before or after its row is appended -
+ * and node i of its own tree, whose row is
  * token tree_pos[b] + i, where bit i of node_mask (u64 [n_nodes]) is up: for a tree its ancestors and itself. A node that sees nothing
  * gets zeros and -inf. Rows on unmapped pages, and rows of a scale of zero or below, are seen by nobody. Outputs of nodes from node_start[B] on, and of a sequence's nodes
  * behind its 64th, are left as they were. scratch = rivoli_mla_tree_attend_scratch_bytes(), zeroed once (it begins with a sticky error

@@ -22,16 +22,21 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& A, int b) {
     s.node0 = max(0, A.node_start[b]);
     s.T = max(0, min(min(A.node_start[b + 1], A.n_nodes) - s.node0, TREE_NODES));
     s.pos = A.tree_pos[b];
-    // a row list whose first entry is the dense marker stands for "row j = token j" over the first n_rows tokens
+    // A row list whose first entry is the dense marker stands for "row j = token j" over the first n_rows tokens. The prefix ends where
+    // the tree begins: a selection that was made once the root's row was there may name it, and may count it.
     s.listed = A.rows && A.rows[(size_t)b * A.row_stride] != 0xffffffffu;
-    const long long cap = s.listed ? A.row_stride : (long long)A.max_pages * A.page_tokens;
+    const long long cap = s.listed ? A.row_stride : min((long long)s.pos, (long long)A.max_pages * A.page_tokens);
     s.n = (int)max(0LL, min(min((long long)(A.n_rows ? A.n_rows[b] : s.pos), cap), 0x7fffff00LL));
     return s;
 }
 
-// Pool row of entry j of sequence b (j < n: the prefix, from n on the tree); 0xffffffff: unmapped, attended by nobody.
+// Token of entry j of sequence b (j < n: the prefix, from n on the tree) and its pool row; 0xffffffff: none, attended by nobody.
 __device__ __forceinline__ uint32_t tree_token(const TreeArgs& A, const TreeSeq& s, int b, int j) {
-    if (j < s.n) return s.listed ? A.rows[(size_t)b * A.row_stride + j] : (uint32_t)j;
+    if (j < s.n) {
+        if (!s.listed) return (uint32_t)j;
+        const uint32_t t = A.rows[(size_t)b * A.row_stride + j];
+        return (int)t >= 0 && (int)t < s.pos ? t : 0xffffffffu;
+    }
     return (uint32_t)s.pos + (uint32_t)(j - s.n);
 }
 __device__ __forceinline__ uint32_t tree_pool_row(const TreeArgs& A, int b, uint32_t token) {

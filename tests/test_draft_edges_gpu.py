@@ -280,3 +280,42 @@ def test_levels_that_rise_and_fall(be, listed):
         assert out[j].isfinite().all()
         assert ((out[j].double() - want).abs() <= tol).all(), ((out[j].double() - want).abs() / tol).max()
         assert ((lse[j].double() - lse_j).abs() <= 2.0 ** -14 + 2.0 ** -20 * lse_j.abs()).all()
+
+
+@pytest.mark.parametrize("kvl, page", [(512, 64), (512, 16), (256, 64)])
+def test_a_selection_that_names_the_tree(be, kvl, page):
+    """The root's selection, made once its row was appended, names that row or counts it: the node sees it once. So with any row from the
+    tree's first on, and with no position at all."""
+    host, H, n, T = random.Random(61), 16, [300, 90, 200, 128, 40], [3, 2, 4, 1, 2]
+    cache = Cache(61, [a + b for a, b in zip(n, T)], page, kvl)
+    masks = [m for t in T for m in masks_of(host, t, "tree")]
+    k = 160
+    rows = [sorted(host.sample(range(m), min(m, k - 4))) for m in n]
+    own = [r + [m, m + 1, m + t - 1, 0x80000000 + m][:k - len(r)] for r, m, t in zip(rows, n, T)]
+    own = [r + [0] * (k - len(r)) for r in own]
+    own[1], own[4] = [0xffffffff] + [0] * (k - 1), [0xffffffff] + [0] * (k - 1)
+    counts = [len(r) + 4 for r in rows]
+    counts[1], counts[4] = n[1] + 1, 1000                          # dense, with the root counted, and with all that is mapped
+    g = be.DsaGeom.make(n_heads=H, kv_lora=kvl, page_tokens=page, max_pages_per_seq=cache.table.shape[1], n_pool_pages=cache.n_pages)
+    q = torch.randn((sum(T), H, kvl + 64), generator=torch.Generator().manual_seed(1)).to(BF).to(DEV)
+    start = np.concatenate(([0], np.cumsum(T))).tolist()
+    pool, scale, table = cache.dev()
+    sc = torch.zeros(be.mla_tree_attend_scratch_bytes(g, 5, sum(T)), dtype=torch.uint8, device=DEV)
+    got = []
+    plain = [r + [0] * (k - len(r)) for r in rows]
+    plain[1], plain[4] = own[1], own[4]
+    for lists, c in ((plain, [len(rows[0]), n[1], len(rows[2]), len(rows[3]), n[4]]), (own, counts)):
+        out, lse = torch.zeros((sum(T), H, kvl), dtype=BF, device=DEV), torch.zeros((sum(T), H), device=DEV)
+        r = i32([[v - (1 << 32) if v >> 31 else v for v in row] for row in lists])
+        be.launch_mla_tree_attend_paged_bf16(g, q, pool, scale, table, r, k, i32(c), i32(n), i32(start), signed(masks), 5, sum(T), out, lse, sc)
+        got.append((out, lse))
+    be.mla_tree_attend_status(g, sc)
+    # the same rows, but for zeros between them, which shift them to other tiles: sums in another order, weights in other units
+    for b in range(5):
+        a, z = start[b], start[b + 1]
+        x, y = (o[0][a:z].double() for o in got)
+        assert (x - y).norm() <= 2.0 ** -8 * x.norm(), b
+        assert (got[0][1][a:z] - got[1][1][a:z]).abs().max() <= 2.0 ** -14, b
+    nobody = torch.zeros_like(got[0][0]), torch.zeros_like(got[0][1])
+    be.launch_mla_tree_attend_paged_bf16(g, q, pool, scale, table, r, k, i32(counts), i32([-5] * 5), i32(start), signed(masks), 5, sum(T), *nobody, sc)
+    assert (nobody[0] == 0).all() and (nobody[1] == -math.inf).all()
