@@ -586,7 +586,8 @@ int rivoli_v4_select_status(void* stream);
  * rivoli_rope_interleave (crates/backend/kernels/activation.hip:362-371). Strides in elements, any sign. dst may be src with the same
  * strides (in place); otherwise the two must not overlap. k may be NULL. Segments of a multiple of 16 values whose bases and strides
  * are multiples of 16 bytes are read and written 16 bytes at a time.
- * 1001 nulls or sizes; 1002 seg > 512 or n_vec > 65536; 1003 layout; 1004 odd seg; 1005 odd addresses. */
+ * 1001 nulls or sizes; 1002 seg > 512 or n_vec > 65536; 1003 layout; 1004 odd seg; 1005 odd addresses, segments written on one another
+ * (strides of dst below seg). */
 enum { RV_ROPE_ADJACENT = 0, RV_ROPE_HALF = 1, RV_ROPE_SPLIT = 2 };
 typedef struct RopeVecs {                  /* vectors of a row: where their segments are read and written */
     const uint16_t* src; uint16_t* dst;

@@ -148,6 +148,11 @@ rope_rows_kernel(RopeArgs A) {
     }
 }
 
+// Segments that are written must not lie on one another: vectors of a row, and rows.
+bool apart(const RopeVecs& w, int n_rows, int seg) {
+    auto near = [&](int64_t stride) { return stride > -seg && stride < seg; };
+    return !(w.n_vec > 1 && near(w.dst_vec)) && !(n_rows > 1 && near(w.dst_row));
+}
 bool aligned16(const RopeVecs& w) {
     return ((((uintptr_t)w.src | (uintptr_t)w.dst) & 15) | ((w.src_row | w.src_vec | w.dst_row | w.dst_vec) & 7)) == 0;
 }
@@ -162,6 +167,7 @@ RIVOLI_API int rivoli_rope_rows_bf16(const RopeVecs* q, const RopeVecs* k, int n
     if (layout < RV_ROPE_ADJACENT || layout > RV_ROPE_SPLIT) return 1003;
     if (seg % 2) return 1004;
     if (((uintptr_t)q->src | (uintptr_t)q->dst | (k ? (uintptr_t)k->src | (uintptr_t)k->dst : 0)) & 1) return 1005;
+    if (!apart(*q, n_rows, seg) || (k && !apart(*k, n_rows, seg))) return 1005;
     RopeArgs a{*q, k ? *k : RopeVecs{}, n_rows, 1, seg, layout, pos, inv_freq, scale};
     const bool vec = seg % 16 == 0 && aligned16(*q) && (!k || aligned16(*k));
     const int n_vec = a.q.n_vec + a.k.n_vec;

@@ -51,3 +51,17 @@ def test_a_step_begins_with_a_position_per_sequence(step):
         with pytest.raises(ValueError):
             step.begin(tree, bad)
     assert torch.equal(step.tree_pos, was) and step.tree is tree
+
+
+def test_rope_segments_written_on_one_another(be):
+    """One vector that stands for several is read for each, but not rotated in place once for each, by warps that do not wait for one
+    another. (One row, or one vector, may have any stride.)"""
+    def code(q, k=None, n=2):
+        return refused(be, be.launch_rope_rows_bf16, q, k, n, P, P, 64, 0, 1.0)
+    fine = (P, P, 128, 64, 128, 64, 2)
+    for bad in ((P, P, 64, 0, 64, 0, 4), (P, P, 0, 64, 0, 64, 4), (P, P, 256, 64, 256, 32, 4), (P, P, 256, 64, 256, -63, 4), (P, P, 64, 64, 63, 64, 1)):
+        assert code(bad) == 1005 and code(fine, bad) == 1005, bad
+    x = torch.zeros((2, 64), dtype=torch.bfloat16)
+    y = x[:, None].expand(2, 4, 64)
+    with pytest.raises(be.BackendError):
+        be.launch_rope_rows_bf16(be.rope_vecs(y), None, 2, P, P, 64, 0)
