@@ -75,7 +75,7 @@ class DraftStep:
         self.no_key = torch.zeros((max_nodes, g.index_dim), dtype=torch.bfloat16, device=d)   # for layers without an indexer
         self.status = torch.zeros(1, dtype=torch.int32, device=d)
         self.layout = be.ROPE_LAYOUTS[layout]
-        self.inv_freq = None if rope is None else torch.from_numpy(rope[0]).to(d)
+        self.inv_freq = None if rope is None else torch.as_tensor(rope[0], dtype=torch.float64, device=d).contiguous()
         self.rope_scale = 1.0 if rope is None else rope[1]
         self.tree = None
 

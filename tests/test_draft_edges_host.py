@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.test_draft_host import P, be, refused, step  # noqa: F401
+from tests.test_draft_host import P, Stack, be, refused, step  # noqa: F401
 
 
 def test_rope_vecs_of_another_type(be):
@@ -65,3 +65,13 @@ def test_rope_segments_written_on_one_another(be):
     y = x[:, None].expand(2, 4, 64)
     with pytest.raises(be.BackendError):
         be.launch_rope_rows_bf16(be.rope_vecs(y), None, 2, P, P, 64, 0)
+
+
+def test_a_step_keeps_its_frequencies_in_64_bits(be):
+    """Whatever they were given in: the kernel reads eight bytes for each."""
+    from rivoli_b200.draft import DraftStep
+    f, scale = be.rope_frequencies(64)
+    for given in (f, f.astype("f4"), f.tolist(), torch.from_numpy(f), f.repeat(2)[::2]):
+        s = DraftStep(Stack(be), 4, (given, scale))
+        assert s.inv_freq.dtype == torch.float64 and s.inv_freq.shape == (32,) and s.inv_freq.is_contiguous()
+        assert torch.allclose(s.inv_freq, torch.from_numpy(f), rtol=1e-6)
