@@ -17,6 +17,7 @@ built, importing a launcher fails loudly.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -716,18 +717,24 @@ def launch_v4_compress_step_bf16(p: CompGeom, n_seqs: int, pos, kv_proj, score_p
 ROPE_LAYOUTS = {"adjacent": 0, "half": 1, "split": 2}
 
 
+@functools.cache
+def _bf16():
+    import torch
+    return torch.bfloat16
+
+
 def rope_vecs(src, dst=None) -> tuple:
     """The fields of ``RopeVecs`` (include/rivoli_kernels.h) for tensors ``[rows, vectors, seg]`` or ``[rows, seg]`` whose last axis is
     contiguous: views of the rotated part of wider rows. ``dst`` None rotates in place."""
-    import torch
     dst = src if dst is None else dst
-    if src.shape != dst.shape or src.dim() not in (2, 3):
-        raise ValueError(f"rope_vecs: shapes {tuple(src.shape)} and {tuple(dst.shape)}")
-    if src.dtype != torch.bfloat16 or dst.dtype != torch.bfloat16 or src.stride(-1) != 1 or dst.stride(-1) != 1:
+    shape, a, b, bf16 = src.shape, src.stride(), dst.stride(), _bf16()
+    if shape != dst.shape or len(shape) not in (2, 3):
+        raise ValueError(f"rope_vecs: shapes {tuple(shape)} and {tuple(dst.shape)}")
+    if src.dtype is not bf16 or dst.dtype is not bf16 or a[-1] != 1 or b[-1] != 1:
         raise ValueError(f"rope_vecs: {src.dtype}, {dst.dtype}; bf16 tensors with a contiguous last axis")
-    if src.dim() == 2:
-        return src, dst, src.stride(0), 0, dst.stride(0), 0, 1
-    return src, dst, src.stride(0), src.stride(1), dst.stride(0), dst.stride(1), src.shape[1]
+    if len(shape) == 2:
+        return src, dst, a[0], 0, b[0], 0, 1
+    return src, dst, a[0], a[1], b[0], b[1], shape[1]
 
 
 def rope_frequencies(seg: int, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0, original: int = 4096,
