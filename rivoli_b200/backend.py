@@ -745,8 +745,10 @@ def rope_frequencies(seg: int, theta: float = 10000.0, scaling: str = "none", fa
     than ``beta_slow`` times over the original context, keeps those that turn more than ``beta_fast`` times, blends between, and
     scales by 0.1 ln(factor) + 1."""
     import numpy as np
-    if seg <= 0 or seg % 2 or theta <= 1 or factor < 1 or original < 1:
+    if seg <= 0 or seg % 2 or not (1 < theta < np.inf and 1 <= factor < np.inf and 1 <= original < np.inf):
         raise ValueError(f"rope_frequencies: seg {seg}, theta {theta}, factor {factor}, original {original}")
+    if not (0 < beta_slow < np.inf and 0 < beta_fast < np.inf):
+        raise ValueError(f"rope_frequencies: beta_fast {beta_fast}, beta_slow {beta_slow}")
     if scaling == "ntk":
         if seg < 4:
             raise ValueError("rope_frequencies: ntk needs two pairs")

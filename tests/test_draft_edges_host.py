@@ -75,3 +75,12 @@ def test_a_step_keeps_its_frequencies_in_64_bits(be):
         s = DraftStep(Stack(be), 4, (given, scale))
         assert s.inv_freq.dtype == torch.float64 and s.inv_freq.shape == (32,) and s.inv_freq.is_contiguous()
         assert torch.allclose(s.inv_freq, torch.from_numpy(f), rtol=1e-6)
+
+
+def test_frequencies_of_no_numbers(be):
+    """NaN, infinity and turns of zero or fewer gave frequencies that are NaN."""
+    nan, inf = float("nan"), float("inf")
+    for bad in (dict(theta=nan), dict(theta=inf), dict(factor=nan), dict(factor=inf), dict(original=nan), dict(original=inf), dict(beta_slow=0.0),
+                dict(beta_fast=-1.0), dict(beta_fast=nan)):
+        with pytest.raises(ValueError):
+            be.rope_frequencies(64, **{**dict(theta=10000.0, scaling="yarn", factor=4.0), **bad})
