@@ -599,7 +599,8 @@ int rivoli_rope_rows_bf16(const RopeVecs* q, const RopeVecs* k, int n_rows, cons
 
 /* Attention of all nodes of all trees: q bf16 [n_nodes][n_heads][kv_lora + rope_dim], out bf16 [n_nodes][n_heads][kv_lora], out_lse
  * f32 [n_nodes][n_heads] (may be NULL). A node of sequence b sees n_rows[b] rows of the prefix - rows u32 [B][row_stride], one list for
- * the whole tree (its root's selection, say), or with rows NULL the first n_rows[b] tokens, n_rows NULL meaning tree_pos[b] of them;
+ * the whole tree (its root's selection, say: in a model whose every token selects rows of its own the deeper nodes then see the root's
+ * and not theirs, and past top_k rows what such a tree accepts is no longer what steps of one token would give), or with rows NULL the first n_rows[b] tokens, n_rows NULL meaning tree_pos[b] of them;
  * a list that begins with the dense marker 0xFFFFFFFF stands for the first n_rows[b] tokens; what either names from tree_pos[b] on is of
  * the tree and not of the prefix, and is left out, so that the selection of the root may be made before or after its row is appended -
  * and node i of its own tree, whose row is
@@ -631,7 +632,7 @@ int rivoli_mla_tree_attend_status(const DsaGeom* g, void* scratch, void* stream)
  * Probabilities that are negative, infinite or NaN count as 0, and so does a token outside the vocabulary; a parent that is not an
  * earlier node is nobody's. Sums and comparisons in f64. path i32 [B][max_path]: the accepted nodes, ascending, from node 0 on, n_path[b]
  * of them (entries behind are left alone; once max_path are accepted no further child is tried); next i32 [B]. A sequence without nodes:
- * n_path 0, next -1. 1001 nulls or sizes; 1002 vocab > 2^20, max_path > 64; 1004 prob_bits; 1005 strides below vocab, alignment. */
+ * n_path 0, next -1. 1001 nulls or sizes; 1002 vocab > 2^20, max_path > 64, B > 65535; 1004 prob_bits; 1005 strides below vocab, alignment. */
 int rivoli_draft_verify(const int32_t* node_start, const int32_t* parent, const int32_t* token, const void* target,
                         long long target_stride, const void* draft, long long draft_stride, int prob_bits, int vocab, const float* u,
                         const float* u_next, int B, int32_t* path, int max_path, int32_t* n_path, int32_t* next, void* stream);
@@ -643,7 +644,7 @@ int rivoli_draft_verify(const int32_t* node_start, const int32_t* parent, const 
  * The paths are what rivoli_draft_verify writes: strictly ascending, path[b][k] >= k. A sequence whose path is not, or whose rows lie
  * on unmapped pages, is left as it is, seq_len included, and raises bit 0 of *status (device i32, may be NULL). Rows behind the path
  * are left as they were. Sequences must not share the pages that their drafts lie on.
- * 1001 nulls or sizes; 1002 path_stride > 64; 1003-1004 geometry; 1005 alignment, seq_len overlaps tree_pos, path, n_path or block_table. */
+ * 1001 nulls or sizes; 1002 path_stride > 64, B > 65535; 1003-1004 geometry; 1005 alignment, seq_len overlaps tree_pos, path, n_path or block_table. */
 typedef struct CommitLayer { uint8_t* latent_pool; float* latent_scale; uint8_t* index_pool; float* index_scale; } CommitLayer;
 int rivoli_kv_commit_paged(const DsaGeom* g, const CommitLayer* layers, int n_layers, const int32_t* block_table,
                            const int32_t* tree_pos, const int32_t* path, int path_stride, const int32_t* n_path, int B,

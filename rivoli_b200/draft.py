@@ -107,7 +107,8 @@ class DraftStep:
               stream=None) -> torch.Tensor:
         """Rows of layer ``i`` into its cache and attention of the tree: ``latent`` [n_nodes, kv_lora + rope], ``index_key``
         [n_nodes, index_dim] or None, ``q`` [n_nodes, heads, kv_lora + rope]. Every node sees the whole prefix, or, with ``selection`` (rows u32
-        [B, k], counts i32 [B]), those rows of it. Returns [n_nodes, heads, kv_lora]."""
+        [B, k], counts i32 [B]), those rows of it: the root's, say, in whose place deeper nodes would have selected their own. Returns
+        [n_nodes, heads, kv_lora], a buffer that the next layer writes again."""
         L, t, n = self.stack.layers[i], self.tree, self.tree.n_nodes
         g, bf16 = L.g, torch.bfloat16
         _fits("latent", latent, n, (g.kv_lora + g.rope_dim,), bf16)
