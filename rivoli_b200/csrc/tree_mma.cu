@@ -18,7 +18,7 @@
 //   * the loops are kept small: with every wait's loop in its place and the query conversion in one piece the kernel waited for its own
 //     instructions.
 // A pair of CTAs per block of 128 rows (cta_group::2, 1,105 cycles of products a tile against 1,400 here) was built and measured: 862 us
-// against 781 for 8 trees of up to 64 nodes x 16,384 rows alone, 982 against 900 back to back, where both are held by the power limit.
+// against 781 then for 8 trees of up to 64 nodes x 16,384 rows alone, 982 against 900 back to back, where both are held by the power limit.
 // Rows of the tree are tested against each node's mask in the tiles that hold them, the last one or two of a sequence. A hidden row's
 // weight is 0, but 0 x NaN is NaN: NaN codes of tree rows are fetched as 0, and the row makes scores NaN where it is seen. Rows that
 // nobody sees, for want of a page or of a scale above zero, are fetched as zeros altogether.
@@ -52,9 +52,10 @@ constexpr float TM_POFF = 5.0f, TM_MOST = 256.0f;    // P' = 2^(s - ref + 5) <= 
 // two and three nats, so that references often move, 14 and 47 %.
 constexpr float TM_FEW = 1.0f / 128, TM_LOST = 1.0f / 2048, TM_LOW = 2.0f, TM_LOW_AT = -6.0f, TM_SPARE = 2.0f, TM_ROOM = 35.0f, TM_LOWEST = -64.0f;
 constexpr int TM_MIN_TILES = 4;                      // tiles a CTA takes at least, while there are few: a CTA per block, or as many as that leaves
-// What a row block costs beside its tiles, in tiles: its queries, its output and the pipeline's ramp take 26,000 cycles, a tile 1,650. A
+// What a row block costs beside its tiles, in tiles: its queries, its output and the pipeline's ramp take 26,000 cycles, a tile some 1,900. A
 // run pays it for each block that it touches; the first is the same for all runs, so that the blocks that begin inside a run count
-// (32 trees over 512 to 8,192 rows: 383 us with runs of as many tiles, 280 with runs of equal cost; 31 nodes over 32,771 rows: 161 and 157).
+// (32 trees over 512 to 8,192 rows, when it was chosen: 383 us with runs of as many tiles, 280 with runs of equal cost; 31 nodes over
+// 32,771 rows: 161 and 157).
 constexpr int TM_BLOCK_COST = 16;
 
 // tensor memory columns
